@@ -48,8 +48,9 @@ int qmv_set_device(int device);
 /* Device status of the current device: bit 0 = a consumer's pipeline wait
  * expired, bit 1 = a producer's wait expired, bit 2 = draining in-flight
  * copies timed out, bit 3 = a peer's exchange flag never arrived, bit 4 = a
- * tensor-core matmul's wait for its MMAs expired.  0 means every bounded
- * wait completed.  clear != 0 resets the word.  No counterpart in the reference (its kernels never wait). */
+ * tensor-core matmul's wait for its MMAs expired, bit 5 = an attention or
+ * append call met a row start, length or page index out of range.  0 means
+ * every bounded wait completed and all metadata was in range.  clear != 0 resets the word.  No counterpart in the reference (its kernels never wait). */
 int qmv_device_status(uint32_t *flags, int clear);
 
 /* GEMV kernel selection for the calling process: 0 = automatic (the
@@ -371,6 +372,92 @@ typedef struct QmvOperationProfile {
  * weight matrices as the reference's per-matrix matvec calls do. */
 int qmv_qwen2_forward_profiled(QmvQwen2 *decoder, int token, float *logits, int *next_token,
                                QmvOperationProfile *profile);
+
+/* ---- attention of many sequences -----------------------------------------
+ * Causal grouped-query attention (transformer_attention_f32,
+ * src/transformer_ops.cpp:71-161) and its rotary embedding and cache append
+ * (src/transformer_ops.cpp:43-69, src/qwen2_architecture.cpp:1302-1343) for a
+ * ragged batch: the tokens of all sequences lie one after another in rows,
+ * sequence s owning rows [start[s], start[s + 1]).  The reference runs one
+ * sequence over one contiguous f32 cache; these serve many requests at once.
+ *
+ * Rows: row r of q holds heads * head_dim elements at q + r * q_ld, of k and v
+ * kv_heads * head_dim (so q, k and v may be slices of one [q | k | v] row);
+ * the *_ld are in elements.  Every row starts on a 16-byte boundary.  Query
+ * head a reads key/value head a / (heads / kv_heads).  head_dim is 64 or 128
+ * and heads / kv_heads at most 64.  Outputs may not overlap inputs except where said.
+ *
+ * Types are GGML type ids: QMV_TYPE_F32, QMV_TYPE_F16, QMV_TYPE_BF16.
+ * Sums, the softmax and its statistics are f32 whatever the types; the
+ * softmax's weights meet the values in the 16-bit type of the values (f32
+ * activations: in pairs of f16, 22 bits).
+ *
+ * Row starts, lengths and page tables are read on the device, so a captured
+ * graph can be replayed after they change; the counts passed by the host stay.
+ * Starts must ascend within 0..tokens; a call whose starts do not leaves its
+ * rows undefined.  A sequence whose length is not in 0..max_pages * page_size
+ * is left out: its rows stay as they were.  A page index outside
+ * 0..page_count - 1 is never followed; the rows that would need it are then
+ * undefined.  Each of these sets bit 5 of qmv_device_status, and nothing
+ * outside the named buffers is read or written. */
+#define QMV_TYPE_F32 0u
+#define QMV_TYPE_F16 1u
+#define QMV_TYPE_BF16 30u
+
+/* One layer's keys and values in pages: position p of a page, key/value head
+ * h, element e lies at page * page_stride + p * position_stride +
+ * h * head_stride + e (in elements; all three strides multiples of 8, both
+ * bases 16-byte aligned).  [page][position][head] and [page][head][position]
+ * are both expressible.  type: F16 (with f32 or f16 activations) or BF16 (with bf16).
+ * page_size: 16, 32, 64, 128 or 256 positions. */
+typedef struct QmvPagedCache {
+    void *keys, *values; /* device */
+    uint32_t type;
+    int kv_heads, head_dim;
+    int page_size, page_count;
+    int64_t page_stride, position_stride, head_stride;
+} QmvPagedCache;
+
+/* The new tokens of a step.  length[s] counts the cached positions of
+ * sequence s with its new tokens, so token i of its n tokens has position
+ * length[s] - n + i; position p lives in page
+ * page_table[s * max_pages + p / page_size].  max_query: about how many new
+ * tokens the longest sequence has (chooses the kernel; any value gives the same function). */
+typedef struct QmvPagedBatch {
+    const int *query_start; /* device, sequences + 1 */
+    const int *length;      /* device, sequences */
+    const int *page_table;  /* device, sequences * max_pages */
+    int sequences, tokens, max_pages, max_query;
+} QmvPagedBatch;
+
+/* Rotary embedding of the new tokens' queries and keys at their positions,
+ * and the append of keys and values to the cache.  rope_base >= 1: element i
+ * and i + head_dim / 2 turn by position * rope_base^(-2i / head_dim) (formed
+ * to 64 bits of a turn, so far positions lose nothing); rope_base = 0: no
+ * rotation.  q_out (may be q itself with q_out_ld = q_ld; null: q is not
+ * read) and k_out (null, or k itself with k_out_ld = k_ld) receive the rotated rows
+ * in the activations' type, for qmv_packed_attention.  A token at a negative
+ * position (more new tokens than length) is skipped.  Two tokens of one call
+ * must not have the same cache slot. */
+int qmv_paged_append(const QmvPagedCache *cache, const QmvPagedBatch *batch, uint32_t type, int heads, const void *q,
+                     int64_t q_ld, const void *k, int64_t k_ld, const void *v, int64_t v_ld, float rope_base,
+                     void *q_out, int64_t q_out_ld, void *k_out, int64_t k_out_ld, void *stream);
+
+/* out[row] = causal attention of each token over its sequence's earlier
+ * tokens and itself, whole prompts without a cache.  start: device,
+ * sequences + 1.  scale multiplies q . k; 0 means 1 / sqrt(head_dim).  Rows
+ * behind the last sequence are left as they were.  Masked places may hold
+ * anything, NaN and infinities too.  q, k, v and out share one type. */
+int qmv_packed_attention(uint32_t type, int heads, int kv_heads, int head_dim, const int *start, int sequences,
+                         int tokens, const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *v,
+                         int64_t v_ld, void *out, int64_t out_ld, float scale, void *stream);
+
+/* out[row] = causal attention of each new token over the cached positions up
+ * to its own (append first).  One token a sequence is a decode step, more are
+ * a chunk of a prompt or a draft; a batch may hold both.  A token at a
+ * negative position has no keys: its row becomes 0. */
+int qmv_paged_attention(const QmvPagedCache *cache, const QmvPagedBatch *batch, uint32_t type, int heads,
+                        const void *q, int64_t q_ld, void *out, int64_t out_ld, float scale, void *stream);
 
 /* ---- GGUF model images ---------------------------------------------------
  * The reference opens a model with gguf_open (src/gguf_reader.h:71,

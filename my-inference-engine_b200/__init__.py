@@ -58,6 +58,7 @@ C_SYMBOLS = [
     "qmv_qwen2_reset", "qmv_qwen2_stream", "qmv_matmul_residual", "qmv_gguf_get_bool",
     "qmv_gguf_array_cursor_init", "qmv_gguf_array_next_string", "qmv_gguf_array_next_uint",
     "qmv_gguf_array_next_int", "qmv_gguf_f32_view",
+    "qmv_paged_append", "qmv_packed_attention", "qmv_paged_attention",
 ]
 CXX_DROPIN_SYMBOLS = {
     "quantized_tensor_matvec_f32": "_Z27quantized_tensor_matvec_f32PK23GgufQuantizedTensorViewPKfiPfi",
@@ -165,6 +166,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         raise RuntimeError(f"{path} is missing: build it with my-inference-engine_b200/build.py")
     lib = ctypes.CDLL(path)
     P, I, U32, U64, SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_size_t
+    I64 = ctypes.c_int64
     IP = ctypes.POINTER(ctypes.c_int)
     VP = ctypes.POINTER(GgufQuantizedTensorView)
     sigs = {
@@ -241,6 +243,9 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "qmv_qwen2_prefill": (I, [P, P, I, P, IP]),
         "qmv_qwen2_reset": (I, [P]),
         "qmv_qwen2_stream": (I, [P, ctypes.POINTER(P)]),
+        "qmv_paged_append": (I, [P, P, U32, I, P, I64, P, I64, P, I64, ctypes.c_float, P, I64, P, I64, P]),
+        "qmv_packed_attention": (I, [U32, I, I, I, P, I, I, P, I64, P, I64, P, I64, P, I64, ctypes.c_float, P]),
+        "qmv_paged_attention": (I, [P, P, U32, I, P, I64, P, I64, ctypes.c_float, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -797,6 +802,81 @@ class GgufFile:
 
     def __exit__(self, *exc):
         self.close()
+
+
+# --------------------------------------------- attention of many sequences
+
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30  # GGML type ids of activations and caches
+
+
+class QmvPagedCache(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("type", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("page_count", ctypes.c_int), ("page_stride", ctypes.c_int64), ("position_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class QmvPagedBatch(ctypes.Structure):
+    _fields_ = [("query_start", ctypes.c_void_p), ("length", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("sequences", ctypes.c_int), ("tokens", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("max_query", ctypes.c_int)]
+
+
+class PagedCache:
+    """One layer's keys and values in pages (QmvPagedCache).  ``keys`` and
+    ``values`` are device buffers the caller keeps; strides are in elements,
+    by default those of [page][position][head][head_dim]."""
+
+    def __init__(self, keys, values, ggml_type: int, kv_heads: int, head_dim: int, page_size: int, page_count: int,
+                 page_stride: int | None = None, position_stride: int | None = None, head_stride: int | None = None):
+        self._keep = (keys, values)
+        row = kv_heads * head_dim
+        self.c = QmvPagedCache(_ptr(keys), _ptr(values), ggml_type, kv_heads, head_dim, page_size, page_count,
+                               page_size * row if page_stride is None else page_stride,
+                               row if position_stride is None else position_stride,
+                               head_dim if head_stride is None else head_stride)
+        self._ref = ctypes.addressof(self.c)
+
+
+class PagedBatch:
+    """The new tokens of one step (QmvPagedBatch): device int32 buffers
+    ``query_start`` [sequences + 1], ``length`` [sequences] and ``page_table``
+    [sequences][max_pages].  ``max_query``: new tokens of the longest sequence
+    (by default all of them); only chooses the kernel."""
+
+    def __init__(self, query_start, length, page_table, sequences: int, tokens: int, max_pages: int,
+                 max_query: int | None = None):
+        self._keep = (query_start, length, page_table)
+        self.c = QmvPagedBatch(_ptr(query_start), _ptr(length), _ptr(page_table), sequences, tokens, max_pages,
+                               tokens if max_query is None else max_query)
+        self._ref = ctypes.addressof(self.c)
+
+
+def paged_append(cache: PagedCache, batch: PagedBatch, ggml_type: int, heads: int, q, q_ld: int, k, k_ld: int, v,
+                 v_ld: int, rope_base: float = 0.0, q_out=None, q_out_ld: int = 0, k_out=None, k_out_ld: int = 0,
+                 stream=None):
+    """Rotary embedding of the new tokens' queries and keys, and their keys and
+    values written to the cache's pages (qmv_paged_append)."""
+    _check(lib().qmv_paged_append(cache._ref, batch._ref, ggml_type, heads, _ptr(q), q_ld, _ptr(k), k_ld, _ptr(v),
+                                  v_ld, rope_base, _ptr(q_out), q_out_ld, _ptr(k_out), k_out_ld, _ptr(stream)),
+           "qmv_paged_append")
+
+
+def packed_attention(ggml_type: int, heads: int, kv_heads: int, head_dim: int, start, sequences: int, tokens: int,
+                     q, q_ld: int, k, k_ld: int, v, v_ld: int, out, out_ld: int, scale: float = 0.0, stream=None):
+    """Causal grouped-query attention over packed whole prompts
+    (qmv_packed_attention); ``start``: device int32 [sequences + 1]."""
+    _check(lib().qmv_packed_attention(ggml_type, heads, kv_heads, head_dim, _ptr(start), sequences, tokens, _ptr(q),
+                                      q_ld, _ptr(k), k_ld, _ptr(v), v_ld, _ptr(out), out_ld, scale, _ptr(stream)),
+           "qmv_packed_attention")
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, ggml_type: int, heads: int, q, q_ld: int, out, out_ld: int,
+                    scale: float = 0.0, stream=None):
+    """Causal grouped-query attention of the new tokens over the paged cache
+    (qmv_paged_attention); append their keys and values first."""
+    _check(lib().qmv_paged_attention(cache._ref, batch._ref, ggml_type, heads, _ptr(q), q_ld, _ptr(out), out_ld,
+                                     scale, _ptr(stream)), "qmv_paged_attention")
 
 
 def set_profiling(enabled: bool) -> None:

@@ -7,6 +7,7 @@ library can be loaded next to torch's own runtime.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -16,8 +17,11 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libqmv_b200.so")
 
-SOURCES = ["qmv_kernels.cu", "qmv_capi.cpp", "qmv_qwen2.cpp", "qmv_gguf.cpp", "quantized_matvec.cpp"]
-HEADERS = ["qmv_internal.h"]
+OBJ_DIR = os.path.join(PKG_DIR, "build")
+
+SOURCES = ["qmv_kernels.cu", "qmv_capi.cpp", "qmv_qwen2.cpp", "qmv_gguf.cpp", "quantized_matvec.cpp",
+           "qmv_attention.cu", "qmv_attention_capi.cpp"]
+HEADERS = ["qmv_internal.h", "qmv_attention.h"]
 PUBLIC_HEADERS = ["qmv_b200.h", "quantized_matvec.h", "gguf_quantized_view.h"]
 
 NVCC_FLAGS = [
@@ -27,7 +31,6 @@ NVCC_FLAGS = [
     "-lineinfo",
     "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall",
     "-Xptxas", "-v",
-    "-shared",
 ]
 
 
@@ -51,22 +54,44 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(f) <= t for f in _inputs())
 
 
+def _compile(source: str, force: bool):
+    """One source to its object (skipped when newer than the source and every
+    header); (object, nvcc's messages)."""
+    src, obj = os.path.join(CSRC, source), os.path.join(OBJ_DIR, source + ".o")
+    log = obj + ".log"
+    deps = [src] + [f for f in _inputs() if f.endswith(".h")] + [os.path.abspath(__file__)]
+    if not force and os.path.exists(obj) and os.path.exists(log) and \
+            all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in deps):
+        with open(log) as fh:
+            return obj, fh.read()
+    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO_DIR, "include"), "-I", CSRC, "-c", src, "-o", obj]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+    with open(log, "w") as fh:
+        fh.write(proc.stderr)
+    return obj, proc.stderr
+
+
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile libqmv_b200.so in place (skipped when up to date)."""
+    """Compile libqmv_b200.so in place (skipped when up to date), the sources
+    side by side."""
     if not force and up_to_date():
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO_DIR, "include"), "-I", CSRC,
-           "-o", LIB_PATH + ".tmp",
-           *[os.path.join(CSRC, s) for s in SOURCES],
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+        built = list(pool.map(lambda s: _compile(s, force), SOURCES))
+    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH + ".tmp", *[obj for obj, _ in built],
            "-Xlinker", "--exclude-libs,ALL"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+    messages = "".join(m for _, m in built)
     if verbose:
-        sys.stderr.write(proc.stderr)
+        sys.stderr.write(messages)
     os.replace(LIB_PATH + ".tmp", LIB_PATH)
     with open(os.path.join(PKG_DIR, "ptxas_report.txt"), "w") as fh:
-        fh.write(proc.stderr)
+        fh.write(messages)
     return LIB_PATH
 
 

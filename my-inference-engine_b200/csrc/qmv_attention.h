@@ -1,0 +1,56 @@
+// Internal interface between the attention entry points
+// (qmv_attention_capi.cpp) and their sm_100a kernels (qmv_attention.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace qmv {
+
+enum : uint32_t { kTypeF32 = 0u, kTypeF16 = 1u, kTypeBF16 = 30u };
+constexpr int kMaxGroup = 64;  // query heads per key/value head
+
+// Where a sequence's keys and values lie, in elements.  Paged: position p of
+// sequence s is row p & (page_size - 1) of page table[s * max_pages +
+// (p >> page_shift)].  Packed (table null): row start[s] + p, the position strides
+// being k_pos and v_pos.
+struct KvView {
+    const void *k, *v;
+    int64_t k_pos, v_pos;  // between positions
+    int64_t page, head;    // between pages, between heads
+    const int *table;
+    int max_pages, page_shift, page_count;
+};
+
+struct AttnArgs {
+    uint32_t type, kv_type;
+    const void *q;
+    void *out;
+    int64_t q_ld, out_ld;
+    KvView kv;
+    const int *start;   // [sequences + 1]
+    const int *length;  // [sequences]; null: a sequence's own tokens are its keys
+    int sequences, tokens, heads, kv_heads, group, head_dim;
+    int max_query;
+    float scale;  // multiplies q . k
+};
+
+struct AppendArgs {
+    uint32_t type, kv_type;
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    int64_t q_ld, k_ld, v_ld, q_out_ld, k_out_ld;
+    KvView kv;  // k / v: the cache's pages (written)
+    const int *start, *length;
+    int sequences, tokens, heads, kv_heads, head_dim;
+    float rope_base;
+};
+
+cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s);
+cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s);
+
+// Status bits of the attention kernels on the current device.
+enum : unsigned int { kStatusBadMetadata = 32u };
+cudaError_t attention_status(unsigned int *out, bool clear);
+
+}  // namespace qmv

@@ -18,6 +18,7 @@
 #include <string>
 #include <tuple>
 
+#include "qmv_attention.h"
 #include "qmv_b200.h"
 #include "qmv_internal.h"
 
@@ -327,7 +328,9 @@ QMV_EXPORT int qmv_device_status(uint32_t *flags, int clear)
     if (flags == nullptr) return fail("flags pointer is null");
     unsigned int v = 0;
     QMV_CUDA(qmv::read_status(&v, clear != 0), "read device status");
-    *flags = v;
+    unsigned int attention = 0;
+    QMV_CUDA(qmv::attention_status(&attention, clear != 0), "read device status");
+    *flags = v | attention;
     return 1;
 }
 
