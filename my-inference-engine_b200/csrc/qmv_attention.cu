@@ -234,18 +234,20 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
 // ------------------------------------------------------ attention by rows
 //
 // One warp computes one (token, query head) in f32 on the CUDA cores: a lane
-// a key for the scores, a lane D / 32 elements for the output.  Masked keys
-// are never read.
+// a key for the scores, a lane D / 32 elements for the output, of which
+// columns [col0, col1) are written.  Masked keys are never read.  The faster
+// kernels come back to it for rows that are not finite: a masked key's weight
+// of 0 times a NaN or infinite value must not reach a sum, and theirs does.
 
 template <typename T, typename KT, int D>
-__device__ void attention_row(const AttnArgs &a, int row, int head, int s, const Seq &sq, float *qs)
+__device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head, int s, const Seq &sq, float *qs, int col0, int col1)
 {
     constexpr int V = Elem<KT>::kVec, E = D / 32;
     const int lane = threadIdx.x & 31, h = head / a.group;
     const int n_keys = sq.keys - sq.n + (row - sq.row0) + 1;
     T *out = (T *)a.out + (int64_t)row * a.out_ld + head * D;
     if (n_keys <= 0) {
-        for (int e = lane; e < D; e += 32) out[e] = Elem<T>::from_float(0.f);
+        for (int e = col0 + lane; e < col1; e += 32) out[e] = Elem<T>::from_float(0.f);
         return;
     }
     const T *q = (const T *)a.q + (int64_t)row * a.q_ld + head * D;
@@ -316,7 +318,8 @@ __device__ void attention_row(const AttnArgs &a, int row, int head, int s, const
         }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e * 32 + lane] = Elem<T>::from_float(o[e] / l);
+    for (int e = 0; e < E; ++e)
+        if (e * 32 + lane >= col0 && e * 32 + lane < col1) out[e * 32 + lane] = Elem<T>::from_float(o[e] / l);
 }
 
 constexpr int kRowWarps = 4;
@@ -330,7 +333,589 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(AttnArgs
     const int s = find_sequence(a.start, a.sequences, row);
     const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
     if (row < sq.row0 || row >= sq.row0 + sq.n || head >= a.heads) return;
-    attention_row<T, KT, D>(a, row, head, s, sq, qs[warp]);
+    attention_row<T, KT, D>(a, row, head, s, sq, qs[warp], 0, D);
+}
+
+// ------------------------------------------------- paged decode attention
+//
+// Few query rows over many cached keys: bound by the bytes of the cache, each
+// read once for all the query heads of its key/value head.
+//
+// Rows r = token * group + head-in-group of one (sequence, key/value head)
+// are cut into tiles of 16, the M of mma.sync m16n8k16; a row tile of one
+// sequence and head is an item, its keys in blocks of 128 are its units, and
+// all units of the launch, in order, are dealt evenly to the CTAs (one an
+// SM), so ragged lengths cost nothing.  Each of the 8 warps takes 16 keys of
+// every unit, streams them through its own cp.async ring (the rings together
+// keep 128 KB a CTA in flight, with no barrier between warps) and holds its
+// own running maximum, sum and output in registers; the warps meet once per
+// item.  An item that ends up in more than one CTA leaves partials (maximum,
+// sum, unnormalised output) that decode_merge_kernel joins in order.
+// tcgen05 is not used: its M of 64 or more would be mostly empty rows here,
+// and the tensor work is a tenth of the time the bytes take.
+
+constexpr int kDcWarps = 8;
+constexpr int kDcThreads = kDcWarps * 32;
+constexpr int kDcKeys = 16;                   // keys of a warp's step
+constexpr int kDcUnit = kDcKeys * kDcWarps;   // keys of a unit
+constexpr int kDcRows = 16;                   // rows of a tile
+
+template <int D> struct Dc {
+    static constexpr uint32_t kRow = D * 2;                    // bytes of a key
+    static constexpr uint32_t kStep = 2 * kDcKeys * kRow;      // K and V of a step
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr uint32_t kRing = kStep * kStages * kDcWarps;
+    static constexpr uint32_t kMerge = kDcWarps * kDcRows * (D / 2) * 4;
+    static constexpr uint32_t kSmem = kRing + kMerge + kDcWarps * kDcRows * 8;
+    static constexpr int kPartial = kDcRows * D + 2 * kDcRows;  // floats: o, m, l
+    // half rows of D / 2 floats, 8-float blocks exchanged by the row so that
+    // the 8 rows a warp writes at once fall on different banks
+    static __device__ __forceinline__ int at(int row, int col) { return row * (D / 2) + (col ^ ((row & (D / 16 - 1)) * 8)); }
+};
+
+// 2^x (2 ulp; results below 2^-126 become 0).
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+__device__ __forceinline__ void ldsm4t(uint32_t r[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+template <typename KT> __device__ __forceinline__ void mma16816(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (sizeof(KT) == 2 && std::is_same<KT, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename KT> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    uint32_t w;
+    if constexpr (std::is_same<KT, __half>::value)
+        *(__half2 *)&w = __floats2half2_rn(a, b);
+    else
+        *(__nv_bfloat162 *)&w = __floats2bfloat162_rn(a, b);
+    return w;
+}
+
+// What is left of (a, b) after their f16 rounding, as f16.
+__device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t hi)
+{
+    const float2 h = __half22float2(*(const __half2 *)&hi);
+    return pack2<__half>(a - h.x, b - h.y);
+}
+
+// Units of one sequence: key blocks x row tiles x heads.
+struct DcPlan {
+    const int *start, *length;
+    int sequences, tokens, max_keys, kv_heads, group;
+    __device__ __forceinline__ Seq seq(int s) const { return load_sequence(start, length, s, tokens, max_keys); }
+    __device__ __forceinline__ int tiles(const Seq &q) const { return (q.n * group + kDcRows - 1) / kDcRows; }
+    __device__ __forceinline__ int blocks(const Seq &q) const { return q.keys > 0 ? (q.keys + kDcUnit - 1) / kDcUnit : 1; }
+    __device__ __forceinline__ long long units(const Seq &q) const { return (long long)tiles(q) * kv_heads * blocks(q); }
+};
+
+// Sum over the CTA of one value a thread, and the exclusive prefix.
+__device__ __forceinline__ long long block_scan(long long v, long long *total, long long *scratch)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, d);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kDcWarps; ++w) {
+        if (w < warp) before += scratch[w];
+        all += scratch[w];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+struct Found {
+    int s;          // sequence
+    long long rel;  // unit within it
+};
+
+// All units of the launch, then the sequence of unit share(total) (by every
+// thread of the CTA together).
+template <typename F> __device__ Found find_unit(const DcPlan &p, long long *scratch, long long *total, const F &share)
+{
+    __shared__ Found found;
+    long long all = 0, v = 0, before = 0;
+    for (int s0 = 0; s0 < p.sequences; s0 += kDcThreads) {
+        const int s = s0 + (int)threadIdx.x;
+        v = s < p.sequences ? p.units(p.seq(s)) : 0;
+        long long t;
+        before = block_scan(v, &t, scratch);
+        all += t;
+    }
+    *total = all;
+    const long long want = share(all);
+    if (threadIdx.x == 0) found = Found{p.sequences, 0};
+    if (p.sequences <= kDcThreads) {  // this thread's sequence is still at hand
+        __syncthreads();
+        if (want >= before && want < before + v) found = Found{(int)threadIdx.x, want - before};
+    } else {
+        long long base = 0;
+        for (int s0 = 0; s0 < p.sequences && base <= want; s0 += kDcThreads) {
+            const int s = s0 + (int)threadIdx.x;
+            v = s < p.sequences ? p.units(p.seq(s)) : 0;
+            long long t;
+            before = base + block_scan(v, &t, scratch);
+            if (want >= before && want < before + v) found = Found{s, want - before};
+            base += t;
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
+// Walks units in order: sequence, head, row tile, key block.
+struct DcIter {
+    Seq q;
+    int s, h, rt, blk, rts, blks;
+    __device__ __forceinline__ void enter(const DcPlan &p)
+    {
+        rts = blks = 0;
+        while (s < p.sequences) {
+            q = p.seq(s);
+            rts = p.tiles(q);
+            blks = p.blocks(q);
+            if (rts > 0) break;
+            ++s;
+        }
+    }
+    __device__ __forceinline__ void begin(const DcPlan &p, int s_, long long rel)
+    {
+        s = s_;
+        enter(p);
+        blk = blks ? (int)(rel % blks) : 0;
+        const int item = blks ? (int)(rel / blks) : 0;
+        rt = rts ? item % rts : 0;
+        h = rts ? item / rts : 0;
+    }
+    __device__ __forceinline__ void next(const DcPlan &p)
+    {
+        if (++blk < blks) return;
+        blk = 0;
+        if (++rt < rts) return;
+        rt = 0;
+        if (++h < p.kv_heads) return;
+        h = 0;
+        ++s;
+        enter(p);
+    }
+};
+
+// Writes 4 columns of an output row; true when one is not finite.
+template <typename T> __device__ __forceinline__ bool store4(T *out, const float4 &v)
+{
+    if constexpr (sizeof(T) == 4) {
+        *(float4 *)out = v;
+    } else {
+        *(uint2 *)out = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    }
+    return !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+}
+
+template <typename T, typename KT, int D>
+__global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ partials)
+{
+    using C = Dc<D>;
+    constexpr int NQ = sizeof(T) == 4 ? 2 : 1;  // f16 pairs for f32 activations
+    constexpr int KS = D / 16, NT = D / 8;
+    // the weights' exponent offset: f16 weights down to 2^-22 stay normal
+    constexpr float kLift = std::is_same<KT, __half>::value ? 8.f : 0.f;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long scratch[kDcWarps];
+    __shared__ unsigned bad_rows;
+    float *merge = (float *)(smem + C::kRing);
+    float2 *ml = (float2 *)(smem + C::kRing + C::kMerge);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, grp = lane >> 2;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
+    if (blockIdx.x == 0) check_metadata(a.start, a.length, a.sequences, a.tokens, plan.max_keys);
+    if (tid == 0) bad_rows = 0u;
+    long long total;
+    const Found f = find_unit(plan, scratch, &total, [&](long long n) { return n * blockIdx.x / gridDim.x; });
+    const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
+    if (u0 >= u1) return;
+
+    DcIter pf, it;
+    it.begin(plan, f.s, f.rel);
+    pf = it;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)warp * C::kStep * C::kStages;
+    const int mask = (1 << a.kv.page_shift) - 1;
+
+    // the page of the next step to fetch, loaded one step ahead of its use
+    auto page_of = [&](const DcIter &i) {
+        const int j0 = i.blk * kDcUnit + warp * kDcKeys;
+        return j0 < i.q.keys ? __ldg(a.kv.table + (int64_t)i.s * a.kv.max_pages + (j0 >> a.kv.page_shift)) : -1;
+    };
+    long long fetched = u0;
+    int page = page_of(pf);
+    auto issue = [&]() {
+        if (fetched < u1) {
+            const int j0 = pf.blk * kDcUnit + warp * kDcKeys;
+            if (j0 < pf.q.keys) {
+                const bool good = page >= 0 && page < a.kv.page_count;
+                if (!good && lane == 0) report(kStatusBadMetadata);
+                const int64_t base = (int64_t)(good ? page : 0) * a.kv.page + (int64_t)(j0 & mask) * a.kv.k_pos + (int64_t)pf.h * a.kv.head;
+                const KT *k = (const KT *)a.kv.k + base, *v = (const KT *)a.kv.v + base;
+                const uint32_t dst = ring + ((uint32_t)(fetched - u0) % C::kStages) * C::kStep;
+                constexpr int CH = D / 8;  // 16-byte pieces of a key
+                const int c = lane % CH;
+#pragma unroll
+                for (int r0 = 0; r0 < kDcKeys; r0 += 32 / CH) {
+                    const int r = r0 + lane / CH;
+                    const bool live = good && j0 + r < pf.q.keys;
+                    const int64_t off = live ? (int64_t)r * a.kv.k_pos + c * 8 : 0;
+                    const uint32_t to = dst + (uint32_t)r * C::kRow + (uint32_t)((c ^ (r & 7)) * 16);
+                    cp16(to, k + off, live);
+                    cp16(to + kDcKeys * C::kRow, v + off, live);
+                }
+            }
+            ++fetched;
+            pf.next(plan);
+            if (fetched < u1) page = page_of(pf);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int i = 0; i < C::kStages - 1; ++i) issue();
+
+    uint32_t qf[NQ][KS][4];
+    float o[NT][4], m[2], l[2], factor[2];
+    int lim[2];
+    long long seg = u0;  // first unit of the current segment
+    for (long long u = u0; u < u1; ++u) {
+        if (u == seg) {
+            // the item's query rows as A fragments: rows grp and grp + 8
+            const int rows = it.q.n * a.group - it.rt * kDcRows;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = it.rt * kDcRows + grp + 8 * half, token = r / a.group;
+                const bool live = grp + 8 * half < rows;
+                lim[half] = live ? it.q.keys - it.q.n + token + 1 : 0;
+                const T *q = (const T *)a.q + (int64_t)(it.q.row0 + (live ? token : 0)) * a.q_ld +
+                             (int64_t)(it.h * a.group + (live ? r - token * a.group : 0)) * D;
+                m[half] = -INFINITY;
+                l[half] = 0.f;
+                factor[half] = a.scale * kLog2e;
+                if constexpr (NQ == 1) {
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        qf[0][k][half] = live ? *(const uint32_t *)(q + 16 * k + 2 * quad) : 0u;
+                        qf[0][k][2 + half] = live ? *(const uint32_t *)(q + 16 * k + 8 + 2 * quad) : 0u;
+                    }
+                } else {
+                    // x = (hi + lo) 2^-e with the row's largest |x| in
+                    // [2^14, 2^15) after the shift: 22 bits a value
+                    float2 x[KS][2];
+                    float big = 0.f;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            x[k][p] = live ? *(const float2 *)(q + 16 * k + 8 * p + 2 * quad) : make_float2(0.f, 0.f);
+                            big = fmaxf(big, fmaxf(fabsf(x[k][p].x), fabsf(x[k][p].y)));
+                        }
+                    big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
+                    int e = 14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127;
+                    e = min(max(e, -100), 100);
+                    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                    factor[half] *= __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            const float y0 = x[k][p].x * up, y1 = x[k][p].y * up;
+                            const uint32_t hi = pack2<__half>(y0, y1);
+                            qf[0][k][2 * p + half] = hi;
+                            qf[NQ - 1][k][2 * p + half] = pack2_rest(y0, y1, hi);
+                        }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 2) : "memory");
+        __syncwarp();
+        issue();  // refills the stage read in the previous step
+        const int j0 = it.blk * kDcUnit + warp * kDcKeys;
+        if (j0 < it.q.keys) {
+            const uint32_t ks = ring + ((uint32_t)(u - u0) % C::kStages) * C::kStep, vs = ks + kDcKeys * C::kRow;
+            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), c0 = (lane >> 3) & 1;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t b[4];
+                    ldsm4(b, ks + (uint32_t)r * C::kRow + (uint32_t)(((2 * k + c0) ^ (r & 7)) * 16));
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        mma16816<KT>(sc[0], qf[n][k], b[0], b[1]);
+                        mma16816<KT>(sc[1], qf[n][k], b[2], b[3]);
+                    }
+                }
+            }
+            float p[2][4];
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int half = e >> 1, j = j0 + 8 * t + 2 * quad + (e & 1);
+                    p[t][e] = j < lim[half] ? sc[t][e] * factor[half] : -INFINITY;
+                    top[half] = fmaxf(top[half], p[t][e]);
+                }
+            float base[2];
+            bool raised = false;
+            float fix[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                top[half] = fmaxf(top[half], __shfl_xor_sync(kFull, top[half], 1));
+                top[half] = fmaxf(top[half], __shfl_xor_sync(kFull, top[half], 2));
+                const float mn = fmaxf(m[half], top[half]);
+                base[half] = mn == -INFINITY ? 0.f : mn - kLift;
+                fix[half] = m[half] == -INFINITY ? 1.f : ex2(m[half] - mn);
+                raised |= mn > m[half];
+                m[half] = mn;
+            }
+            if (__any_sync(kFull, raised)) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    l[half] *= fix[half];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        o[t][2 * half] *= fix[half];
+                        o[t][2 * half + 1] *= fix[half];
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[t][e] = ex2(p[t][e] - base[e >> 1]);
+                    l[e >> 1] += p[t][e];
+                }
+            uint32_t pa[NQ][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = e >> 1, half = e & 1;
+                pa[0][e] = pack2<KT>(p[t][2 * half], p[t][2 * half + 1]);
+                if constexpr (NQ == 2) pa[1][e] = pack2_rest(p[t][2 * half], p[t][2 * half + 1], pa[0][e]);
+            }
+            {
+                const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c0 = lane >> 4;
+#pragma unroll
+                for (int t = 0; t < NT; t += 2) {
+                    uint32_t b[4];
+                    ldsm4t(b, vs + (uint32_t)r * C::kRow + (uint32_t)(((t + c0) ^ (r & 7)) * 16));
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        mma16816<KT>(o[t], pa[n], b[0], b[1]);
+                        mma16816<KT>(o[t + 1], pa[n], b[2], b[3]);
+                    }
+                }
+            }
+        }
+        const bool last_block = it.blk + 1 == it.blks;
+        if (last_block || u + 1 == u1) {
+            // the warps' shares of the segment meet in shared memory, half of
+            // the columns at a time
+            const bool whole = last_block && u - it.blk >= u0;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                l[half] += __shfl_xor_sync(kFull, l[half], 1);
+                l[half] += __shfl_xor_sync(kFull, l[half], 2);
+                if (quad == 0) ml[warp * kDcRows + grp + 8 * half] = make_float2(m[half], l[half]);
+            }
+            __syncthreads();
+            float top[2], mine[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                top[half] = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kDcWarps; ++w) top[half] = fmaxf(top[half], ml[w * kDcRows + grp + 8 * half].x);
+                mine[half] = m[half] == -INFINITY ? 0.f : ex2(m[half] - top[half]);
+            }
+            const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
+            // a partial that starts inside its item goes to the first slot
+            float *part = partials + (size_t)(2 * blockIdx.x + (u - it.blk >= u0 ? 1 : 0)) * C::kPartial;
+#pragma unroll
+            for (int hc = 0; hc < 2; ++hc) {
+#pragma unroll
+                for (int t = 0; t < NT / 2; ++t)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+                        *(float2 *)(merge + C::at(warp * kDcRows + grp + 8 * half, 8 * t + 2 * quad)) =
+                            make_float2(o[hc * NT / 2 + t][2 * half] * mine[half], o[hc * NT / 2 + t][2 * half + 1] * mine[half]);
+                __syncthreads();
+                constexpr int C4 = D / 8;  // float4 columns of half a row
+                for (int i = tid; i < rows * C4; i += kDcThreads) {
+                    const int r = i / C4, c = (i % C4) * 4;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float big = -INFINITY, den = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kDcWarps; ++w) big = fmaxf(big, ml[w * kDcRows + r].x);
+#pragma unroll
+                    for (int w = 0; w < kDcWarps; ++w) {
+                        const float4 x = *(const float4 *)(merge + C::at(w * kDcRows + r, c));
+                        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+                        const float2 y = ml[w * kDcRows + r];
+                        den += y.x == -INFINITY ? 0.f : y.y * ex2(y.x - big);
+                    }
+                    if (whole) {
+                        const int row = it.rt * kDcRows + r, token = row / a.group;
+                        const bool none = it.q.keys - it.q.n + token + 1 <= 0;
+                        const float inv = 1.f / den;
+                        const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                              : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+                        T *out = (T *)a.out + (int64_t)(it.q.row0 + token) * a.out_ld +
+                                 (int64_t)(it.h * a.group + row - token * a.group) * D + hc * (D / 2) + c;
+                        if (store4<T>(out, v)) atomicOr(&bad_rows, 1u << r);
+                    } else {
+                        *(float4 *)(part + r * D + hc * (D / 2) + c) = sum;
+                        if (hc == 0 && c == 0) {
+                            part[kDcRows * D + r] = big;
+                            part[kDcRows * D + kDcRows + r] = den;
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            const unsigned bad = bad_rows;
+            if (bad) {  // a masked NaN or infinity met the sums: those rows again, without it
+                for (int r = warp; r < rows; r += kDcWarps) {
+                    if (!(bad >> r & 1u)) continue;
+                    const int row = it.rt * kDcRows + r, token = row / a.group;
+                    attention_row<T, KT, D>(a, it.q.row0 + token, it.h * a.group + row - token * a.group, it.s, it.q,
+                                            merge + warp * D, 0, D);
+                }
+                __syncthreads();
+                if (tid == 0) bad_rows = 0u;
+                __syncthreads();
+            }
+            seg = u + 1;
+        }
+        it.next(plan);
+    }
+}
+
+// Joins the partials of items split between CTAs.  Boundary c (CTA c's first
+// unit) lies inside an item or at its start; the boundaries inside one item
+// share its join, each taking a slice of the output.  Partials are added in
+// order, so the result does not depend on timing.
+template <typename T, typename KT, int D>
+__global__ void __launch_bounds__(kDcThreads) decode_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials, int ctas)
+{
+    using C = Dc<D>;
+    __shared__ long long scratch[kDcWarps];
+    __shared__ float qs[kDcWarps][D];
+    const int tid = threadIdx.x, c = blockIdx.x + 1;
+    const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
+    long long total;
+    const Found f = find_unit(plan, scratch, &total, [&](long long n) { return n * c / ctas; });
+    // every CTA waits for the partials, also those with nothing to join: the
+    // next launch of the stream follows this one
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto first = [&](int cta) { return total * cta / ctas; };
+    const long long u = first(c);
+    if (u >= total || u == first(c + 1)) return;  // an empty share: its neighbour has this unit
+    DcIter it;
+    it.begin(plan, f.s, f.rel);
+    if (it.blk == 0) return;  // the item starts here
+    const long long begin = u - it.blk, end = begin + it.blks;
+    // CTAs [c0, c1) hold the item; boundaries c0 + 1 .. c1 - 1 (non-empty) join it
+    int c0 = c, c1 = c + 1, slice = 0, slices = 0;
+    for (int x = c; x > 0 && first(x) > begin; --x) c0 = x - 1;
+    while (c1 < ctas && first(c1) < end) ++c1;
+    for (int x = c0 + 1; x < c1; ++x) {
+        if (first(x) <= begin || first(x) == first(x + 1)) continue;
+        if (x < c) ++slice;
+        ++slices;
+    }
+    const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
+    const int positions = rows * (D / 4), p0 = (int)((long long)positions * slice / slices);
+    const int p1 = (int)((long long)positions * (slice + 1) / slices);
+    int width = 1;  // lanes that share a position
+    while (width < 32 && (p1 - p0) * width * 2 <= kDcThreads) width *= 2;
+    const int lane = tid % width;
+    for (int i0 = p0; i0 < p1; i0 += kDcThreads / width) {
+        const int i = i0 + tid / width;
+        const bool live = i < p1;
+        const int r = live ? i / (D / 4) : 0, col = live ? (i % (D / 4)) * 4 : 0;
+        auto slot = [&](int x) { return partials + (size_t)(2 * x + (first(x) <= begin ? 1 : 0)) * C::kPartial; };
+        float big = -INFINITY, den = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = c0 + lane; x < c1; x += width) {
+            if (first(x) == first(x + 1)) continue;
+            const float *p = slot(x);
+            const float mx = p[kDcRows * D + r];
+            if (mx == -INFINITY) continue;
+            const float4 v = *(const float4 *)(p + r * D + col);
+            const float nb = fmaxf(big, mx), fo = big == -INFINITY ? 0.f : ex2(big - nb), fn = ex2(mx - nb);
+            den = den * fo + p[kDcRows * D + kDcRows + r] * fn;
+            sum = make_float4(sum.x * fo + v.x * fn, sum.y * fo + v.y * fn, sum.z * fo + v.z * fn, sum.w * fo + v.w * fn);
+            big = nb;
+        }
+        for (int d = width >> 1; d; d >>= 1) {
+            const float ob = __shfl_xor_sync(kFull, big, d), od = __shfl_xor_sync(kFull, den, d);
+            const float4 ov = make_float4(__shfl_xor_sync(kFull, sum.x, d), __shfl_xor_sync(kFull, sum.y, d),
+                                          __shfl_xor_sync(kFull, sum.z, d), __shfl_xor_sync(kFull, sum.w, d));
+            const float nb = fmaxf(big, ob), fo = big == -INFINITY ? 0.f : ex2(big - nb), fn = ob == -INFINITY ? 0.f : ex2(ob - nb);
+            den = den * fo + od * fn;
+            sum = make_float4(sum.x * fo + ov.x * fn, sum.y * fo + ov.y * fn, sum.z * fo + ov.z * fn, sum.w * fo + ov.w * fn);
+            big = nb;
+        }
+        bool bad = false;
+        const int row = it.rt * kDcRows + r, token = row / a.group, head = it.h * a.group + row - token * a.group;
+        if (live && lane == 0) {
+            const bool none = it.q.keys - it.q.n + token + 1 <= 0;
+            const float inv = 1.f / den;
+            const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            bad = store4<T>((T *)a.out + (int64_t)(it.q.row0 + token) * a.out_ld + (int64_t)head * D + col, v);
+        }
+        for (unsigned left = __ballot_sync(kFull, bad); left; left &= left - 1) {
+            const int who = __ffs(left) - 1;
+            const int wt = __shfl_sync(kFull, token, who), wh = __shfl_sync(kFull, head, who), wc = __shfl_sync(kFull, col, who);
+            attention_row<T, KT, D>(a, it.q.row0 + wt, wh, it.s, it.q, qs[tid >> 5], wc, wc + 4);
+        }
+    }
 }
 
 // The factors of `base` for head dimension d, to 64 bits of a turn; kept per
@@ -375,6 +960,52 @@ cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s)
     return by_type(a.type, a.kv_type, a.head_dim, [&](auto t, auto kt, auto d) {
         paged_append_kernel<decltype(t), decltype(kt), d.value><<<(unsigned)a.tokens, kAppendThreads, 0, s>>>(a, turns);
         return cudaGetLastError();
+    });
+}
+
+cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
+{
+    return by_type(a.type, a.kv_type, a.head_dim, [&](auto t, auto kt, auto d) {
+        using T = decltype(t);
+        using KT = decltype(kt);
+        constexpr int D = d.value;
+        if constexpr (sizeof(KT) == 4) {
+            return cudaErrorInvalidValue;
+        } else {
+            using C = Dc<D>;
+            int dev = 0, sms = 0;
+            cudaError_t e = cudaGetDevice(&dev);
+            if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(decode_attention_kernel<T, KT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+            // no more CTAs than units there can be, and no partials where an
+            // item has one unit at most
+            const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.page_shift) + kDcUnit - 1) / kDcUnit;
+            const int64_t tiles = ((int64_t)a.tokens * a.group + kDcRows - 1) / kDcRows + a.sequences;
+            const int64_t most = tiles * a.kv_heads * blocks;
+            const int ctas = (int)(most < sms ? most : sms);
+            const bool split = ctas > 1 && blocks > 1;
+            float *partials = nullptr;
+            if (e == cudaSuccess && split) e = stream_alloc((void **)&partials, (size_t)2 * ctas * C::kPartial * sizeof(float), s);
+            if (e != cudaSuccess) return e;
+            decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, partials);
+            e = cudaGetLastError();
+            if (!split) return e;
+            if (e == cudaSuccess) {
+                cudaLaunchConfig_t cfg{};
+                cfg.gridDim = dim3((unsigned)ctas - 1);
+                cfg.blockDim = dim3(kDcThreads);
+                cfg.stream = s;
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attr[0].val.programmaticStreamSerializationAllowed = 1;
+                cfg.attrs = attr;
+                cfg.numAttrs = 1;
+                e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, KT, D>, a, (const float *)partials, ctas);
+            }
+            const cudaError_t f = stream_free(partials, s);
+            return e != cudaSuccess ? e : f;
+        }
     });
 }
 

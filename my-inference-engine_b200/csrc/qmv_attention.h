@@ -47,6 +47,8 @@ struct AppendArgs {
 };
 
 cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s);
+// Paged, 16-bit cache: for few rows a sequence over many keys.
+cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s);
 cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s);
 
 // Status bits of the attention kernels on the current device.

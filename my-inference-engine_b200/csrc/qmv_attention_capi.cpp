@@ -190,6 +190,6 @@ QMV_EXPORT int qmv_paged_attention(const QmvPagedCache *cache, const QmvPagedBat
     const qmv::AttnArgs a{type, cache->type, q, out, q_ld, out_ld, kv, batch->query_start, batch->length,
                           batch->sequences, batch->tokens, heads, cache->kv_heads, heads / cache->kv_heads, d,
                           batch->max_query, scale};
-    const cudaError_t e = qmv::launch_attention_rows(a, (cudaStream_t)stream);
+    const cudaError_t e = qmv::launch_decode_attention(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("attention launch", e);
 }
