@@ -343,34 +343,39 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(AttnArgs
 //
 // Rows r = token * group + head-in-group of one (sequence, key/value head)
 // are cut into tiles of 16, the M of mma.sync m16n8k16; a row tile of one
-// sequence and head is an item, its keys in blocks of 128 are its units, and
-// all units of the launch, in order, are dealt evenly to the CTAs (one an
-// SM), so ragged lengths cost nothing.  Each of the 8 warps takes 16 keys of
-// every unit, streams them through its own cp.async ring (the rings together
-// keep 128 KB a CTA in flight, with no barrier between warps) and holds its
-// own running maximum, sum and output in registers; the warps meet once per
-// item.  An item that ends up in more than one CTA leaves partials (maximum,
+// sequence and head is an item, its keys in blocks of 64 are its units, and
+// all units of the launch, in order, are dealt evenly to the CTAs (two an
+// SM, so that one streams while the other ends an item), and ragged lengths
+// cost nothing.  Each of the 4 warps takes 16 keys of every unit, streams
+// them through its own cp.async ring (the rings together keep 128 KB an SM in
+// flight, with no barrier between warps) and holds its own running maximum,
+// sum and output in registers; the warps meet once per item.  An item that ends up in more than one CTA leaves partials (maximum,
 // sum, unnormalised output) that decode_merge_kernel joins in order.
 // tcgen05 is not used: its M of 64 or more would be mostly empty rows here,
 // and the tensor work is a tenth of the time the bytes take.
 
-constexpr int kDcWarps = 8;
+constexpr int kDcWarps = 4;
+constexpr int kDcPerSm = 2;
 constexpr int kDcThreads = kDcWarps * 32;
 constexpr int kDcKeys = 16;                   // keys of a warp's step
 constexpr int kDcUnit = kDcKeys * kDcWarps;   // keys of a unit
 constexpr int kDcRows = 16;                   // rows of a tile
+// What an item costs beside its keys, in units: loading its queries, the
+// warps' meeting and the output take 3700 cycles, a unit 1100 (D = 128).
+// Dealt without it, 64 sequences of 16..8192 positions took 66 us instead of 39.
+constexpr int kDcItemCost = 3;
 
 template <int D> struct Dc {
     static constexpr uint32_t kRow = D * 2;                    // bytes of a key
     static constexpr uint32_t kStep = 2 * kDcKeys * kRow;      // K and V of a step
     static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr uint32_t kRing = kStep * kStages * kDcWarps;
-    static constexpr uint32_t kMerge = kDcWarps * kDcRows * (D / 2) * 4;
+    static constexpr uint32_t kMerge = kDcWarps * 8 * D * 4;   // 8 rows of every warp
     static constexpr uint32_t kSmem = kRing + kMerge + kDcWarps * kDcRows * 8;
     static constexpr int kPartial = kDcRows * D + 2 * kDcRows;  // floats: o, m, l
-    // half rows of D / 2 floats, 8-float blocks exchanged by the row so that
-    // the 8 rows a warp writes at once fall on different banks
-    static __device__ __forceinline__ int at(int row, int col) { return row * (D / 2) + (col ^ ((row & (D / 16 - 1)) * 8)); }
+    // rows of D floats, 8-float blocks exchanged by the row so that the 8
+    // rows a warp writes at once fall on different banks
+    static __device__ __forceinline__ int at(int row, int col) { return row * D + (col ^ ((row & 7) * 8)); }
 };
 
 // 2^x (2 ulp; results below 2^-126 become 0).
@@ -429,14 +434,15 @@ __device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t hi)
     return pack2<__half>(a - h.x, b - h.y);
 }
 
-// Units of one sequence: key blocks x row tiles x heads.
+// What a sequence costs, in blocks of keys: row tiles x heads items, each of
+// its key blocks and of kDcItemCost for its beginning and end.
 struct DcPlan {
     const int *start, *length;
     int sequences, tokens, max_keys, kv_heads, group;
     __device__ __forceinline__ Seq seq(int s) const { return load_sequence(start, length, s, tokens, max_keys); }
     __device__ __forceinline__ int tiles(const Seq &q) const { return (q.n * group + kDcRows - 1) / kDcRows; }
     __device__ __forceinline__ int blocks(const Seq &q) const { return q.keys > 0 ? (q.keys + kDcUnit - 1) / kDcUnit : 1; }
-    __device__ __forceinline__ long long units(const Seq &q) const { return (long long)tiles(q) * kv_heads * blocks(q); }
+    __device__ __forceinline__ long long cost(const Seq &q) const { return (long long)tiles(q) * kv_heads * (blocks(q) + kDcItemCost); }
 };
 
 // Sum over the CTA of one value a thread, and the exclusive prefix.
@@ -462,46 +468,48 @@ __device__ __forceinline__ long long block_scan(long long v, long long *total, l
     return before + x - v;
 }
 
-struct Found {
-    int s;          // sequence
-    long long rel;  // unit within it
+// How `total` is dealt to `ctas` CTAs in order: the first total % ctas get
+// one more.
+struct Deal {
+    long long each, more;
+    __device__ __forceinline__ Deal(long long total, int ctas) : each(total / ctas), more(total - each * ctas) {}
+    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
+    __device__ __forceinline__ int holder(long long u) const
+    {
+        const long long big = more * (each + 1);
+        return u < big ? (int)(u / (each + 1)) : (int)(more + (u - big) / each);
+    }
 };
 
-// All units of the launch, then the sequence of unit share(total) (by every
-// thread of the CTA together).
-template <typename F> __device__ Found find_unit(const DcPlan &p, long long *scratch, long long *total, const F &share)
+struct Found {
+    int s;          // sequence
+    long long rel;  // place within it
+};
+
+// The cost of the whole launch, and the sequence in which place share(total)
+// falls (by every thread of the CTA together; a thread takes a run of
+// sequences).
+template <typename F> __device__ Found find_place(const DcPlan &p, long long *scratch, long long *total, const F &share)
 {
     __shared__ Found found;
-    long long all = 0, v = 0, before = 0;
-    for (int s0 = 0; s0 < p.sequences; s0 += kDcThreads) {
-        const int s = s0 + (int)threadIdx.x;
-        v = s < p.sequences ? p.units(p.seq(s)) : 0;
-        long long t;
-        before = block_scan(v, &t, scratch);
-        all += t;
-    }
-    *total = all;
-    const long long want = share(all);
+    const int per = (p.sequences + kDcThreads - 1) / kDcThreads, s0 = (int)threadIdx.x * per, s1 = min(s0 + per, p.sequences);
+    long long v = 0;
+    for (int s = s0; s < s1; ++s) v += p.cost(p.seq(s));
     if (threadIdx.x == 0) found = Found{p.sequences, 0};
-    if (p.sequences <= kDcThreads) {  // this thread's sequence is still at hand
-        __syncthreads();
-        if (want >= before && want < before + v) found = Found{(int)threadIdx.x, want - before};
-    } else {
-        long long base = 0;
-        for (int s0 = 0; s0 < p.sequences && base <= want; s0 += kDcThreads) {
-            const int s = s0 + (int)threadIdx.x;
-            v = s < p.sequences ? p.units(p.seq(s)) : 0;
-            long long t;
-            before = base + block_scan(v, &t, scratch);
-            if (want >= before && want < before + v) found = Found{s, want - before};
-            base += t;
-        }
+    long long before = block_scan(v, total, scratch);
+    const long long want = share(*total);
+    if (want >= before && want < before + v) {
+        int s = s0;
+        for (long long c; want >= before + (c = p.cost(p.seq(s))); ++s) before += c;
+        found = Found{s, want - before};
     }
     __syncthreads();
     return found;
 }
 
-// Walks units in order: sequence, head, row tile, key block.
+// Walks units in order: sequence, head, row tile, key block.  A unit's place
+// is its item's first place + kDcItemCost + blk; a CTA has the units whose
+// places fall in its share.
 struct DcIter {
     Seq q;
     int s, h, rt, blk, rts, blks;
@@ -516,25 +524,31 @@ struct DcIter {
             ++s;
         }
     }
-    __device__ __forceinline__ void begin(const DcPlan &p, int s_, long long rel)
+    // The first unit at or behind place rel of sequence s_; how far behind.
+    __device__ __forceinline__ int begin(const DcPlan &p, int s_, long long rel)
     {
         s = s_;
         enter(p);
-        blk = blks ? (int)(rel % blks) : 0;
-        const int item = blks ? (int)(rel / blks) : 0;
-        rt = rts ? item % rts : 0;
-        h = rts ? item / rts : 0;
+        blk = h = rt = 0;
+        if (rts == 0) return 0;
+        const int span = blks + kDcItemCost, item = (int)(rel / span), at = (int)(rel - (long long)item * span);
+        blk = max(0, at - kDcItemCost);
+        rt = item % rts;
+        h = item / rts;
+        return kDcItemCost + blk - at;
     }
-    __device__ __forceinline__ void next(const DcPlan &p)
+    // To the next unit; the places between.
+    __device__ __forceinline__ int next(const DcPlan &p)
     {
-        if (++blk < blks) return;
+        if (++blk < blks) return 1;
         blk = 0;
-        if (++rt < rts) return;
+        if (++rt < rts) return 1 + kDcItemCost;
         rt = 0;
-        if (++h < p.kv_heads) return;
+        if (++h < p.kv_heads) return 1 + kDcItemCost;
         h = 0;
         ++s;
         enter(p);
+        return 1 + kDcItemCost;
     }
 };
 
@@ -550,7 +564,7 @@ template <typename T> __device__ __forceinline__ bool store4(T *out, const float
 }
 
 template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ partials)
+__global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ partials)
 {
     using C = Dc<D>;
     constexpr int NQ = sizeof(T) == 4 ? 2 : 1;  // f16 pairs for f32 activations
@@ -568,12 +582,14 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
     if (blockIdx.x == 0) check_metadata(a.start, a.length, a.sequences, a.tokens, plan.max_keys);
     if (tid == 0) bad_rows = 0u;
     long long total;
-    const Found f = find_unit(plan, scratch, &total, [&](long long n) { return n * blockIdx.x / gridDim.x; });
-    const long long u0 = total * blockIdx.x / gridDim.x, u1 = total * (blockIdx.x + 1) / gridDim.x;
-    if (u0 >= u1) return;
+    const Found f = find_place(plan, scratch, &total, [&](long long n) { return Deal(n, gridDim.x).first(blockIdx.x); });
+    const Deal deal(total, gridDim.x);
+    long long u = deal.first(blockIdx.x);
+    const long long u1 = deal.first(blockIdx.x + 1);
+    if (u >= u1) return;
 
     DcIter pf, it;
-    it.begin(plan, f.s, f.rel);
+    u += it.begin(plan, f.s, f.rel);
     pf = it;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)warp * C::kStep * C::kStages;
     const int mask = (1 << a.kv.page_shift) - 1;
@@ -583,17 +599,18 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
         const int j0 = i.blk * kDcUnit + warp * kDcKeys;
         return j0 < i.q.keys ? __ldg(a.kv.table + (int64_t)i.s * a.kv.max_pages + (j0 >> a.kv.page_shift)) : -1;
     };
-    long long fetched = u0;
+    long long ahead = u;     // place of the next unit to fetch
+    uint32_t to_stage = 0u;  // its stage
     int page = page_of(pf);
     auto issue = [&]() {
-        if (fetched < u1) {
+        if (ahead < u1) {
             const int j0 = pf.blk * kDcUnit + warp * kDcKeys;
             if (j0 < pf.q.keys) {
                 const bool good = page >= 0 && page < a.kv.page_count;
                 if (!good && lane == 0) report(kStatusBadMetadata);
                 const int64_t base = (int64_t)(good ? page : 0) * a.kv.page + (int64_t)(j0 & mask) * a.kv.k_pos + (int64_t)pf.h * a.kv.head;
                 const KT *k = (const KT *)a.kv.k + base, *v = (const KT *)a.kv.v + base;
-                const uint32_t dst = ring + ((uint32_t)(fetched - u0) % C::kStages) * C::kStep;
+                const uint32_t dst = ring + to_stage * C::kStep;
                 constexpr int CH = D / 8;  // 16-byte pieces of a key
                 const int c = lane % CH;
 #pragma unroll
@@ -606,9 +623,9 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
                     cp16(to + kDcKeys * C::kRow, v + off, live);
                 }
             }
-            ++fetched;
-            pf.next(plan);
-            if (fetched < u1) page = page_of(pf);
+            to_stage = to_stage + 1 == C::kStages ? 0u : to_stage + 1;
+            ahead += pf.next(plan);
+            if (ahead < u1) page = page_of(pf);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -618,9 +635,13 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
     uint32_t qf[NQ][KS][4];
     float o[NT][4], m[2], l[2], factor[2];
     int lim[2];
-    long long seg = u0;  // first unit of the current segment
-    for (long long u = u0; u < u1; ++u) {
-        if (u == seg) {
+    uint32_t stage = 0u;
+    bool fresh = true;  // at the first unit of a segment, this CTA's part of an item
+    int first_blk = 0;  // its key block
+    while (u < u1) {
+        if (fresh) {
+            fresh = false;
+            first_blk = it.blk;
             // the item's query rows as A fragments: rows grp and grp + 8
             const int rows = it.q.n * a.group - it.rt * kDcRows;
 #pragma unroll
@@ -676,7 +697,7 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
         issue();  // refills the stage read in the previous step
         const int j0 = it.blk * kDcUnit + warp * kDcKeys;
         if (j0 < it.q.keys) {
-            const uint32_t ks = ring + ((uint32_t)(u - u0) % C::kStages) * C::kStep, vs = ks + kDcKeys * C::kRow;
+            const uint32_t ks = ring + stage * C::kStep, vs = ks + kDcKeys * C::kRow;
             float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             {
                 const int r = (lane & 7) + ((lane >> 4) << 3), c0 = (lane >> 3) & 1;
@@ -753,11 +774,12 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
                 }
             }
         }
+        stage = stage + 1 == C::kStages ? 0u : stage + 1;
         const bool last_block = it.blk + 1 == it.blks;
-        if (last_block || u + 1 == u1) {
-            // the warps' shares of the segment meet in shared memory, half of
-            // the columns at a time
-            const bool whole = last_block && u - it.blk >= u0;
+        if (last_block || u + 1 >= u1) {
+            // the warps' shares of the segment meet in shared memory, 8 rows
+            // at a time
+            const bool whole = last_block && first_blk == 0;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 l[half] += __shfl_xor_sync(kFull, l[half], 1);
@@ -765,36 +787,31 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
                 if (quad == 0) ml[warp * kDcRows + grp + 8 * half] = make_float2(m[half], l[half]);
             }
             __syncthreads();
-            float top[2], mine[2];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                top[half] = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kDcWarps; ++w) top[half] = fmaxf(top[half], ml[w * kDcRows + grp + 8 * half].x);
-                mine[half] = m[half] == -INFINITY ? 0.f : ex2(m[half] - top[half]);
-            }
             const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
             // a partial that starts inside its item goes to the first slot
-            float *part = partials + (size_t)(2 * blockIdx.x + (u - it.blk >= u0 ? 1 : 0)) * C::kPartial;
+            float *part = partials + (size_t)(2 * blockIdx.x + (first_blk == 0 ? 1 : 0)) * C::kPartial;
 #pragma unroll
-            for (int hc = 0; hc < 2; ++hc) {
+            for (int half = 0; half < 2; ++half) {
+                if (8 * half >= rows) break;
+                float top = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < NT / 2; ++t)
+                for (int w = 0; w < kDcWarps; ++w) top = fmaxf(top, ml[w * kDcRows + grp + 8 * half].x);
+                const float mine = m[half] == -INFINITY ? 0.f : ex2(m[half] - top);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        *(float2 *)(merge + C::at(warp * kDcRows + grp + 8 * half, 8 * t + 2 * quad)) =
-                            make_float2(o[hc * NT / 2 + t][2 * half] * mine[half], o[hc * NT / 2 + t][2 * half + 1] * mine[half]);
+                for (int t = 0; t < NT; ++t)
+                    *(float2 *)(merge + C::at(warp * 8 + grp, 8 * t + 2 * quad)) =
+                        make_float2(o[t][2 * half] * mine, o[t][2 * half + 1] * mine);
                 __syncthreads();
-                constexpr int C4 = D / 8;  // float4 columns of half a row
-                for (int i = tid; i < rows * C4; i += kDcThreads) {
-                    const int r = i / C4, c = (i % C4) * 4;
+                constexpr int C4 = D / 4;  // float4 columns of a row
+                for (int i = tid; i < min(8, rows - 8 * half) * C4; i += kDcThreads) {
+                    const int r8 = i / C4, r = r8 + 8 * half, c = (i % C4) * 4;
                     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
                     float big = -INFINITY, den = 0.f;
 #pragma unroll
                     for (int w = 0; w < kDcWarps; ++w) big = fmaxf(big, ml[w * kDcRows + r].x);
 #pragma unroll
                     for (int w = 0; w < kDcWarps; ++w) {
-                        const float4 x = *(const float4 *)(merge + C::at(w * kDcRows + r, c));
+                        const float4 x = *(const float4 *)(merge + C::at(w * 8 + r8, c));
                         sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
                         const float2 y = ml[w * kDcRows + r];
                         den += y.x == -INFINITY ? 0.f : y.y * ex2(y.x - big);
@@ -806,11 +823,11 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
                         const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
                                               : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
                         T *out = (T *)a.out + (int64_t)(it.q.row0 + token) * a.out_ld +
-                                 (int64_t)(it.h * a.group + row - token * a.group) * D + hc * (D / 2) + c;
+                                 (int64_t)(it.h * a.group + row - token * a.group) * D + c;
                         if (store4<T>(out, v)) atomicOr(&bad_rows, 1u << r);
                     } else {
-                        *(float4 *)(part + r * D + hc * (D / 2) + c) = sum;
-                        if (hc == 0 && c == 0) {
+                        *(float4 *)(part + r * D + c) = sum;
+                        if (c == 0) {
                             part[kDcRows * D + r] = big;
                             part[kDcRows * D + kDcRows + r] = den;
                         }
@@ -830,9 +847,9 @@ __global__ void __launch_bounds__(kDcThreads, 1) decode_attention_kernel(const _
                 if (tid == 0) bad_rows = 0u;
                 __syncthreads();
             }
-            seg = u + 1;
+            fresh = true;
         }
-        it.next(plan);
+        u += it.next(plan);
     }
 }
 
@@ -849,26 +866,19 @@ __global__ void __launch_bounds__(kDcThreads) decode_merge_kernel(const __grid_c
     const int tid = threadIdx.x, c = blockIdx.x + 1;
     const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
     long long total;
-    const Found f = find_unit(plan, scratch, &total, [&](long long n) { return n * c / ctas; });
+    const Found f = find_place(plan, scratch, &total, [&](long long n) { return Deal(n, ctas).first(c); });
     // every CTA waits for the partials, also those with nothing to join: the
     // next launch of the stream follows this one
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    auto first = [&](int cta) { return total * cta / ctas; };
-    const long long u = first(c);
-    if (u >= total || u == first(c + 1)) return;  // an empty share: its neighbour has this unit
+    const Deal deal(total, ctas);
+    const long long u = deal.first(c);
+    if (u >= total) return;  // an empty share
     DcIter it;
-    it.begin(plan, f.s, f.rel);
+    const int behind = it.begin(plan, f.s, f.rel);
     if (it.blk == 0) return;  // the item starts here
-    const long long begin = u - it.blk, end = begin + it.blks;
-    // CTAs [c0, c1) hold the item; boundaries c0 + 1 .. c1 - 1 (non-empty) join it
-    int c0 = c, c1 = c + 1, slice = 0, slices = 0;
-    for (int x = c; x > 0 && first(x) > begin; --x) c0 = x - 1;
-    while (c1 < ctas && first(c1) < end) ++c1;
-    for (int x = c0 + 1; x < c1; ++x) {
-        if (first(x) <= begin || first(x) == first(x + 1)) continue;
-        if (x < c) ++slice;
-        ++slices;
-    }
+    // CTAs c0 .. c1 hold the item, and the boundaries c0 + 1 .. c1 join it
+    const long long begin = u + behind - it.blk;  // place of its first unit
+    const int c0 = deal.holder(begin), c1 = deal.holder(begin + it.blks - 1), slice = c - c0 - 1, slices = c1 - c0;
     const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
     const int positions = rows * (D / 4), p0 = (int)((long long)positions * slice / slices);
     const int p1 = (int)((long long)positions * (slice + 1) / slices);
@@ -879,11 +889,10 @@ __global__ void __launch_bounds__(kDcThreads) decode_merge_kernel(const __grid_c
         const int i = i0 + tid / width;
         const bool live = i < p1;
         const int r = live ? i / (D / 4) : 0, col = live ? (i % (D / 4)) * 4 : 0;
-        auto slot = [&](int x) { return partials + (size_t)(2 * x + (first(x) <= begin ? 1 : 0)) * C::kPartial; };
+        auto slot = [&](int x) { return partials + (size_t)(2 * x + (x == c0 ? 1 : 0)) * C::kPartial; };
         float big = -INFINITY, den = 0.f;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int x = c0 + lane; x < c1; x += width) {
-            if (first(x) == first(x + 1)) continue;
+        for (int x = c0 + lane; x <= c1; x += width) {
             const float *p = slot(x);
             const float mx = p[kDcRows * D + r];
             if (mx == -INFINITY) continue;
@@ -983,7 +992,7 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
             const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.page_shift) + kDcUnit - 1) / kDcUnit;
             const int64_t tiles = ((int64_t)a.tokens * a.group + kDcRows - 1) / kDcRows + a.sequences;
             const int64_t most = tiles * a.kv_heads * blocks;
-            const int ctas = (int)(most < sms ? most : sms);
+            const int ctas = (int)(most < kDcPerSm * sms ? most : kDcPerSm * sms);
             const bool split = ctas > 1 && blocks > 1;
             float *partials = nullptr;
             if (e == cudaSuccess && split) e = stream_alloc((void **)&partials, (size_t)2 * ctas * C::kPartial * sizeof(float), s);
