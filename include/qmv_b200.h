@@ -49,7 +49,8 @@ int qmv_set_device(int device);
  * expired, bit 1 = a producer's wait expired, bit 2 = draining in-flight
  * copies timed out, bit 3 = a peer's exchange flag never arrived, bit 4 = a
  * tensor-core matmul's wait for its MMAs expired, bit 5 = an attention or
- * append call met a row start, length or page index out of range.  0 means
+ * append call met a row start, length or page index out of range, bit 6 = an
+ * attention kernel's wait expired.  0 means
  * every bounded wait completed and all metadata was in range.  clear != 0 resets the word.  No counterpart in the reference (its kernels never wait). */
 int qmv_device_status(uint32_t *flags, int clear);
 

@@ -20,8 +20,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libqmv_b200.so")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 
 SOURCES = ["qmv_kernels.cu", "qmv_capi.cpp", "qmv_qwen2.cpp", "qmv_gguf.cpp", "quantized_matvec.cpp",
-           "qmv_attention.cu", "qmv_attention_capi.cpp"]
-HEADERS = ["qmv_internal.h", "qmv_attention.h"]
+           "qmv_attention.cu", "qmv_attention_tc.cu", "qmv_attention_capi.cpp"]
+HEADERS = ["qmv_internal.h", "qmv_attention.h", "qmv_attention.cuh"]
 PUBLIC_HEADERS = ["qmv_b200.h", "quantized_matvec.h", "gguf_quantized_view.h"]
 
 NVCC_FLAGS = [
@@ -59,7 +59,7 @@ def _compile(source: str, force: bool):
     header); (object, nvcc's messages)."""
     src, obj = os.path.join(CSRC, source), os.path.join(OBJ_DIR, source + ".o")
     log = obj + ".log"
-    deps = [src] + [f for f in _inputs() if f.endswith(".h")] + [os.path.abspath(__file__)]
+    deps = [src] + [f for f in _inputs() if f.endswith((".h", ".cuh"))] + [os.path.abspath(__file__)]
     if not force and os.path.exists(obj) and os.path.exists(log) and \
             all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in deps):
         with open(log) as fh:

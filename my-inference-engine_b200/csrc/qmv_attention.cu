@@ -9,146 +9,18 @@
 // The softmax runs in base 2 (scale * log2 e folded into one factor) and
 // online: a running maximum m, sum l and unnormalised output o are rescaled
 // by 2^(m_old - m_new) when a later key raises the maximum.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
-#include <type_traits>
-
-#include "qmv_attention.h"
+#include "qmv_attention.cuh"
 #include "qmv_internal.h"
 
 namespace qmv {
 
 namespace {
 
-constexpr unsigned kFull = 0xffffffffu;
-constexpr float kLog2e = 1.4426950408889634f;
-
 __device__ unsigned int g_attention_status;
-
-__device__ __forceinline__ void report(unsigned int bit) { atomicOr(&g_attention_status, bit); }
-
-// --------------------------------------------------------- element types
-
-// 16 bytes of a row as floats, and back.
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-    static constexpr int kVec = 4;
-    static __device__ __forceinline__ void load(const float *p, float v[4])
-    {
-        const float4 x = *(const float4 *)p;
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    }
-    static __device__ __forceinline__ void store(float *p, const float v[4]) { *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]); }
-    static __device__ __forceinline__ float to_float(float x) { return x; }
-    static __device__ __forceinline__ float from_float(float x) { return x; }
-};
-template <> struct Elem<__half> {
-    static constexpr int kVec = 8;
-    static __device__ __forceinline__ void load(const __half *p, float v[8])
-    {
-        const uint4 x = *(const uint4 *)p;
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*(const __half2 *)&w[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ void store(__half *p, const float v[8])
-    {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(__half2 *)&w[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    static __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-    static __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
-};
-template <> struct Elem<__nv_bfloat16> {
-    static constexpr int kVec = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float v[8])
-    {
-        const uint4 x = *(const uint4 *)p;
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float v[8])
-    {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(__nv_bfloat162 *)&w[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    static __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-    static __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
-};
-
-// ------------------------------------------------------------ metadata
-
-// The last s in [0, n) with start[s] <= row (0 when there is none), by the
-// 32 lanes of a warp together: 32 splits a step.
-__device__ __forceinline__ int find_sequence(const int *__restrict__ start, int n, int row)
-{
-    const int lane = threadIdx.x & 31;
-    int lo = 0, len = n;
-    while (len > 1) {
-        const int step = (len + 31) / 32;
-        const int s = lo + lane * step;
-        const bool below = s < lo + len && __ldg(start + s) <= row;
-        const unsigned m = __ballot_sync(kFull, below);
-        const int k = m ? 31 - __clz(m) : 0;
-        const int end = lo + len;
-        lo += k * step;
-        len = min(step, end - lo);
-    }
-    return lo;
-}
-
-struct Seq {
-    int row0;  // first row
-    int n;     // new tokens (0: left out)
-    int keys;  // cached positions, new tokens included
-};
-
-__device__ __forceinline__ Seq load_sequence(const int *__restrict__ start, const int *__restrict__ length, int s,
-                                             int tokens, int max_keys)
-{
-    const int a = __ldg(start + s), b = __ldg(start + s + 1);
-    Seq q{a, b - a, b - a};
-    bool ok = a >= 0 && a <= b && b <= tokens;
-    if (length != nullptr) {
-        q.keys = __ldg(length + s);
-        ok = ok && q.keys >= 0 && q.keys <= max_keys;
-    }
-    if (!ok) q.n = q.keys = 0;
-    return q;
-}
-
-__device__ __forceinline__ int max_keys_of(const KvView &kv) { return kv.table ? kv.max_pages << kv.page_shift : 0x7fffffff; }
-
-// Reports metadata out of range (one CTA of a launch calls it).
-__device__ void check_metadata(const int *__restrict__ start, const int *__restrict__ length, int n, int tokens, int max_keys)
-{
-    bool bad = false;
-    for (int s = threadIdx.x; s < n; s += blockDim.x) {
-        const int a = __ldg(start + s), b = __ldg(start + s + 1);
-        bad |= !(a >= 0 && a <= b && b <= tokens);
-        if (length != nullptr) {
-            const int k = __ldg(length + s);
-            bad |= k < 0 || k > max_keys;
-        }
-    }
-    if (bad) report(kStatusBadMetadata);
-}
 
 // ------------------------------------------------------ rope and append
 //
@@ -172,14 +44,14 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
     constexpr int V = Elem<T>::kVec, H = D / 2, U = H / V;  // pieces of a half head
     __shared__ float cs[H], sn[H];
     const int row = blockIdx.x;
-    if (row == 0) check_metadata(a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
+    if (row == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
     const int s = find_sequence(a.start, a.sequences, row);
     const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
     const int i = row - sq.row0, pos = sq.keys - sq.n + i;
     if (i < 0 || i >= sq.n || pos < 0) return;  // the same for the whole CTA
     const int page = __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (pos >> a.kv.page_shift));
     const bool stored = page >= 0 && page < a.kv.page_count;
-    if (!stored && threadIdx.x == 0) report(kStatusBadMetadata);
+    if (!stored && threadIdx.x == 0) report(a.status, kStatusBadMetadata);
     const bool rope = a.rope_base > 0.f;
     if (rope) {
         for (int e = threadIdx.x; e < H; e += kAppendThreads) {
@@ -231,104 +103,13 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
     }
 }
 
-// ------------------------------------------------------ attention by rows
-//
-// One warp computes one (token, query head) in f32 on the CUDA cores: a lane
-// a key for the scores, a lane D / 32 elements for the output, of which
-// columns [col0, col1) are written.  Masked keys are never read.  The faster
-// kernels come back to it for rows that are not finite: a masked key's weight
-// of 0 times a NaN or infinite value must not reach a sum, and theirs does.
-
-template <typename T, typename KT, int D>
-__device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head, int s, const Seq &sq, float *qs, int col0, int col1)
-{
-    constexpr int V = Elem<KT>::kVec, E = D / 32;
-    const int lane = threadIdx.x & 31, h = head / a.group;
-    const int n_keys = sq.keys - sq.n + (row - sq.row0) + 1;
-    T *out = (T *)a.out + (int64_t)row * a.out_ld + head * D;
-    if (n_keys <= 0) {
-        for (int e = col0 + lane; e < col1; e += 32) out[e] = Elem<T>::from_float(0.f);
-        return;
-    }
-    const T *q = (const T *)a.q + (int64_t)row * a.q_ld + head * D;
-    __syncwarp();
-    for (int e = lane; e < D; e += 32) qs[e] = Elem<T>::to_float(q[e]);
-    __syncwarp();
-    const float f = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int j0 = 0; j0 < n_keys; j0 += 32) {
-        const int j = j0 + lane;
-        bool live = j < n_keys;
-        int64_t ko = 0, vo = 0;
-        if (live) {
-            if (a.kv.table) {
-                const int page = __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (j >> a.kv.page_shift));
-                if (page < 0 || page >= a.kv.page_count) {
-                    report(kStatusBadMetadata);
-                    live = false;
-                } else {
-                    ko = (int64_t)page * a.kv.page + (int64_t)(j & ((1 << a.kv.page_shift) - 1)) * a.kv.k_pos;
-                    vo = ko;
-                }
-            } else {
-                ko = (int64_t)(sq.row0 + j) * a.kv.k_pos;
-                vo = (int64_t)(sq.row0 + j) * a.kv.v_pos;
-            }
-            ko += h * a.kv.head;
-            vo += h * a.kv.head;
-        }
-        float sc = -INFINITY;
-        if (live) {
-            const KT *k = (const KT *)a.kv.k + ko;
-            float acc = 0.f;
-            for (int e = 0; e < D; e += V) {
-                float x[V];
-                Elem<KT>::load(k + e, x);
-#pragma unroll
-                for (int t = 0; t < V; ++t) acc = fmaf(x[t], qs[e + t], acc);
-            }
-            sc = acc * f;
-        }
-        float mt = sc;
-        bool nan = isnan(sc);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(kFull, mt, d));
-        if (__any_sync(kFull, nan)) mt = NAN;
-        const float mn = isnan(mt) || isnan(m) ? NAN : fmaxf(m, mt);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        const float p = live ? exp2f(sc - ms) : 0.f;
-        const float fix = m == -INFINITY ? 0.f : exp2f(m - ms);
-        m = mn;
-        float sum = p;
-#pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-        l = l * fix + sum;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] *= fix;
-        const unsigned alive = __ballot_sync(kFull, live);
-        for (int t = 0; t < 32; ++t) {
-            if (!(alive >> t & 1u)) continue;
-            const float pt = __shfl_sync(kFull, p, t);
-            const int64_t at = __shfl_sync(kFull, vo, t);
-            const KT *v = (const KT *)a.kv.v + at;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(pt, Elem<KT>::to_float(v[e * 32 + lane]), o[e]);
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e * 32 + lane >= col0 && e * 32 + lane < col1) out[e * 32 + lane] = Elem<T>::from_float(o[e] / l);
-}
-
 constexpr int kRowWarps = 4;
 
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(AttnArgs a)
 {
     __shared__ float qs[kRowWarps][D];
-    if (blockIdx.x == 0 && blockIdx.y == 0) check_metadata(a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
     const int row = blockIdx.x, warp = threadIdx.x >> 5, head = blockIdx.y * kRowWarps + warp;
     const int s = find_sequence(a.start, a.sequences, row);
     const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
@@ -378,14 +159,6 @@ template <int D> struct Dc {
     static __device__ __forceinline__ int at(int row, int col) { return row * D + (col ^ ((row & 7) * 8)); }
 };
 
-// 2^x (2 ulp; results below 2^-126 become 0).
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16u : 0u) : "memory");
@@ -415,23 +188,6 @@ template <typename KT> __device__ __forceinline__ void mma16816(float d[4], cons
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <typename KT> __device__ __forceinline__ uint32_t pack2(float a, float b)
-{
-    uint32_t w;
-    if constexpr (std::is_same<KT, __half>::value)
-        *(__half2 *)&w = __floats2half2_rn(a, b);
-    else
-        *(__nv_bfloat162 *)&w = __floats2bfloat162_rn(a, b);
-    return w;
-}
-
-// What is left of (a, b) after their f16 rounding, as f16.
-__device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t hi)
-{
-    const float2 h = __half22float2(*(const __half2 *)&hi);
-    return pack2<__half>(a - h.x, b - h.y);
 }
 
 // What a sequence costs, in blocks of keys: row tiles x heads items, each of
@@ -579,7 +335,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, grp = lane >> 2;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
-    if (blockIdx.x == 0) check_metadata(a.start, a.length, a.sequences, a.tokens, plan.max_keys);
+    if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
     if (tid == 0) bad_rows = 0u;
     long long total;
     const Found f = find_place(plan, scratch, &total, [&](long long n) { return Deal(n, gridDim.x).first(blockIdx.x); });
@@ -607,7 +363,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             const int j0 = pf.blk * kDcUnit + warp * kDcKeys;
             if (j0 < pf.q.keys) {
                 const bool good = page >= 0 && page < a.kv.page_count;
-                if (!good && lane == 0) report(kStatusBadMetadata);
+                if (!good && lane == 0) report(a.status, kStatusBadMetadata);
                 const int64_t base = (int64_t)(good ? page : 0) * a.kv.page + (int64_t)(j0 & mask) * a.kv.k_pos + (int64_t)pf.h * a.kv.head;
                 const KT *k = (const KT *)a.kv.k + base, *v = (const KT *)a.kv.v + base;
                 const uint32_t dst = ring + to_stage * C::kStep;
@@ -1025,6 +781,17 @@ cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s)
         attention_rows_kernel<decltype(t), decltype(kt), d.value><<<grid, kRowWarps * 32, 0, s>>>(a);
         return cudaGetLastError();
     });
+}
+
+cudaError_t attention_status_word(unsigned int **word)
+{
+    static thread_local unsigned int *have[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64)) e = cudaErrorInvalidDevice;
+    if (e == cudaSuccess && have[dev] == nullptr) e = cudaGetSymbolAddress((void **)&have[dev], g_attention_status);
+    if (e == cudaSuccess) *word = have[dev];
+    return e;
 }
 
 cudaError_t attention_status(unsigned int *out, bool clear)

@@ -33,6 +33,7 @@ struct AttnArgs {
     int sequences, tokens, heads, kv_heads, group, head_dim;
     int max_query;
     float scale;  // multiplies q . k
+    unsigned int *status;  // attention_status_word of the device
 };
 
 struct AppendArgs {
@@ -44,15 +45,19 @@ struct AppendArgs {
     const int *start, *length;
     int sequences, tokens, heads, kv_heads, head_dim;
     float rope_base;
+    unsigned int *status;
 };
 
 cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s);
 // Paged, 16-bit cache: for few rows a sequence over many keys.
 cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s);
+// f16 and bf16: prompts and chunks, on tcgen05.
+cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s);
 cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s);
 
 // Status bits of the attention kernels on the current device.
-enum : unsigned int { kStatusBadMetadata = 32u };
+enum : unsigned int { kStatusBadMetadata = 32u, kStatusAttentionWait = 64u };
+cudaError_t attention_status_word(unsigned int **word);
 cudaError_t attention_status(unsigned int *out, bool clear);
 
 }  // namespace qmv

@@ -108,10 +108,11 @@ int check_scale(float *scale, int head_dim)
     return 1;
 }
 
-int current_device(int *dev)
+int current_device(int *dev, unsigned int **status)
 {
-    const cudaError_t e = cudaGetDevice(dev);
-    return e == cudaSuccess ? 1 : qmv::set_cuda_error("cudaGetDevice", e);
+    cudaError_t e = cudaGetDevice(dev);
+    if (e == cudaSuccess) e = qmv::attention_status_word(status);
+    return e == cudaSuccess ? 1 : qmv::set_cuda_error("current device", e);
 }
 
 }  // namespace
@@ -137,13 +138,14 @@ QMV_EXPORT int qmv_paged_append(const QmvPagedCache *cache, const QmvPagedBatch 
     if ((q_out == q && q_out != nullptr && q_out_ld != q_ld) || (k_out == k && k_out_ld != k_ld))
         return fail("an output in its input's place needs the same ld");
     int dev = 0;
-    if (!current_device(&dev) || !check_device("keys", cache->keys, dev) ||
+    unsigned int *status = nullptr;
+    if (!current_device(&dev, &status) || !check_device("keys", cache->keys, dev) ||
         !check_device("values", cache->values, dev) || !check_device("k", k, dev) || !check_device("v", v, dev) ||
         (q_out != nullptr && !check_device("q_out", q_out, dev)) || !check_device("query_start", batch->query_start, dev))
         return 0;
     const qmv::AppendArgs a{type, cache->type, q, k, v, q_out, k_out, q_ld, k_ld, v_ld, q_out_ld, k_out_ld, kv,
                             batch->query_start, batch->length, batch->sequences, batch->tokens, heads, cache->kv_heads, d,
-                            rope_base};
+                            rope_base, status};
     const cudaError_t e = qmv::launch_paged_append(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("append launch", e);
 }
@@ -162,13 +164,15 @@ QMV_EXPORT int qmv_packed_attention(uint32_t type, int heads, int kv_heads, int 
         !check_rows("out", out, out_ld, nq, bytes))
         return 0;
     int dev = 0;
-    if (!current_device(&dev) || !check_device("q", q, dev) || !check_device("k", k, dev) || !check_device("v", v, dev) ||
+    unsigned int *status = nullptr;
+    if (!current_device(&dev, &status) || !check_device("q", q, dev) || !check_device("k", k, dev) || !check_device("v", v, dev) ||
         !check_device("out", out, dev) || !check_device("start", start, dev))
         return 0;
     const qmv::KvView kv{k, v, k_ld, v_ld, 0, head_dim, nullptr, 0, 0, 0};
     const qmv::AttnArgs a{type, type, q, out, q_ld, out_ld, kv, start, nullptr, sequences, tokens, heads, kv_heads,
-                          heads / kv_heads, head_dim, tokens, scale};
-    const cudaError_t e = qmv::launch_attention_rows(a, (cudaStream_t)stream);
+                          heads / kv_heads, head_dim, tokens, scale, status};
+    const cudaError_t e = type == QMV_TYPE_F32 ? qmv::launch_attention_rows(a, (cudaStream_t)stream)
+                                               : qmv::launch_tc_attention(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("attention launch", e);
 }
 
@@ -184,12 +188,14 @@ QMV_EXPORT int qmv_paged_attention(const QmvPagedCache *cache, const QmvPagedBat
     const int bytes = element_bytes(type), d = cache->head_dim;
     if (!check_rows("q", q, q_ld, (int64_t)heads * d, bytes) || !check_rows("out", out, out_ld, (int64_t)heads * d, bytes)) return 0;
     int dev = 0;
-    if (!current_device(&dev) || !check_device("keys", cache->keys, dev) ||
+    unsigned int *status = nullptr;
+    if (!current_device(&dev, &status) || !check_device("keys", cache->keys, dev) ||
         !check_device("values", cache->values, dev) || !check_device("q", q, dev) || !check_device("out", out, dev) || !check_device("query_start", batch->query_start, dev))
         return 0;
     const qmv::AttnArgs a{type, cache->type, q, out, q_ld, out_ld, kv, batch->query_start, batch->length,
                           batch->sequences, batch->tokens, heads, cache->kv_heads, heads / cache->kv_heads, d,
-                          batch->max_query, scale};
-    const cudaError_t e = qmv::launch_decode_attention(a, (cudaStream_t)stream);
+                          batch->max_query, scale, status};
+    const bool few = type == QMV_TYPE_F32 || (int64_t)a.max_query * a.group <= 32;
+    const cudaError_t e = few ? qmv::launch_decode_attention(a, (cudaStream_t)stream) : qmv::launch_tc_attention(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("attention launch", e);
 }

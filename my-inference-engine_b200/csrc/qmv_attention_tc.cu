@@ -1,0 +1,876 @@
+// Causal grouped-query attention on the 5th-generation tensor cores, for
+// prompts (packed rows) and for chunks of new tokens over the paged cache.
+//
+// The query rows of one (sequence, key/value head) are its tokens times its
+// group of query heads, so a 128-row MMA tile holds 128 / group tokens with
+// all heads that read the same keys: the tile is full for any group, keys are
+// fetched once for the group, and the diagonal wastes few keys.  A CTA works
+// on two such tiles at once over the same keys, so that the tensor cores
+// multiply for one while its partner's softmax runs:
+//   S = Q K^T   tcgen05.mma, both operands in shared memory (TMA, 128-byte
+//               swizzle), 128 x 128 f32 in tensor memory;
+//   softmax     one thread a row: the whole row of S in registers, running
+//               reference m and sum l; P = 2^(S f - m) rounded to the values'
+//               16-bit type and stored over S in tensor memory;
+//   O += P V    tcgen05.mma, P from tensor memory, V from shared memory.
+// The reference m is the running maximum, but it is raised only when the
+// maximum passes it by 8 (a factor of 256; f32 sums and 16-bit floating
+// weights do not care), so O is rescaled a few times a row at most.
+//
+// Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
+// the launch in order are cut into one equal share per SM at multiples of 128 keys,
+// and a tile that is cut leaves partials (m, l, O) that tc_merge_kernel joins.
+// So ragged lengths, causal triangles and single long chunks load every SM alike.
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "qmv_attention.cuh"
+#include "qmv_internal.h"
+
+namespace qmv {
+
+namespace {
+
+constexpr int kTcKeys = 128;     // keys of a block
+constexpr int kTcRows = 128;     // rows of a tile
+constexpr int kTcSubs = 2;       // tiles of a CTA
+constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; 8: MMA; 9: loads
+constexpr int kTcMmaWarp = 8, kTcLoadWarp = 9;
+// What a tile costs beside its keys, in keys.
+constexpr int kTcOver = 256;
+constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+template <int D> struct Tc {
+    static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
+    static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
+    static constexpr int kSlots = (int)((220u * 1024u - kTcSubs * kTile) / kTile) > 6 ? 6 : (int)((220u * 1024u - kTcSubs * kTile) / kTile);
+    static constexpr uint32_t kSmem = (kTcSubs + kSlots) * kTile + 1024;
+    static constexpr int kPartial = kTcSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
+};
+
+// ------------------------------------------------------------------- PTX
+
+__device__ __forceinline__ unsigned long long now_ns()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(1000u)
+        : "memory");
+    return ok != 0;
+}
+
+// Bounded wait for the phase with the given parity; false when it expired.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity)
+{
+    if (bar_try(bar, parity)) return true;
+    const unsigned long long t0 = now_ns();
+    for (;;) {
+        if (bar_try(bar, parity)) return true;
+        if (now_ns() - t0 > kWaitLimitNs) return false;
+    }
+}
+
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(kFull, bar_wait(bar, parity)); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void bar_arrive(uint32_t bar)
+{
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// TMA tile loads (no multicast).
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// 32 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float *v)
+{
+    uint32_t *r = (uint32_t *)v;
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
+        "r"(addr)
+        : "memory");
+}
+
+// Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 rows x 128
+// bytes, 1024 bytes apart along the rows).  K-major (Q, K): the contiguous
+// 64 elements run along the reduction.  MN-major (V): they run along the
+// output columns, the second 64 columns one half tile (16 KB) further.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr)
+{
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr)
+{
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Instruction descriptor: f32 accumulator, M = 128, N = n, A and B of the
+// same 16-bit type, A K-major, B K-major or MN-major.
+template <typename KT> __host__ __device__ constexpr uint32_t idesc(int n, bool mn_major)
+{
+    return (1u << 4) | (std::is_same<KT, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (mn_major ? 1u << 16 : 0u) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// ------------------------------------------------------------------ work
+
+struct TcPlan {
+    const int *start, *length;
+    int sequences, tokens, max_keys, kv_heads;
+    int sub, wide;  // tokens of a tile and of a CTA's pair of tiles
+    __device__ __forceinline__ Seq seq(int s) const { return load_sequence(start, length, s, tokens, max_keys); }
+    // Pair i of a sequence spans kTcOver + the keys its last token sees (at
+    // least 1) places; the first k pairs of a head span:
+    __device__ __forceinline__ long long before(const Seq &q, int k) const
+    {
+        const long long c = (q.keys > q.n ? q.keys - q.n : 0) + kTcOver, all = (long long)k * wide;
+        return (long long)k * c + (long long)wide * ((long long)k * (k + 1) / 2) - (all > q.n ? all - q.n : 0);
+    }
+    __device__ __forceinline__ int pairs(const Seq &q) const { return (q.n + wide - 1) / wide; }
+    __device__ __forceinline__ long long cost(const Seq &q) const { return before(q, pairs(q)) * kv_heads; }
+};
+
+struct TcDeal {
+    long long each, more;
+    __device__ __forceinline__ TcDeal(long long total, int ctas) : each(total / ctas), more(total - each * ctas) {}
+    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
+    __device__ __forceinline__ int holder(long long u) const
+    {
+        const long long big = more * (each + 1);
+        return u < big ? (int)(u / (each + 1)) : (int)(more + (u - big) / each);
+    }
+};
+
+struct TcFound {
+    int s;
+    long long rel;
+};
+
+// The cost of the whole launch and the sequence that holds place
+// share(total), by all NT threads of the CTA together.
+template <int NT, typename F> __device__ __forceinline__ TcFound tc_find(const TcPlan &p, long long *total, const F &share)
+{
+    __shared__ TcFound found;
+    __shared__ long long scratch[NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (p.sequences + NT - 1) / NT, s0 = min((int)threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
+    long long v = 0;
+    for (int s = s0; s < s1; ++s) v += p.cost(p.seq(s));
+    long long x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, d);
+        if (lane >= d) x += y;
+    }
+    if (threadIdx.x == 0) found = TcFound{p.sequences, 0};
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    long long base = 0, all = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) base += scratch[w];
+        all += scratch[w];
+    }
+    *total = all;
+    long long at = base + x - v;
+    const long long want = share(all);
+    if (want >= at && want < at + v) {
+        int s = s0;
+        for (long long c; want >= at + (c = p.cost(p.seq(s))); ++s) at += c;
+        found = TcFound{s, want - at};
+    }
+    __syncthreads();
+    return found;
+}
+
+// Walks the pairs of tiles in order: sequence, head, pair.  Key block b of a
+// pair lies at place origin + kTcOver + 128 b; a CTA has the blocks whose
+// places fall in its share.
+struct TcIter {
+    Seq q;
+    int s, h, i, pairs, b0, blocks;
+    long long origin;
+    __device__ __forceinline__ void size(const TcPlan &p)
+    {
+        const int keys = q.keys - q.n + min((i + 1) * p.wide, q.n);
+        blocks = keys > 0 ? (keys + kTcKeys - 1) / kTcKeys : 1;
+    }
+    __device__ __forceinline__ void enter(const TcPlan &p)
+    {
+        pairs = 0;
+        while (s < p.sequences) {
+            q = p.seq(s);
+            pairs = p.pairs(q);
+            if (pairs > 0) break;
+            ++s;
+        }
+    }
+    __device__ __forceinline__ void next(const TcPlan &p)
+    {
+        origin += p.before(q, i + 1) - p.before(q, i);
+        b0 = 0;
+        if (++i == pairs) {
+            i = 0;
+            if (++h == p.kv_heads) {
+                h = 0;
+                ++s;
+                enter(p);
+            }
+        }
+        if (pairs) size(p);
+    }
+    // The first block at or behind place u, which is place rel of sequence s_.
+    __device__ __forceinline__ void begin(const TcPlan &p, int s_, long long rel, long long u)
+    {
+        s = s_;
+        enter(p);
+        h = i = b0 = 0;
+        blocks = 1;
+        origin = u;
+        if (pairs == 0) return;
+        const long long head = p.before(q, pairs);
+        h = (int)(rel / head);
+        rel -= h * head;
+        int lo = 0, hi = pairs - 1;  // the last pair that starts at or before rel
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (p.before(q, mid) <= rel)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        i = lo;
+        const long long at = rel - p.before(q, i);
+        origin = u - at;
+        size(p);
+        b0 = block_at(u);
+        if (b0 >= blocks) next(p);
+    }
+    // The first block at or behind place u.
+    __device__ __forceinline__ int block_at(long long u) const
+    {
+        const long long k = u - origin - kTcOver;
+        return k <= 0 ? 0 : (int)min((k + kTcKeys - 1) / kTcKeys, (long long)blocks);
+    }
+};
+
+// One tile of a pair: its tokens and key blocks.
+struct TcSub {
+    int token0, tokens;  // within the sequence's new tokens
+    int blocks;          // that any of its rows sees (at least 1 when it has tokens)
+    __device__ __forceinline__ TcSub(const TcPlan &p, const TcIter &it, int x)
+    {
+        token0 = it.i * p.wide + x * p.sub;
+        tokens = max(0, min(p.sub, it.q.n - token0));
+        const int keys = it.q.keys - it.q.n + token0 + tokens;
+        blocks = tokens == 0 ? 0 : keys > 0 ? (keys + kTcKeys - 1) / kTcKeys : 1;
+    }
+};
+
+struct TcMaps {
+    CUtensorMap q, k, v;
+};
+
+template <typename T, typename KT, int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, int sub, float *__restrict__ partials)
+{
+    using C = Tc<D>;
+    constexpr int NS = C::kSlots;
+    constexpr float kLift = std::is_same<KT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * NS + 5 * kTcSubs + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ float row_q[8][D];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q_s = smem0, ring = smem0 + kTcSubs * C::kTile;
+    const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t full = bar0, empty = full + 8 * NS, q_full = empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
+                   s_full = q_empty + 8 * kTcSubs, p_full = s_full + 8 * kTcSubs, o_full = p_full + 8 * kTcSubs,
+                   tail_bar = o_full + 8 * kTcSubs, drain_bar = tail_bar + 8;
+    const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
+
+    if (tid == 0) {
+        for (int i = 0; i < NS; ++i) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        for (int x = 0; x < kTcSubs; ++x) {
+            bar_init(q_full + 8 * x, 1);
+            bar_init(q_empty + 8 * x, 1);
+            bar_init(s_full + 8 * x, 1);
+            bar_init(p_full + 8 * x, 4);
+            bar_init(o_full + 8 * x, 1);
+        }
+        bar_init(tail_bar, 1);
+        bar_init(drain_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kTcMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_slot)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
+    long long total;
+    const TcFound f = tc_find<kTcThreads>(plan, &total, [&](long long n) { return TcDeal(n, gridDim.x).first(blockIdx.x); });
+    fence_before();
+    __syncthreads();
+    fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    const TcDeal deal(total, gridDim.x);
+    const long long u0 = deal.first(blockIdx.x), u1 = deal.first(blockIdx.x + 1);
+    TcIter it;
+    it.begin(plan, f.s, f.rel, u0);
+    // the next segment of this CTA: blocks [it.b0, b1) of the pair
+    auto segment = [&](int *b1) {
+        if (u0 >= u1 || it.s >= plan.sequences) return false;
+        *b1 = it.block_at(u1);
+        return *b1 > it.b0;
+    };
+    bool ok = true;
+    int b1 = 0;
+
+    if (warp < 8) {
+        // --------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
+        const uint32_t s_t = lanes + 128u * x, o_t = lanes + 256u + 128u * x;
+        uint32_t s_phase = 0, o_phase = 0;
+        for (; ok && segment(&b1); it.next(plan)) {
+            const TcSub me(plan, it, x);
+            const int end = min(b1, me.blocks), token = r / a.group;
+            const bool row = token < me.tokens;
+            const int keys = it.q.keys - it.q.n + me.token0 + token + 1;
+            // rows without a token run along unmasked and are never written
+            const int lim = row ? max(keys, 0) : 0x7fffffff;
+            const float f = row ? a.scale * kLog2e : 0.f;
+            float m = -INFINITY, l = 0.f;
+            for (int b = it.b0; b < end; ++b) {
+                if (!(ok = warp_wait(s_full + 8 * x, s_phase))) break;
+                s_phase ^= 1;
+                fence_after();
+                float s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(s_t + 32 * i, s + 32 * i);
+                wait_ld();
+                const int j0 = b * kTcKeys;
+                if (__any_sync(kFull, j0 + kTcKeys > lim)) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (j0 + i >= lim) s[i] = -INFINITY;
+                }
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+                if (__any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise))) {
+                    const float mn = fmaxf(m, mx), fix = m == -INFINITY ? 0.f : ex2(m - mn);
+                    m = mn;
+                    l *= fix;
+                    if (b > it.b0) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            tmem_ld32(o_t + c, o);
+                            wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= fix;
+                            tmem_st32(o_t + c, (const uint32_t *)o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : m - kLift;
+                const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 e = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), f2, n2);
+                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                        sum[i & 1] = __fadd2_rn(sum[i & 1], w);
+                        p[i] = pack2<KT>(w.x, w.y);
+                    }
+                    tmem_st32(s_t + 32 * h, p);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full + 8 * x);
+            }
+            if (!ok) break;
+            if (me.tokens == 0) continue;
+            const bool any = end > it.b0;  // this segment holds blocks of this tile
+            if (any) {
+                if (!(ok = warp_wait(o_full + 8 * x, o_phase))) break;
+                o_phase ^= 1;
+                fence_after();
+            }
+            const bool whole = it.b0 == 0 && b1 == it.blocks;
+            const int head = it.h * a.group + r - token * a.group, token_row = it.q.row0 + me.token0 + token;
+            if (whole) {
+                const float inv = 1.f / l;
+                const bool none = keys <= 0;
+                T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D;
+                bool bad = false;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    tmem_ld32(o_t + c, o);
+                    wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        o[i] = none ? 0.f : o[i] * inv;
+                        bad |= !isfinite(o[i]);
+                    }
+                    if (row) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += Elem<T>::kVec) Elem<T>::store(out + c + i, o + i);
+                    }
+                }
+                // a masked NaN or infinity met the sums: those rows again, without it
+                for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
+                    const int who = __ffs(left) - 1;
+                    __syncwarp();
+                    attention_row<T, KT, D>(a, __shfl_sync(kFull, token_row, who), __shfl_sync(kFull, head, who), it.s, it.q, row_q[warp], 0, D);
+                }
+            } else {
+                // a partial that starts inside its pair goes to the first slot
+                float *part = partials + (size_t)(2 * blockIdx.x + (it.b0 == 0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / kTcSubs);
+                if (any) {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        tmem_ld32(o_t + c, o);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *(float4 *)(part + ((c + i) / 4 * kTcRows + r) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+                part[kTcRows * D + r] = m;
+                part[kTcRows * D + kTcRows + r] = l;
+            }
+            fence_before();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == kTcMmaWarp && lane == 0) {
+            // --------------------------------------------------- MMA issue
+            constexpr uint32_t kIdS = idesc<KT>(128, false), kIdO = idesc<KT>(D, true);
+            uint32_t base = 0;  // ring tiles before this segment
+            uint32_t q_phase[kTcSubs] = {0, 0}, p_phase[kTcSubs] = {0, 0};
+            auto slot = [&](uint32_t n) { return n % NS; };
+            auto landed = [&](uint32_t n) { return bar_wait(full + 8 * (n % NS), (n / NS) & 1); };
+            auto scores = [&](int x, uint32_t n) {
+                const uint32_t qa = q_s + x * C::kTile, kb = ring + slot(n) * C::kTile;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k / 4) * C::kHalf + (k % 4) * 32;
+                    mma_ss(tmem + 128u * x, desc_k(qa + off), desc_k(kb + off), kIdS, k != 0);
+                }
+                commit(s_full + 8 * x);
+            };
+            for (; ok && segment(&b1); it.next(plan)) {
+                const int b0 = it.b0, blocks = b1 - b0;
+                int count[kTcSubs];
+#pragma unroll
+                for (int x = 0; x < kTcSubs; ++x) count[x] = max(0, min(b1, TcSub(plan, it, x).blocks) - b0);
+                // block j's K is ring tile base + 2 j, its V base + 2 j + 1
+                ok = landed(base);
+                for (int x = 0; ok && x < kTcSubs; ++x) {
+                    if (count[x] == 0) continue;
+                    if (!(ok = bar_wait(q_full + 8 * x, q_phase[x]))) break;
+                    q_phase[x] ^= 1;
+                    fence_after();
+                    scores(x, base);
+                    if (count[x] == 1) commit(q_empty + 8 * x);
+                }
+                if (!ok) break;
+                commit(empty + 8 * slot(base));
+                for (int j = 0; ok && j < blocks; ++j) {
+                    const uint32_t kn = base + 2 * j + 2, vn = base + 2 * j + 1;
+                    if (!(ok = landed(vn))) break;
+                    bool k_here = false;
+                    for (int x = 0; x < kTcSubs; ++x) {
+                        if (j >= count[x]) continue;
+                        if (!(ok = bar_wait(p_full + 8 * x, p_phase[x]))) break;
+                        p_phase[x] ^= 1;
+                        fence_after();
+                        const uint32_t vb = ring + slot(vn) * C::kTile;
+#pragma unroll
+                        for (int k = 0; k < kTcKeys / 16; ++k)
+                            mma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 8u * k, desc_mn(vb + 2048u * k), kIdO, (j | k) != 0);
+                        if (j + 1 == count[x]) {
+                            commit(o_full + 8 * x);
+                        } else {
+                            if (!k_here && !(ok = landed(kn))) break;
+                            k_here = true;
+                            scores(x, kn);
+                            if (j + 2 == count[x]) commit(q_empty + 8 * x);
+                        }
+                    }
+                    if (!ok) break;
+                    commit(empty + 8 * slot(vn));
+                    if (j + 1 < blocks) commit(empty + 8 * slot(kn));
+                }
+                base += 2 * blocks;
+            }
+            if (!ok) {  // let what was issued end before tensor memory is given back
+                commit(drain_bar);
+                bar_wait(drain_bar, 0);
+            }
+        } else if (warp == kTcLoadWarp) {
+            // ------------------------------------------------------- loads
+            uint32_t n = 0;  // ring tiles issued
+            uint32_t q_phase[kTcSubs] = {1, 1}, tail_phase = 0;
+            const bool paged = a.kv.table != nullptr;
+            const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys, piece = min(page_size, kTcKeys);
+            const int pieces = kTcKeys / piece;
+            uint32_t q_bytes = 0;
+            auto load_q = [&](int x) {
+                const TcSub me(plan, it, x);
+                if (min(b1, me.blocks) <= it.b0) return true;
+                if (!warp_wait(q_empty + 8 * x, q_phase[x])) return false;
+                q_phase[x] ^= 1;
+                if (lane == 0) {
+                    bar_expect(q_full + 8 * x, q_bytes);
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c)
+                        tma3(q_s + x * C::kTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
+                }
+                return true;
+            };
+            q_bytes = (uint32_t)(sub * a.group) * D * 2;
+            // page of the piece that this lane copies of block b
+            auto page_of = [&](int b) {
+                const int j = b * kTcKeys + lane * piece;
+                if (!paged || lane >= pieces || j >= it.q.keys) return -1;
+                const int page = __ldg(a.kv.table + (int64_t)it.s * a.kv.max_pages + (j >> a.kv.page_shift));
+                if (page >= 0 && page < a.kv.page_count) return page;
+                report(a.status, kStatusBadMetadata);
+                return a.kv.page_count;  // outside the map: zeros
+            };
+            auto load_tile = [&](const CUtensorMap *map, int b, int page, bool values) {
+                const uint32_t st = n % NS;
+                if (n >= NS && !warp_wait(empty + 8 * st, ((n / NS) & 1) ^ 1)) return false;
+                const int j0 = b * kTcKeys, left = it.q.keys - j0;
+                // the rows behind the last key: zeros, so that no stale NaN
+                // meets a weight of 0
+                const bool tail = values && left < kTcKeys;
+                const uint32_t bar = tail ? tail_bar : full + 8 * st, dst = ring + st * C::kTile;
+                const int live = paged ? min(pieces, max(0, (left + piece - 1) / piece)) : 1;
+                if (lane == 0) {
+                    if (live > 0)
+                        bar_expect(bar, (uint32_t)(live * piece) * D * 2);
+                    else if (!tail)
+                        bar_arrive(bar);
+                }
+                __syncwarp();
+                if (lane < live) {
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        const uint32_t to = dst + c * C::kHalf + (uint32_t)(lane * piece) * 128u;
+                        if (paged)
+                            tma4(to, map, 64 * c, it.h, (j0 + lane * piece) & (page_size - 1), page, bar);
+                        else
+                            tma4(to, map, 64 * c, it.h, it.q.row0 + j0, 0, bar);
+                    }
+                }
+                if (tail) {
+                    if (live > 0) {
+                        if (!warp_wait(tail_bar, tail_phase)) return false;
+                        tail_phase ^= 1;
+                    }
+                    for (int row = max(0, left) + (lane >> 3); row < kTcKeys; row += 4)
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * C::kHalf + (uint32_t)row * 128u + (lane & 7) * 16u),
+                                         "r"(0u)
+                                         : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(full + 8 * st);
+                }
+                ++n;
+                return true;
+            };
+            for (; ok && segment(&b1); it.next(plan)) {
+                ok = load_q(0);
+                for (int b = it.b0; ok && b < b1; ++b) {
+                    const int page = page_of(b);
+                    ok = load_tile(&maps.k, b, page, false);
+                    if (ok && b == it.b0) ok = load_q(1);
+                    if (ok) ok = load_tile(&maps.v, b, page, true);
+                }
+            }
+            if (!ok) {  // copies in flight land before the CTA ends
+                const uint32_t from = n > NS ? n - NS : 0;
+                for (uint32_t i = from; i < n; ++i) bar_wait(full + 8 * (i % NS), (i / NS) & 1);
+                for (int x = 0; x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
+            }
+        }
+    }
+    if (!ok && lane == 0) report(a.status, kStatusAttentionWait);
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == kTcMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+// Joins the partials of pairs cut between CTAs; the boundaries inside one
+// pair share its rows.  Partials are added in order.
+constexpr int kTcMergeThreads = 256;
+
+template <typename T, typename KT, int D>
+__global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials, int sub, int ctas)
+{
+    using C = Tc<D>;
+    __shared__ float row_q[kTcMergeThreads / 32][D];
+    const int c = blockIdx.x + 1, x = blockIdx.y, warp = threadIdx.x >> 5;
+    const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
+    long long total;
+    const TcFound f = tc_find<kTcMergeThreads>(plan, &total, [&](long long n) { return TcDeal(n, ctas).first(c); });
+    // also by CTAs with nothing to join: the next launch of the stream follows this one
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const TcDeal deal(total, ctas);
+    const long long u = deal.first(c);
+    if (u >= total) return;
+    TcIter it;
+    it.begin(plan, f.s, f.rel, u);
+    if (it.b0 == 0) return;  // no pair is cut here
+    const int c0 = deal.holder(it.origin + kTcOver), c1 = deal.holder(it.origin + kTcOver + (long long)kTcKeys * (it.blocks - 1));
+    const int slice = c - c0 - 1, slices = c1 - c0;
+    const TcSub me(plan, it, x);
+    constexpr int G = D / 16;  // 16-column pieces of a row
+    const int rows = me.tokens * a.group, work = kTcRows * G;
+    const int w0 = (int)((long long)work * slice / slices), w1 = (int)((long long)work * (slice + 1) / slices);
+    for (int first = (w0 & ~31) + 32 * warp; first < w1; first += kTcMergeThreads) {
+        const int w = first + (int)(threadIdx.x & 31), r = w % kTcRows, g = w / kTcRows;
+        const bool live = w >= w0 && w < w1 && r < rows;
+        float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = 0.f;
+        for (int p = c0; live && p <= c1; ++p) {
+            if (p > c0 && it.block_at(deal.first(p)) == it.block_at(deal.first(p + 1))) continue;  // no block of its own
+            const float *part = partials + (size_t)(2 * p + (p == c0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / kTcSubs);
+            const float pm = part[kTcRows * D + r], pl = part[kTcRows * D + kTcRows + r];
+            if (pm == -INFINITY) continue;
+            const float mn = fmaxf(m, pm), fo = m == -INFINITY ? 0.f : ex2(m - mn), fn = ex2(pm - mn);
+            m = mn;
+            l = l * fo + pl * fn;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = *(const float4 *)(part + ((4 * g + i) * kTcRows + r) * 4);
+                o[4 * i] = o[4 * i] * fo + v.x * fn;
+                o[4 * i + 1] = o[4 * i + 1] * fo + v.y * fn;
+                o[4 * i + 2] = o[4 * i + 2] * fo + v.z * fn;
+                o[4 * i + 3] = o[4 * i + 3] * fo + v.w * fn;
+            }
+        }
+        const int token = r / a.group, head = it.h * a.group + r - token * a.group, token_row = it.q.row0 + me.token0 + token;
+        bool bad = false;
+        if (live) {
+            const bool none = it.q.keys - it.q.n + me.token0 + token + 1 <= 0;
+            const float inv = 1.f / l;
+            T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                o[i] = none ? 0.f : o[i] * inv;
+                bad |= !isfinite(o[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += Elem<T>::kVec) Elem<T>::store(out + i, o + i);
+        }
+        for (unsigned left = __ballot_sync(kFull, bad); left; left &= left - 1) {
+            const int who = __ffs(left) - 1;
+            const int row = __shfl_sync(kFull, token_row, who), hd = __shfl_sync(kFull, head, who), col = 16 * __shfl_sync(kFull, g, who);
+            __syncwarp();
+            attention_row<T, KT, D>(a, row, hd, it.s, it.q, row_q[warp], col, col + 16);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launch
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t encode_tiled(EncodeTiled *fn)
+{
+    static EncodeTiled have = nullptr;  // the same for every thread that looks it up
+    if (have == nullptr) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+        if (e != cudaSuccess) return e;
+        if (found != cudaDriverEntryPointSuccess || p == nullptr) return cudaErrorNotSupported;
+        have = (EncodeTiled)p;
+    }
+    *fn = have;
+    return cudaSuccess;
+}
+
+// 64-element wide boxes of 16-bit elements, 128-byte swizzle, zeros outside.
+template <typename KT>
+cudaError_t make_map(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims, const int64_t *strides, const cuuint32_t *box)
+{
+    EncodeTiled encode = nullptr;
+    const cudaError_t e = encode_tiled(&encode);
+    if (e != cudaSuccess) return e;
+    cuuint64_t bytes[3];
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank - 1; ++i) bytes[i] = (cuuint64_t)strides[i] * 2;
+    const CUresult r = encode(map, std::is_same<KT, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              (cuuint32_t)rank, const_cast<void *>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t s)
+{
+    using C = Tc<D>;
+    const int sub = kTcRows / a.group;
+    TcMaps maps;
+    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
+    const int64_t qs[2] = {D, a.q_ld};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)a.group, (cuuint32_t)sub};
+    cudaError_t e = make_map<T>(&maps.q, a.q, 3, qd, qs, qb);
+    const bool paged = a.kv.table != nullptr;
+    const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys;
+    const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.kv_heads, paged ? (cuuint64_t)page_size : (cuuint64_t)a.tokens,
+                              paged ? (cuuint64_t)a.kv.page_count : 1};
+    const int64_t ks[3] = {a.kv.head, a.kv.k_pos, paged ? a.kv.page : a.kv.k_pos}, vs[3] = {a.kv.head, a.kv.v_pos, paged ? a.kv.page : a.kv.v_pos};
+    const cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
+    if (e == cudaSuccess) e = make_map<T>(&maps.k, a.kv.k, 4, kd, ks, kb);
+    if (e == cudaSuccess) e = make_map<T>(&maps.v, a.kv.v, 4, kd, vs, kb);
+    int dev = 0, sms = 0;
+    if (e == cudaSuccess) e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_attention_kernel<T, T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    if (e != cudaSuccess) return e;
+    const int64_t keys = paged ? (int64_t)a.kv.max_pages << a.kv.page_shift : a.tokens, blocks = (keys + kTcKeys - 1) / kTcKeys;
+    const int64_t pairs = a.tokens / (sub * kTcSubs) + a.sequences, most = pairs * a.kv_heads * blocks;
+    const int ctas = (int)(most < sms ? most : sms);
+    const bool split = ctas > 1 && blocks > 1;
+    float *partials = nullptr;
+    if (split) e = stream_alloc((void **)&partials, (size_t)2 * ctas * C::kPartial * sizeof(float), s);
+    if (e != cudaSuccess) return e;
+    tc_attention_kernel<T, T, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, sub, partials);
+    e = cudaGetLastError();
+    if (!split) return e;
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)ctas - 1, kTcSubs);
+        cfg.blockDim = dim3(kTcMergeThreads);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, T, D>, a, (const float *)partials, sub, ctas);
+    }
+    const cudaError_t f = stream_free(partials, s);
+    return e != cudaSuccess ? e : f;
+}
+
+}  // namespace
+
+cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s)
+{
+    if (a.type != a.kv_type) return cudaErrorInvalidValue;
+    if (a.type == kTypeF16) return a.head_dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+    if (a.type == kTypeBF16) return a.head_dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace qmv
