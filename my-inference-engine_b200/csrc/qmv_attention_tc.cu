@@ -28,6 +28,10 @@
 #include "qmv_attention.cuh"
 #include "qmv_internal.h"
 
+#ifndef QMV_P128
+#define QMV_P128 2
+#define QMV_P64 3
+#endif
 namespace qmv {
 
 namespace {
@@ -38,7 +42,7 @@ constexpr int kTcSubs = 2;       // tiles of a CTA
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; 8: MMA; 9: loads
 constexpr int kTcMmaWarp = 8, kTcLoadWarp = 9;
 // What a tile costs beside its keys, in keys.
-constexpr int kTcOver = 256;
+constexpr int kTcOver = 384;
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
@@ -120,26 +124,50 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// The MMA warp runs converged, so that descriptors stay in uniform registers;
+// one elected lane issues.  (With a single lane in the loop, each MMA took
+// 140 cycles to issue, twice what it takes to run.)
 __device__ __forceinline__ void commit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+        : "memory");
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+// d (+)= A B over 64 elements of the reduction, both operands in shared
+// memory, K-major: 16 elements are 32 bytes, 2 in a descriptor.
+__device__ __forceinline__ void mma_ss64(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+
+// The same with A (16-bit pairs, 8 columns for 16 elements) in tensor memory
+// and B MN-major: 16 rows of the reduction are 2048 bytes, 128 in a descriptor.
+__device__ __forceinline__ void mma_ts64(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred e, p, t;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+        "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
@@ -170,6 +198,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r)
         : "memory");
 }
 
+// 2^x for two x on the FMA pipe, to 2.6e-6 of the value (the weights keep 8 or
+// 11 bits): x = n + f with n the nearest whole number, read off the low bits of
+// x + 1.5 * 2^23, and a minimax polynomial of degree 4 (Remez, relative error) on |f| <= 1/2.  x
+// below -126 counts as -126.
+__device__ __forceinline__ float2 ex2_poly(float2 x)
+{
+    const float2 big = make_float2(12582912.f, 12582912.f);
+    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const float2 t = __fadd2_rn(x, big), n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 p = __ffma2_rn(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
+    p = __ffma2_rn(f, p, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = __ffma2_rn(f, p, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = __ffma2_rn(f, p, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 rows x 128
 // bytes, 1024 bytes apart along the rows).  K-major (Q, K): the contiguous
 // 64 elements run along the reduction.  MN-major (V): they run along the
@@ -189,6 +235,30 @@ template <typename KT> __host__ __device__ constexpr uint32_t idesc(int n, bool 
 {
     return (1u << 4) | (std::is_same<KT, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (mn_major ? 1u << 16 : 0u) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// 32 values of a row, whole 32-byte sectors a store where rows allow.
+template <typename T> __device__ __forceinline__ void store32(T *out, const float *o, bool wide)
+{
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 32 / (int)sizeof(T)) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (sizeof(T) == 4)
+                    w[j] = __float_as_uint(o[i + j]);
+                else
+                    w[j] = pack2<T>(o[i + 2 * j], o[i + 2 * j + 1]);
+            }
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + i), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                         "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += Elem<T>::kVec) Elem<T>::store(out + i, o + i);
+    }
 }
 
 // ------------------------------------------------------------------ work
@@ -356,8 +426,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     using C = Tc<D>;
     constexpr int NS = C::kSlots;
     constexpr float kLift = std::is_same<KT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
+    // of 8 exponentials, those on the FMA pipe beside the special-function unit
+    constexpr int kPoly = D == 128 ? QMV_P128 : QMV_P64;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * NS + 5 * kTcSubs + 2];
+    __shared__ __align__(8) unsigned long long bars[2 * NS + 6 * kTcSubs + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ float row_q[8][D];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -365,7 +437,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const uint32_t q_s = smem0, ring = smem0 + kTcSubs * C::kTile;
     const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
     const uint32_t full = bar0, empty = full + 8 * NS, q_full = empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
-                   s_full = q_empty + 8 * kTcSubs, p_full = s_full + 8 * kTcSubs, o_full = p_full + 8 * kTcSubs,
+                   s_full = q_empty + 8 * kTcSubs, p_full = s_full + 8 * kTcSubs, o_full = p_full + 16 * kTcSubs,
                    tail_bar = o_full + 8 * kTcSubs, drain_bar = tail_bar + 8;
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
 
@@ -378,7 +450,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             bar_init(q_full + 8 * x, 1);
             bar_init(q_empty + 8 * x, 1);
             bar_init(s_full + 8 * x, 1);
-            bar_init(p_full + 8 * x, 4);
+            bar_init(p_full + 16 * x, 4);  // the first and the second 64 keys of P
+            bar_init(p_full + 16 * x + 8, 4);
             bar_init(o_full + 8 * x, 1);
         }
         bar_init(tail_bar, 1);
@@ -413,7 +486,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
     if (warp < 8) {
         // --------------------------------------------------------- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
         const uint32_t s_t = lanes + 128u * x, o_t = lanes + 256u + 128u * x;
@@ -470,17 +543,17 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 e = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), f2, n2);
-                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                        const float2 w = i % 8 >= 8 - kPoly ? ex2_poly(e) : make_float2(ex2(e.x), ex2(e.y));
                         sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                         p[i] = pack2<KT>(w.x, w.y);
                     }
                     tmem_st32(s_t + 32 * h, p);
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(p_full + 16 * x + 8 * h);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(p_full + 8 * x);
             }
             if (!ok) break;
             if (me.tokens == 0) continue;
@@ -495,6 +568,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             if (whole) {
                 const float inv = 1.f / l;
                 const bool none = keys <= 0;
+                const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
                 T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D;
                 bool bad = false;
 #pragma unroll 1
@@ -507,10 +581,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         o[i] = none ? 0.f : o[i] * inv;
                         bad |= !isfinite(o[i]);
                     }
-                    if (row) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += Elem<T>::kVec) Elem<T>::store(out + c + i, o + i);
-                    }
+                    if (row) store32<T>(out + c, o, wide);
                 }
                 // a masked NaN or infinity met the sums: those rows again, without it
                 for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
@@ -538,21 +609,19 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             fence_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == kTcMmaWarp && lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == kTcMmaWarp) {
             // --------------------------------------------------- MMA issue
             constexpr uint32_t kIdS = idesc<KT>(128, false), kIdO = idesc<KT>(D, true);
+            const uint32_t tm = __shfl_sync(kFull, tmem, 0);
             uint32_t base = 0;  // ring tiles before this segment
             uint32_t q_phase[kTcSubs] = {0, 0}, p_phase[kTcSubs] = {0, 0};
-            auto slot = [&](uint32_t n) { return n % NS; };
-            auto landed = [&](uint32_t n) { return bar_wait(full + 8 * (n % NS), (n / NS) & 1); };
+            auto slot = [&](uint32_t n) { return __shfl_sync(kFull, n % NS, 0); };
+            auto landed = [&](uint32_t n) { return warp_wait(full + 8 * (n % NS), (n / NS) & 1); };
             auto scores = [&](int x, uint32_t n) {
-                const uint32_t qa = q_s + x * C::kTile, kb = ring + slot(n) * C::kTile;
+                const uint64_t qa = desc_k(q_s + x * C::kTile), kb = desc_k(ring + slot(n) * C::kTile);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k / 4) * C::kHalf + (k % 4) * 32;
-                    mma_ss(tmem + 128u * x, desc_k(qa + off), desc_k(kb + off), kIdS, k != 0);
-                }
+                for (int k = 0; k < D / 64; ++k) mma_ss64(tm + 128u * x, qa + k * (C::kHalf >> 4), kb + k * (C::kHalf >> 4), kIdS, k != 0);
                 commit(s_full + 8 * x);
             };
             for (; ok && segment(&b1); it.next(plan)) {
@@ -562,9 +631,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 for (int x = 0; x < kTcSubs; ++x) count[x] = max(0, min(b1, TcSub(plan, it, x).blocks) - b0);
                 // block j's K is ring tile base + 2 j, its V base + 2 j + 1
                 ok = landed(base);
-                for (int x = 0; ok && x < kTcSubs; ++x) {
-                    if (count[x] == 0) continue;
-                    if (!(ok = bar_wait(q_full + 8 * x, q_phase[x]))) break;
+#pragma unroll
+                for (int x = 0; x < kTcSubs; ++x) {
+                    if (!ok || count[x] == 0) continue;
+                    if (!(ok = warp_wait(q_full + 8 * x, q_phase[x]))) continue;
                     q_phase[x] ^= 1;
                     fence_after();
                     scores(x, base);
@@ -572,23 +642,26 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
                 if (!ok) break;
                 commit(empty + 8 * slot(base));
-                for (int j = 0; ok && j < blocks; ++j) {
+                for (int j = 0; j < blocks; ++j) {
                     const uint32_t kn = base + 2 * j + 2, vn = base + 2 * j + 1;
                     if (!(ok = landed(vn))) break;
+                    const uint64_t vb = desc_mn(ring + slot(vn) * C::kTile);
                     bool k_here = false;
-                    for (int x = 0; x < kTcSubs; ++x) {
-                        if (j >= count[x]) continue;
-                        if (!(ok = bar_wait(p_full + 8 * x, p_phase[x]))) break;
-                        p_phase[x] ^= 1;
-                        fence_after();
-                        const uint32_t vb = ring + slot(vn) * C::kTile;
 #pragma unroll
-                        for (int k = 0; k < kTcKeys / 16; ++k)
-                            mma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 8u * k, desc_mn(vb + 2048u * k), kIdO, (j | k) != 0);
+                    for (int x = 0; x < kTcSubs; ++x) {
+                        if (!ok || j >= count[x]) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (ok) ok = warp_wait(p_full + 16 * x + 8 * h, p_phase[x]);
+                            fence_after();
+                            if (ok) mma_ts64(tm + 256u + 128u * x, tm + 128u * x + 32u * h, vb + 512 * h, kIdO, (j | h) != 0);
+                        }
+                        p_phase[x] ^= 1;
+                        if (!ok) continue;
                         if (j + 1 == count[x]) {
                             commit(o_full + 8 * x);
                         } else {
-                            if (!k_here && !(ok = landed(kn))) break;
+                            if (!k_here && !(ok = landed(kn))) continue;
                             k_here = true;
                             scores(x, kn);
                             if (j + 2 == count[x]) commit(q_empty + 8 * x);
@@ -598,6 +671,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     commit(empty + 8 * slot(vn));
                     if (j + 1 < blocks) commit(empty + 8 * slot(kn));
                 }
+                if (!ok) break;
                 base += 2 * blocks;
             }
             if (!ok) {  // let what was issued end before tensor memory is given back
