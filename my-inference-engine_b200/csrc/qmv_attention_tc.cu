@@ -5,14 +5,23 @@
 // group of query heads, so a 128-row MMA tile holds 128 / group tokens with
 // all heads that read the same keys: the tile is full for any group, keys are
 // fetched once for the group, and the diagonal wastes few keys.  A CTA works
-// on two such tiles at once over the same keys, so that the tensor cores
-// multiply for one while its partner's softmax runs:
+// on two such tiles at once over the same blocks of 128 keys, so that the
+// tensor cores multiply for one while the other's softmax runs:
 //   S = Q K^T   tcgen05.mma, both operands in shared memory (TMA, 128-byte
 //               swizzle), 128 x 128 f32 in tensor memory;
-//   softmax     one thread a row: the whole row of S in registers, running
-//               reference m and sum l; P = 2^(S f - m) rounded to the values'
-//               16-bit type and stored over S in tensor memory;
+//   softmax     one thread a row: the row of S in registers, running reference
+//               m and sum l; P = 2^(S f - m) rounded to the values' 16-bit type
+//               and stored to tensor memory;
 //   O += P V    tcgen05.mma, P from tensor memory, V from shared memory.
+// S is needed only until it is in registers, so the next scores are multiplied
+// while the exponentials run: head_dim 128 has room for one S that the two
+// tiles use in turn (S 128 columns, P 2 x 64, O 2 x 128), head_dim 64 for one
+// each.  An MMA holds its issuer until the tensor cores take it, so one warp
+// issues the QK and another the PV products, and the waits of one hide behind
+// the other's work (with one issuer, 1450 of 3500 cycles a block were gaps).
+//  (With P over S a
+// softmax waited 950 to 1250 of 3250 cycles a block for its next scores; with
+// S in halves of 64 keys it did not wait, but the N = 64 MMAs ran at half rate.)
 // The reference m is the running maximum, but it is raised only when the
 // maximum passes it by 8 (a factor of 256; f32 sums and 16-bit floating
 // weights do not care), so O is rescaled a few times a row at most.
@@ -39,8 +48,8 @@ namespace {
 constexpr int kTcKeys = 128;     // keys of a block
 constexpr int kTcRows = 128;     // rows of a tile
 constexpr int kTcSubs = 2;       // tiles of a CTA
-constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; 8: MMA; 9: loads
-constexpr int kTcMmaWarp = 8, kTcLoadWarp = 9;
+constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; then
+constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
 // What a tile costs beside its keys, in keys.
 constexpr int kTcOver = 384;
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
@@ -49,8 +58,12 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 template <int D> struct Tc {
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
-    static constexpr int kSlots = (int)((220u * 1024u - kTcSubs * kTile) / kTile) > 6 ? 6 : (int)((220u * 1024u - kTcSubs * kTile) / kTile);
-    static constexpr uint32_t kSmem = (kTcSubs + kSlots) * kTile + 1024;
+    static constexpr int kSlots = D == 64 ? 4 : 2;  // blocks of K, and of V, in flight
+    static constexpr uint32_t kSmem = (kTcSubs + 2 * kSlots) * kTile + 1024;
+    static constexpr int kScores = D == 64 ? 2 : 1;  // S buffers
+    static __host__ __device__ constexpr uint32_t s_col(int x) { return kScores == 2 ? 128u * x : 0u; }
+    static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + 64u * x; }
+    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + 128u + (uint32_t)D * x; }
     static constexpr int kPartial = kTcSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
 };
 
@@ -429,36 +442,39 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     // of 8 exponentials, those on the FMA pipe beside the special-function unit
     constexpr int kPoly = D == 128 ? QMV_P128 : QMV_P64;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * NS + 6 * kTcSubs + 2];
+    __shared__ __align__(8) unsigned long long bars[4 * NS + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ float row_q[8][D];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = smem0, ring = smem0 + kTcSubs * C::kTile;
+    const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kTile, v_s = k_s + NS * C::kTile;
     const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t full = bar0, empty = full + 8 * NS, q_full = empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
-                   s_full = q_empty + 8 * kTcSubs, p_full = s_full + 8 * kTcSubs, o_full = p_full + 16 * kTcSubs,
-                   tail_bar = o_full + 8 * kTcSubs, drain_bar = tail_bar + 8;
+    const uint32_t k_full = bar0, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, q_full = v_empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
+                   s_full = q_empty + 8 * kTcSubs, s_free = s_full + 8 * kTcSubs, p_full = s_free + 8 * kTcSubs,
+                   pv_done = p_full + 8 * kTcSubs, tail_bar = pv_done + 8 * kTcSubs, drain_bar = tail_bar + 8;
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
 
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
-            bar_init(full + 8 * i, 1);
-            bar_init(empty + 8 * i, 1);
+            bar_init(k_full + 8 * i, 1);
+            bar_init(k_empty + 8 * i, 1);
+            bar_init(v_full + 8 * i, 1);
+            bar_init(v_empty + 8 * i, 1);
         }
         for (int x = 0; x < kTcSubs; ++x) {
             bar_init(q_full + 8 * x, 1);
             bar_init(q_empty + 8 * x, 1);
             bar_init(s_full + 8 * x, 1);
-            bar_init(p_full + 16 * x, 4);  // the first and the second 64 keys of P
-            bar_init(p_full + 16 * x + 8, 4);
-            bar_init(o_full + 8 * x, 1);
+            bar_init(s_free + 8 * x, 4);
+            bar_init(p_full + 8 * x, 4);
+            bar_init(pv_done + 8 * x, 1);
         }
         bar_init(tail_bar, 1);
         bar_init(drain_bar, 1);
+        bar_init(drain_bar + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kTcMmaWarp) {
+    if (warp == kTcQkWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_slot)),
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -489,8 +505,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
-        const uint32_t s_t = lanes + 128u * x, o_t = lanes + 256u + 128u * x;
-        uint32_t s_phase = 0, o_phase = 0;
+        const uint32_t s_t = lanes + C::s_col(x), p_t = lanes + C::p_col(x), o_t = lanes + C::o_col(x);
+        uint32_t done = 0;  // blocks of this tile slot handed over so far
         for (; ok && segment(&b1); it.next(plan)) {
             const TcSub me(plan, it, x);
             const int end = min(b1, me.blocks), token = r / a.group;
@@ -501,13 +517,15 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const float f = row ? a.scale * kLog2e : 0.f;
             float m = -INFINITY, l = 0.f;
             for (int b = it.b0; b < end; ++b) {
-                if (!(ok = warp_wait(s_full + 8 * x, s_phase))) break;
-                s_phase ^= 1;
+                if (!(ok = warp_wait(s_full + 8 * x, done & 1))) break;
                 fence_after();
                 float s[128];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tmem_ld32(s_t + 32 * i, s + 32 * i);
                 wait_ld();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
                 const int j0 = b * kTcKeys;
                 if (__any_sync(kFull, j0 + kTcKeys > lim)) {
 #pragma unroll
@@ -518,7 +536,13 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
                 for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
-                if (__any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise))) {
+                const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
+                // P and O as the block before this one left them
+                if (done > 0) {
+                    if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
+                    fence_after();
+                }
+                if (raise) {
                     const float mn = fmaxf(m, mx), fix = m == -INFINITY ? 0.f : ex2(m - mn);
                     m = mn;
                     l *= fix;
@@ -547,20 +571,20 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                         p[i] = pack2<KT>(w.x, w.y);
                     }
-                    tmem_st32(s_t + 32 * h, p);
-                    wait_st();
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(p_full + 16 * x + 8 * h);
+                    tmem_st32(p_t + 32 * h, p);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full + 8 * x);
+                ++done;
             }
             if (!ok) break;
             if (me.tokens == 0) continue;
             const bool any = end > it.b0;  // this segment holds blocks of this tile
             if (any) {
-                if (!(ok = warp_wait(o_full + 8 * x, o_phase))) break;
-                o_phase ^= 1;
+                if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
                 fence_after();
             }
             const bool whole = it.b0 == 0 && b1 == it.blocks;
@@ -610,96 +634,93 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == kTcMmaWarp) {
-            // --------------------------------------------------- MMA issue
-            constexpr uint32_t kIdS = idesc<KT>(128, false), kIdO = idesc<KT>(D, true);
+        uint32_t slot = 0, phase = 0;  // of this warp's next block of K or V
+        auto step = [&]() {
+            if (++slot == NS) {
+                slot = 0;
+                phase ^= 1;
+            }
+        };
+        if (warp == kTcQkWarp) {
+            // ----------------------------------------------------- S = Q K^T
+            constexpr uint32_t kId = idesc<KT>(128, false);
             const uint32_t tm = __shfl_sync(kFull, tmem, 0);
-            uint32_t base = 0;  // ring tiles before this segment
-            uint32_t q_phase[kTcSubs] = {0, 0}, p_phase[kTcSubs] = {0, 0};
-            auto slot = [&](uint32_t n) { return __shfl_sync(kFull, n % NS, 0); };
-            auto landed = [&](uint32_t n) { return warp_wait(full + 8 * (n % NS), (n / NS) & 1); };
-            auto scores = [&](int x, uint32_t n) {
-                const uint64_t qa = desc_k(q_s + x * C::kTile), kb = desc_k(ring + slot(n) * C::kTile);
-#pragma unroll
-                for (int k = 0; k < D / 64; ++k) mma_ss64(tm + 128u * x, qa + k * (C::kHalf >> 4), kb + k * (C::kHalf >> 4), kIdS, k != 0);
-                commit(s_full + 8 * x);
-            };
+            uint32_t q_phase[kTcSubs] = {0, 0}, s_phase[kTcSubs] = {1, 1};  // s_phase: of each S buffer
             for (; ok && segment(&b1); it.next(plan)) {
-                const int b0 = it.b0, blocks = b1 - b0;
-                int count[kTcSubs];
+                int end[kTcSubs];  // of the blocks of each tile
 #pragma unroll
-                for (int x = 0; x < kTcSubs; ++x) count[x] = max(0, min(b1, TcSub(plan, it, x).blocks) - b0);
-                // block j's K is ring tile base + 2 j, its V base + 2 j + 1
-                ok = landed(base);
-#pragma unroll
-                for (int x = 0; x < kTcSubs; ++x) {
-                    if (!ok || count[x] == 0) continue;
-                    if (!(ok = warp_wait(q_full + 8 * x, q_phase[x]))) continue;
-                    q_phase[x] ^= 1;
-                    fence_after();
-                    scores(x, base);
-                    if (count[x] == 1) commit(q_empty + 8 * x);
-                }
-                if (!ok) break;
-                commit(empty + 8 * slot(base));
-                for (int j = 0; j < blocks; ++j) {
-                    const uint32_t kn = base + 2 * j + 2, vn = base + 2 * j + 1;
-                    if (!(ok = landed(vn))) break;
-                    const uint64_t vb = desc_mn(ring + slot(vn) * C::kTile);
-                    bool k_here = false;
+                for (int x = 0; x < kTcSubs; ++x) end[x] = min(b1, TcSub(plan, it, x).blocks);
+                for (int b = it.b0; b < b1; ++b) {
+                    if (!(ok = warp_wait(k_full + 8 * slot, phase))) break;
+                    const uint64_t kb = desc_k(k_s + __shfl_sync(kFull, slot, 0) * C::kTile);
 #pragma unroll
                     for (int x = 0; x < kTcSubs; ++x) {
-                        if (!ok || j >= count[x]) continue;
+                        if (!ok || b >= end[x]) continue;
+                        if (b == it.b0) {
+                            ok = warp_wait(q_full + 8 * x, q_phase[x]);
+                            q_phase[x] ^= 1;
+                        }
+                        constexpr int kBuf = C::kScores - 1;
+                        if (!ok || !(ok = warp_wait(s_free + 8 * (kBuf * x), s_phase[kBuf * x]))) continue;
+                        s_phase[kBuf * x] ^= 1;
+                        fence_after();
+                        const uint64_t qa = desc_k(q_s + x * C::kTile);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (ok) ok = warp_wait(p_full + 16 * x + 8 * h, p_phase[x]);
-                            fence_after();
-                            if (ok) mma_ts64(tm + 256u + 128u * x, tm + 128u * x + 32u * h, vb + 512 * h, kIdO, (j | h) != 0);
-                        }
-                        p_phase[x] ^= 1;
-                        if (!ok) continue;
-                        if (j + 1 == count[x]) {
-                            commit(o_full + 8 * x);
-                        } else {
-                            if (!k_here && !(ok = landed(kn))) continue;
-                            k_here = true;
-                            scores(x, kn);
-                            if (j + 2 == count[x]) commit(q_empty + 8 * x);
-                        }
+                        for (int k = 0; k < D / 64; ++k)
+                            mma_ss64(tm + C::s_col(x), qa + k * (C::kHalf >> 4), kb + k * (C::kHalf >> 4), kId, k != 0);
+                        commit(s_full + 8 * x);
+                        if (b + 1 == end[x]) commit(q_empty + 8 * x);
                     }
                     if (!ok) break;
-                    commit(empty + 8 * slot(vn));
-                    if (j + 1 < blocks) commit(empty + 8 * slot(kn));
+                    commit(k_empty + 8 * slot);
+                    step();
                 }
-                if (!ok) break;
-                base += 2 * blocks;
             }
             if (!ok) {  // let what was issued end before tensor memory is given back
                 commit(drain_bar);
                 bar_wait(drain_bar, 0);
             }
-        } else if (warp == kTcLoadWarp) {
-            // ------------------------------------------------------- loads
-            uint32_t n = 0;  // ring tiles issued
-            uint32_t q_phase[kTcSubs] = {1, 1}, tail_phase = 0;
-            const bool paged = a.kv.table != nullptr;
-            const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys, piece = min(page_size, kTcKeys);
-            const int pieces = kTcKeys / piece;
-            uint32_t q_bytes = 0;
-            auto load_q = [&](int x) {
-                const TcSub me(plan, it, x);
-                if (min(b1, me.blocks) <= it.b0) return true;
-                if (!warp_wait(q_empty + 8 * x, q_phase[x])) return false;
-                q_phase[x] ^= 1;
-                if (lane == 0) {
-                    bar_expect(q_full + 8 * x, q_bytes);
+        } else if (warp == kTcPvWarp) {
+            // ------------------------------------------------------ O += P V
+            constexpr uint32_t kId = idesc<KT>(D, true);
+            const uint32_t tm = __shfl_sync(kFull, tmem, 0);
+            uint32_t p_phase[kTcSubs] = {0, 0};
+            for (; ok && segment(&b1); it.next(plan)) {
+                int end[kTcSubs];
 #pragma unroll
-                    for (int c = 0; c < D / 64; ++c)
-                        tma3(q_s + x * C::kTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
+                for (int x = 0; x < kTcSubs; ++x) end[x] = min(b1, TcSub(plan, it, x).blocks);
+                for (int b = it.b0; b < b1; ++b) {
+                    if (!(ok = warp_wait(v_full + 8 * slot, phase))) break;
+                    const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kTile);
+#pragma unroll
+                    for (int x = 0; x < kTcSubs; ++x) {
+                        if (!ok || b >= end[x]) continue;
+                        if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
+                        p_phase[x] ^= 1;
+                        fence_after();
+                        mma_ts64(tm + C::o_col(x), tm + C::p_col(x), vb, kId, b != it.b0);
+                        mma_ts64(tm + C::o_col(x), tm + C::p_col(x) + 32u, vb + (64 * 128 >> 4), kId, 1u);
+                        commit(pv_done + 8 * x);
+                    }
+                    if (!ok) break;
+                    commit(v_empty + 8 * slot);
+                    step();
                 }
-                return true;
-            };
-            q_bytes = (uint32_t)(sub * a.group) * D * 2;
+            }
+            if (!ok) {
+                commit(drain_bar + 8);
+                bar_wait(drain_bar + 8, 0);
+            }
+        } else {
+            // ------------------------------------------------------- loads
+            const bool values = warp == kTcLoadVWarp;
+            const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty, tiles = values ? v_s : k_s;
+            const CUtensorMap *map = values ? &maps.v : &maps.k;
+            const bool paged = a.kv.table != nullptr;
+            const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys, piece = min(page_size, kTcKeys), pieces = kTcKeys / piece;
+            const uint32_t q_bytes = (uint32_t)(sub * a.group) * D * 2;
+            uint32_t issued = 0, q_phase[kTcSubs] = {1, 1}, tail_phase = 0;
+            phase = 1;  // of the empty barriers
             // page of the piece that this lane copies of block b
             auto page_of = [&](int b) {
                 const int j = b * kTcKeys + lane * piece;
@@ -709,63 +730,72 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 report(a.status, kStatusBadMetadata);
                 return a.kv.page_count;  // outside the map: zeros
             };
-            auto load_tile = [&](const CUtensorMap *map, int b, int page, bool values) {
-                const uint32_t st = n % NS;
-                if (n >= NS && !warp_wait(empty + 8 * st, ((n / NS) & 1) ^ 1)) return false;
-                const int j0 = b * kTcKeys, left = it.q.keys - j0;
-                // the rows behind the last key: zeros, so that no stale NaN
-                // meets a weight of 0
-                const bool tail = values && left < kTcKeys;
-                const uint32_t bar = tail ? tail_bar : full + 8 * st, dst = ring + st * C::kTile;
-                const int live = paged ? min(pieces, max(0, (left + piece - 1) / piece)) : 1;
-                if (lane == 0) {
-                    if (live > 0)
-                        bar_expect(bar, (uint32_t)(live * piece) * D * 2);
-                    else if (!tail)
-                        bar_arrive(bar);
-                }
-                __syncwarp();
-                if (lane < live) {
-#pragma unroll
-                    for (int c = 0; c < D / 64; ++c) {
-                        const uint32_t to = dst + c * C::kHalf + (uint32_t)(lane * piece) * 128u;
-                        if (paged)
-                            tma4(to, map, 64 * c, it.h, (j0 + lane * piece) & (page_size - 1), page, bar);
-                        else
-                            tma4(to, map, 64 * c, it.h, it.q.row0 + j0, 0, bar);
-                    }
-                }
-                if (tail) {
-                    if (live > 0) {
-                        if (!warp_wait(tail_bar, tail_phase)) return false;
-                        tail_phase ^= 1;
-                    }
-                    for (int row = max(0, left) + (lane >> 3); row < kTcKeys; row += 4)
-#pragma unroll
-                        for (int c = 0; c < D / 64; ++c)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * C::kHalf + (uint32_t)row * 128u + (lane & 7) * 16u),
-                                         "r"(0u)
-                                         : "memory");
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(full + 8 * st);
-                }
-                ++n;
-                return true;
-            };
             for (; ok && segment(&b1); it.next(plan)) {
-                ok = load_q(0);
+                if (!values) {
+                    for (int x = 0; ok && x < kTcSubs; ++x) {
+                        const TcSub me(plan, it, x);
+                        if (min(b1, me.blocks) <= it.b0) continue;
+                        if (!(ok = warp_wait(q_empty + 8 * x, q_phase[x]))) break;
+                        q_phase[x] ^= 1;
+                        if (lane == 0) {
+                            bar_expect(q_full + 8 * x, q_bytes);
+#pragma unroll
+                            for (int c = 0; c < D / 64; ++c)
+                                tma3(q_s + x * C::kTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
+                        }
+                    }
+                }
+                int page = page_of(it.b0);
                 for (int b = it.b0; ok && b < b1; ++b) {
-                    const int page = page_of(b);
-                    ok = load_tile(&maps.k, b, page, false);
-                    if (ok && b == it.b0) ok = load_q(1);
-                    if (ok) ok = load_tile(&maps.v, b, page, true);
+                    const int page_next = b + 1 < b1 ? page_of(b + 1) : -1;
+                    if (!(ok = warp_wait(empty + 8 * slot, phase))) break;
+                    const int j0 = b * kTcKeys, left = it.q.keys - j0;
+                    // the rows behind the last value: zeros, so that no stale
+                    // NaN meets a weight of 0
+                    const bool tail = values && left < kTcKeys;
+                    const uint32_t bar = tail ? tail_bar : full + 8 * slot, dst = tiles + slot * C::kTile;
+                    const int live = paged ? min(pieces, max(0, (left + piece - 1) / piece)) : 1;
+                    if (lane == 0) {
+                        if (live > 0)
+                            bar_expect(bar, (uint32_t)(live * piece) * D * 2);
+                        else if (!tail)
+                            bar_arrive(bar);
+                    }
+                    __syncwarp();
+                    if (lane < live) {
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) {
+                            const uint32_t to = dst + c * C::kHalf + (uint32_t)(lane * piece) * 128u;
+                            if (paged)
+                                tma4(to, map, 64 * c, it.h, (j0 + lane * piece) & (page_size - 1), page, bar);
+                            else
+                                tma4(to, map, 64 * c, it.h, it.q.row0 + j0, 0, bar);
+                        }
+                    }
+                    if (tail) {
+                        if (live > 0) {
+                            if (!(ok = warp_wait(tail_bar, tail_phase))) break;
+                            tail_phase ^= 1;
+                        }
+                        for (int row = max(0, left) + (lane >> 3); row < kTcKeys; row += 4)
+#pragma unroll
+                            for (int c = 0; c < D / 64; ++c)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * C::kHalf + (uint32_t)row * 128u + (lane & 7) * 16u),
+                                             "r"(0u)
+                                             : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(full + 8 * slot);
+                    }
+                    page = page_next;
+                    ++issued;
+                    step();
                 }
             }
             if (!ok) {  // copies in flight land before the CTA ends
-                const uint32_t from = n > NS ? n - NS : 0;
-                for (uint32_t i = from; i < n; ++i) bar_wait(full + 8 * (i % NS), (i / NS) & 1);
-                for (int x = 0; x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
+                const uint32_t from = issued > NS ? issued - NS : 0;
+                for (uint32_t i = from; i < issued; ++i) bar_wait(full + 8 * (i % NS), (i / NS) & 1);
+                for (int x = 0; !values && x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
             }
         }
     }
@@ -773,7 +803,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == kTcMmaWarp) {
+    if (warp == kTcQkWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
