@@ -37,10 +37,6 @@
 #include "qmv_attention.cuh"
 #include "qmv_internal.h"
 
-#ifndef QMV_P128
-#define QMV_P128 2
-#define QMV_P64 3
-#endif
 namespace qmv {
 
 namespace {
@@ -50,12 +46,13 @@ constexpr int kTcRows = 128;     // rows of a tile
 constexpr int kTcSubs = 2;       // tiles of a CTA
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; then
 constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
-// What a tile costs beside its keys, in keys.
-constexpr int kTcOver = 384;
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
 template <int D> struct Tc {
+    // What a pair of tiles costs beside its keys, in keys: 4600 cycles at
+    // head_dim 64 and 6700 at 128, where 128 keys take 2560 and 2300.
+    static constexpr int kOver = D == 64 ? 256 : 384;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr int kSlots = D == 64 ? 4 : 2;  // blocks of K, and of V, in flight
@@ -211,24 +208,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r)
         : "memory");
 }
 
-// 2^x for two x on the FMA pipe, to 2.6e-6 of the value (the weights keep 8 or
-// 11 bits): x = n + f with n the nearest whole number, read off the low bits of
-// x + 1.5 * 2^23, and a minimax polynomial of degree 4 (Remez, relative error) on |f| <= 1/2.  x
-// below -126 counts as -126.
-__device__ __forceinline__ float2 ex2_poly(float2 x)
-{
-    const float2 big = make_float2(12582912.f, 12582912.f);
-    x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const float2 t = __fadd2_rn(x, big), n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-    float2 p = __ffma2_rn(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
-    p = __ffma2_rn(f, p, make_float2(0.240247443318367f, 0.240247443318367f));
-    p = __ffma2_rn(f, p, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    p = __ffma2_rn(f, p, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-
 // Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 rows x 128
 // bytes, 1024 bytes apart along the rows).  K-major (Q, K): the contiguous
 // 64 elements run along the reduction.  MN-major (V): they run along the
@@ -276,84 +255,57 @@ template <typename T> __device__ __forceinline__ void store32(T *out, const floa
 
 // ------------------------------------------------------------------ work
 
+// Division by a number the host knows: its floor(2^64 / d) + 1 (exact for
+// dividends below 2^31; within 1 above, and corrected).
+struct Divisor {
+    unsigned long long magic;
+    int d;
+};
+
 struct TcPlan {
     const int *start, *length;
-    int sequences, tokens, max_keys, kv_heads;
-    int sub, wide;  // tokens of a tile and of a CTA's pair of tiles
+    int sequences, tokens, max_keys, kv_heads, over;
+    int sub;       // tokens of a tile
+    Divisor wide;  // tokens of a CTA's pair of tiles
+    Divisor ctas;
     __device__ __forceinline__ Seq seq(int s) const { return load_sequence(start, length, s, tokens, max_keys); }
-    // Pair i of a sequence spans kTcOver + the keys its last token sees (at
+    // Pair i of a sequence spans over + the keys its last token sees (at
     // least 1) places; the first k pairs of a head span:
     __device__ __forceinline__ long long before(const Seq &q, int k) const
     {
-        const long long c = (q.keys > q.n ? q.keys - q.n : 0) + kTcOver, all = (long long)k * wide;
-        return (long long)k * c + (long long)wide * ((long long)k * (k + 1) / 2) - (all > q.n ? all - q.n : 0);
+        const long long c = (q.keys > q.n ? q.keys - q.n : 0) + over, all = (long long)k * wide.d;
+        return (long long)k * c + (all * (k + 1) >> 1) - (all > q.n ? all - q.n : 0);
     }
-    __device__ __forceinline__ int pairs(const Seq &q) const { return (q.n + wide - 1) / wide; }
+    __device__ __forceinline__ int pairs(const Seq &q) const { return (int)__umul64hi((unsigned long long)(q.n + wide.d - 1), wide.magic); }
     __device__ __forceinline__ long long cost(const Seq &q) const { return before(q, pairs(q)) * kv_heads; }
 };
 
+// How `total` places are dealt to the CTAs in order: the first total % ctas
+// get one more.
 struct TcDeal {
-    long long each, more;
-    __device__ __forceinline__ TcDeal(long long total, int ctas) : each(total / ctas), more(total - each * ctas) {}
-    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
-    __device__ __forceinline__ int holder(long long u) const
+    long long each;
+    int more;
+    static __device__ __forceinline__ TcDeal of(long long total, const Divisor &d)
     {
-        const long long big = more * (each + 1);
-        return u < big ? (int)(u / (each + 1)) : (int)(more + (u - big) / each);
+        TcDeal t;
+        t.each = (long long)__umul64hi((unsigned long long)total, d.magic);
+        if (t.each * d.d > total) --t.each;
+        t.more = (int)(total - t.each * d.d);
+        return t;
     }
+    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
 };
-
-struct TcFound {
-    int s;
-    long long rel;
-};
-
-// The cost of the whole launch and the sequence that holds place
-// share(total), by all NT threads of the CTA together.
-template <int NT, typename F> __device__ __forceinline__ TcFound tc_find(const TcPlan &p, long long *total, const F &share)
-{
-    __shared__ TcFound found;
-    __shared__ long long scratch[NT / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = (p.sequences + NT - 1) / NT, s0 = min((int)threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
-    long long v = 0;
-    for (int s = s0; s < s1; ++s) v += p.cost(p.seq(s));
-    long long x = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(kFull, x, d);
-        if (lane >= d) x += y;
-    }
-    if (threadIdx.x == 0) found = TcFound{p.sequences, 0};
-    if (lane == 31) scratch[warp] = x;
-    __syncthreads();
-    long long base = 0, all = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) base += scratch[w];
-        all += scratch[w];
-    }
-    *total = all;
-    long long at = base + x - v;
-    const long long want = share(all);
-    if (want >= at && want < at + v) {
-        int s = s0;
-        for (long long c; want >= at + (c = p.cost(p.seq(s))); ++s) at += c;
-        found = TcFound{s, want - at};
-    }
-    __syncthreads();
-    return found;
-}
 
 // Walks the pairs of tiles in order: sequence, head, pair.  Key block b of a
-// pair lies at place origin + kTcOver + 128 b; a CTA has the blocks whose
-// places fall in its share.
+// pair lies at place origin + over + 128 b; a CTA has the blocks whose places
+// fall in its share.
 struct TcIter {
     Seq q;
     int s, h, i, pairs, b0, blocks;
     long long origin;
     __device__ __forceinline__ void size(const TcPlan &p)
     {
-        const int keys = q.keys - q.n + min((i + 1) * p.wide, q.n);
+        const int keys = q.keys - q.n + min((i + 1) * p.wide.d, q.n);
         blocks = keys > 0 ? (keys + kTcKeys - 1) / kTcKeys : 1;
     }
     __device__ __forceinline__ void enter(const TcPlan &p)
@@ -368,7 +320,8 @@ struct TcIter {
     }
     __device__ __forceinline__ void next(const TcPlan &p)
     {
-        origin += p.before(q, i + 1) - p.before(q, i);
+        // (before(i + 1) - before(i), without the products)
+        origin += (q.keys > q.n ? q.keys - q.n : 0) + p.over + min((i + 1) * p.wide.d, q.n);
         b0 = 0;
         if (++i == pairs) {
             i = 0;
@@ -380,40 +333,91 @@ struct TcIter {
         }
         if (pairs) size(p);
     }
-    // The first block at or behind place u, which is place rel of sequence s_.
-    __device__ __forceinline__ void begin(const TcPlan &p, int s_, long long rel, long long u)
+    // The first block at or behind place u, which is place rel of sequence s_
+    // (one with pairs).
+    __device__ __forceinline__ void begin(const TcPlan &p, int s_, const Seq &q_, long long rel, long long u)
     {
         s = s_;
-        enter(p);
-        h = i = b0 = 0;
-        blocks = 1;
-        origin = u;
-        if (pairs == 0) return;
+        q = q_;
+        pairs = p.pairs(q);
         const long long head = p.before(q, pairs);
-        h = (int)(rel / head);
+        h = min(p.kv_heads - 1, (int)((float)rel / (float)head));
+        while (h * head > rel) --h;
+        while ((h + 1) * head <= rel) ++h;
         rel -= h * head;
-        int lo = 0, hi = pairs - 1;  // the last pair that starts at or before rel
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (p.before(q, mid) <= rel)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        i = lo;
-        const long long at = rel - p.before(q, i);
-        origin = u - at;
+        // the last pair i with before(i) <= rel: the root of before's
+        // quadratic, then exactly
+        const float c = (float)((q.keys > q.n ? q.keys - q.n : 0) + p.over) + 0.5f * (float)p.wide.d;
+        i = (int)((sqrtf(c * c + 2.f * (float)p.wide.d * (float)rel) - c) / (float)p.wide.d);
+        i = min(max(i, 0), pairs - 1);
+        while (i > 0 && p.before(q, i) > rel) --i;
+        while (i + 1 < pairs && p.before(q, i + 1) <= rel) ++i;
+        origin = u - (rel - p.before(q, i));
         size(p);
-        b0 = block_at(u);
+        b0 = block_at(p, u);
         if (b0 >= blocks) next(p);
     }
     // The first block at or behind place u.
-    __device__ __forceinline__ int block_at(long long u) const
+    __device__ __forceinline__ int block_at(const TcPlan &p, long long u) const
     {
-        const long long k = u - origin - kTcOver;
+        const long long k = u - origin - p.over;
         return k <= 0 ? 0 : (int)min((k + kTcKeys - 1) / kTcKeys, (long long)blocks);
     }
 };
+
+// Where CTA c's share of the whole launch begins, and its places [u0, u1), by
+// all threads of the CTA together: a thread sums the cost of a run of
+// sequences, and the one whose run holds the place walks to it.
+struct TcStart {
+    TcIter it;  // it.s == sequences: nothing
+    long long u0, u1;
+};
+
+template <int NT> __device__ __forceinline__ void tc_find(const TcPlan &p, int c, TcStart *out)
+{
+    __shared__ long long scratch[NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = p.sequences <= NT ? 1 : (p.sequences + NT - 1) / NT, s0 = min((int)threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
+    long long v = 0;
+    Seq q{0, 0, 0};
+    for (int s = s0; s < s1; ++s) {
+        q = p.seq(s);
+        v += p.cost(q);
+    }
+    long long x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    long long base = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) base += scratch[w];
+        all += scratch[w];
+    }
+    const TcDeal deal = TcDeal::of(all, p.ctas);
+    const long long u0 = deal.first(c), u1 = deal.first(c + 1);
+    long long at = base + x - v;
+    if (u0 >= u1) {
+        if (threadIdx.x == 0) {
+            out->it.s = p.sequences;
+            out->u0 = out->u1 = 0;
+        }
+    } else if (u0 >= at && u0 < at + v) {
+        int s = s0;
+        if (per > 1)
+            for (long long cost; u0 >= at + (cost = p.cost(q = p.seq(s))); ++s) at += cost;
+        TcIter it;
+        it.begin(p, s, q, u0 - at, u0);
+        out->it = it;
+        out->u0 = u0;
+        out->u1 = u1;
+    }
+    __syncthreads();
+}
 
 // One tile of a pair: its tokens and key blocks.
 struct TcSub {
@@ -421,7 +425,7 @@ struct TcSub {
     int blocks;          // that any of its rows sees (at least 1 when it has tokens)
     __device__ __forceinline__ TcSub(const TcPlan &p, const TcIter &it, int x)
     {
-        token0 = it.i * p.wide + x * p.sub;
+        token0 = it.i * p.wide.d + x * p.sub;
         tokens = max(0, min(p.sub, it.q.n - token0));
         const int keys = it.q.keys - it.q.n + token0 + tokens;
         blocks = tokens == 0 ? 0 : keys > 0 ? (keys + kTcKeys - 1) / kTcKeys : 1;
@@ -434,16 +438,16 @@ struct TcMaps {
 
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
-tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, int sub, float *__restrict__ partials)
+tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, const __grid_constant__ TcPlan plan,
+                    float *__restrict__ partials, TcStart *__restrict__ starts)
 {
     using C = Tc<D>;
     constexpr int NS = C::kSlots;
     constexpr float kLift = std::is_same<KT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
-    // of 8 exponentials, those on the FMA pipe beside the special-function unit
-    constexpr int kPoly = D == 128 ? QMV_P128 : QMV_P64;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) unsigned long long bars[4 * NS + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
+    __shared__ TcStart begin;
     __shared__ float row_q[8][D];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
@@ -452,7 +456,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const uint32_t k_full = bar0, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, q_full = v_empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
                    s_full = q_empty + 8 * kTcSubs, s_free = s_full + 8 * kTcSubs, p_full = s_free + 8 * kTcSubs,
                    pv_done = p_full + 8 * kTcSubs, tail_bar = pv_done + 8 * kTcSubs, drain_bar = tail_bar + 8;
-    const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
 
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
@@ -479,22 +482,19 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
-    long long total;
-    const TcFound f = tc_find<kTcThreads>(plan, &total, [&](long long n) { return TcDeal(n, gridDim.x).first(blockIdx.x); });
     fence_before();
-    __syncthreads();
+    tc_find<kTcThreads>(plan, blockIdx.x, &begin);
     fence_after();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = tmem_slot;
-    const TcDeal deal(total, gridDim.x);
-    const long long u0 = deal.first(blockIdx.x), u1 = deal.first(blockIdx.x + 1);
-    TcIter it;
-    it.begin(plan, f.s, f.rel, u0);
+    const long long u1 = begin.u1;
+    TcIter it = begin.it;
+    if (starts != nullptr && tid == 0) starts[blockIdx.x] = begin;  // for the joining of partials
+    const int sub = plan.sub;
     // the next segment of this CTA: blocks [it.b0, b1) of the pair
     auto segment = [&](int *b1) {
-        if (u0 >= u1 || it.s >= plan.sequences) return false;
-        *b1 = it.block_at(u1);
+        if (it.s >= plan.sequences) return false;
+        *b1 = it.block_at(plan, u1);
         return *b1 > it.b0;
     };
     bool ok = true;
@@ -567,7 +567,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float2 e = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), f2, n2);
-                        const float2 w = i % 8 >= 8 - kPoly ? ex2_poly(e) : make_float2(ex2(e.x), ex2(e.y));
+                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                         p[i] = pack2<KT>(w.x, w.y);
                     }
@@ -799,6 +799,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
         }
     }
+    if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
     if (!ok && lane == 0) report(a.status, kStatusAttentionWait);
     __syncwarp();
     fence_before();
@@ -814,23 +815,21 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 constexpr int kTcMergeThreads = 256;
 
 template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials, int sub, int ctas)
+__global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials,
+                                                                   const TcStart *__restrict__ starts, const __grid_constant__ TcPlan plan)
 {
     using C = Tc<D>;
     __shared__ float row_q[kTcMergeThreads / 32][D];
     const int c = blockIdx.x + 1, x = blockIdx.y, warp = threadIdx.x >> 5;
-    const TcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, sub, sub * kTcSubs};
-    long long total;
-    const TcFound f = tc_find<kTcMergeThreads>(plan, &total, [&](long long n) { return TcDeal(n, ctas).first(c); });
     // also by CTAs with nothing to join: the next launch of the stream follows this one
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TcDeal deal(total, ctas);
-    const long long u = deal.first(c);
-    if (u >= total) return;
-    TcIter it;
-    it.begin(plan, f.s, f.rel, u);
-    if (it.b0 == 0) return;  // no pair is cut here
-    const int c0 = deal.holder(it.origin + kTcOver), c1 = deal.holder(it.origin + kTcOver + (long long)kTcKeys * (it.blocks - 1));
+    const TcIter it = starts[c].it;
+    if (it.s >= plan.sequences || it.b0 == 0) return;  // no pair is cut here
+    // CTAs c0 .. c1 hold the pair
+    int c0 = c, c1 = c;
+    while (starts[c0].u0 > it.origin + plan.over) --c0;
+    const long long last = it.origin + plan.over + (long long)kTcKeys * (it.blocks - 1);
+    while (c1 + 1 < plan.ctas.d && starts[c1 + 1].u0 <= last && starts[c1 + 1].it.s < plan.sequences) ++c1;
     const int slice = c - c0 - 1, slices = c1 - c0;
     const TcSub me(plan, it, x);
     constexpr int G = D / 16;  // 16-column pieces of a row
@@ -843,7 +842,7 @@ __global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = 0.f;
         for (int p = c0; live && p <= c1; ++p) {
-            if (p > c0 && it.block_at(deal.first(p)) == it.block_at(deal.first(p + 1))) continue;  // no block of its own
+            if (p > c0 && it.block_at(plan, starts[p].u0) == it.block_at(plan, starts[p].u1)) continue;  // no block of its own
             const float *part = partials + (size_t)(2 * p + (p == c0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / kTcSubs);
             const float pm = part[kTcRows * D + r], pl = part[kTcRows * D + kTcRows + r];
             if (pm == -INFINITY) continue;
@@ -946,9 +945,14 @@ template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t 
     const int ctas = (int)(most < sms ? most : sms);
     const bool split = ctas > 1 && blocks > 1;
     float *partials = nullptr;
-    if (split) e = stream_alloc((void **)&partials, (size_t)2 * ctas * C::kPartial * sizeof(float), s);
+    const size_t bytes = (size_t)2 * ctas * C::kPartial * sizeof(float);
+    if (split) e = stream_alloc((void **)&partials, bytes + (size_t)ctas * sizeof(TcStart), s);
     if (e != cudaSuccess) return e;
-    tc_attention_kernel<T, T, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, sub, partials);
+    TcStart *starts = split ? (TcStart *)((char *)partials + bytes) : nullptr;
+    auto divisor = [](int d) { return Divisor{d > 1 ? ~0ull / (unsigned long long)d + 1 : ~0ull, d}; };
+    const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
+                      sub, divisor(sub * kTcSubs), divisor(ctas)};
+    tc_attention_kernel<T, T, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, starts);
     e = cudaGetLastError();
     if (!split) return e;
     if (e == cudaSuccess) {
@@ -961,7 +965,7 @@ template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t 
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, T, D>, a, (const float *)partials, sub, ctas);
+        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, T, D>, a, (const float *)partials, (const TcStart *)starts, plan);
     }
     const cudaError_t f = stream_free(partials, s);
     return e != cudaSuccess ? e : f;
