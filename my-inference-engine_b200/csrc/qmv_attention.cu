@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int half = e >> 1, j = j0 + 8 * t + 2 * quad + (e & 1);
-                    p[t][e] = j < lim[half] ? sc[t][e] * factor[half] : -INFINITY;
+                    p[t][e] = j < lim[half] ? sc[t][e] : -INFINITY;
                     top[half] = fmaxf(top[half], p[t][e]);
                 }
             float base[2];
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             for (int half = 0; half < 2; ++half) {
                 top[half] = fmaxf(top[half], __shfl_xor_sync(kFull, top[half], 1));
                 top[half] = fmaxf(top[half], __shfl_xor_sync(kFull, top[half], 2));
-                const float mn = fmaxf(m[half], top[half]);
+                const float mn = fmaxf(m[half], top[half] * factor[half]);
                 base[half] = mn == -INFINITY ? 0.f : mn - kLift;
                 fix[half] = m[half] == -INFINITY ? 1.f : ex2(m[half] - mn);
                 raised |= mn > m[half];
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[t][e] = ex2(p[t][e] - base[e >> 1]);
+                    p[t][e] = ex2(fmaf(p[t][e], factor[e >> 1], -base[e >> 1]));
                     l[e >> 1] += p[t][e];
                 }
             uint32_t pa[NQ][4];

@@ -171,8 +171,7 @@ QMV_EXPORT int qmv_packed_attention(uint32_t type, int heads, int kv_heads, int 
     const qmv::KvView kv{k, v, k_ld, v_ld, 0, head_dim, nullptr, 0, 0, 0};
     const qmv::AttnArgs a{type, type, q, out, q_ld, out_ld, kv, start, nullptr, sequences, tokens, heads, kv_heads,
                           heads / kv_heads, head_dim, tokens, scale, status};
-    const cudaError_t e = type == QMV_TYPE_F32 ? qmv::launch_attention_rows(a, (cudaStream_t)stream)
-                                               : qmv::launch_tc_attention(a, (cudaStream_t)stream);
+    const cudaError_t e = qmv::launch_tc_attention(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("attention launch", e);
 }
 
@@ -195,7 +194,7 @@ QMV_EXPORT int qmv_paged_attention(const QmvPagedCache *cache, const QmvPagedBat
     const qmv::AttnArgs a{type, cache->type, q, out, q_ld, out_ld, kv, batch->query_start, batch->length,
                           batch->sequences, batch->tokens, heads, cache->kv_heads, heads / cache->kv_heads, d,
                           batch->max_query, scale, status};
-    const bool few = type == QMV_TYPE_F32 || (int64_t)a.max_query * a.group <= 32;
+    const bool few = (int64_t)a.max_query * a.group <= 32;
     const cudaError_t e = few ? qmv::launch_decode_attention(a, (cudaStream_t)stream) : qmv::launch_tc_attention(a, (cudaStream_t)stream);
     return e == cudaSuccess ? 1 : qmv::set_cuda_error("attention launch", e);
 }

@@ -43,25 +43,36 @@ namespace {
 
 constexpr int kTcKeys = 128;     // keys of a block
 constexpr int kTcRows = 128;     // rows of a tile
-constexpr int kTcSubs = 2;       // tiles of a CTA
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; then
 constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
-template <int D> struct Tc {
+// T, KT: types of the activations and of the keys and values.  f32 operands
+// meet the tensor cores as pairs of f16, x = hi + lo to 22 bits of the largest
+// value of their row (scaled by a power of two), in the products hi hi, lo hi
+// and hi lo.
+template <typename T, typename KT, int D> struct Tc {
+    static constexpr int kQ = sizeof(T) == 4 ? 2 : 1;   // parts of Q and P
+    static constexpr int kK = sizeof(KT) == 4 ? 2 : 1;  // parts of K and V
+    using MT = typename std::conditional<kQ == 2, __half, T>::type;
+    static constexpr int kSubs = kQ == 2 && D == 128 ? 1 : 2;  // tiles of a CTA: what tensor memory holds
     // What a pair of tiles costs beside its keys, in keys: 4600 cycles at
     // head_dim 64 and 6700 at 128, where 128 keys take 2560 and 2300.
     static constexpr int kOver = D == 64 ? 256 : 384;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
-    static constexpr int kSlots = D == 64 ? 4 : 2;  // blocks of K, and of V, in flight
-    static constexpr uint32_t kSmem = (kTcSubs + 2 * kSlots) * kTile + 1024;
-    static constexpr int kScores = D == 64 ? 2 : 1;  // S buffers
+    static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
+    // blocks of K, and of V, in flight
+    static constexpr int kSlots = kKTile == 65536 ? 1 : kKTile == 32768 ? 2 : 4;
+    static constexpr uint32_t kSmem = kSubs * kQTile + 2 * kSlots * kKTile + 1024;
+    // tensor memory columns
+    static constexpr int kScores = D == 64 && kQ == 1 ? 2 : 1;  // S buffers
     static __host__ __device__ constexpr uint32_t s_col(int x) { return kScores == 2 ? 128u * x : 0u; }
-    static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + 64u * x; }
-    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + 128u + (uint32_t)D * x; }
-    static constexpr int kPartial = kTcSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
+    static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + 64u * kQ * x; }
+    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + 64u * kQ * kSubs + (uint32_t)D * x; }
+    static_assert(128 * kScores + (64 * kQ + D) * kSubs <= 512, "tensor memory");
+    static constexpr int kPartial = kSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
 };
 
 // ------------------------------------------------------------------- PTX
@@ -227,6 +238,83 @@ template <typename KT> __host__ __device__ constexpr uint32_t idesc(int n, bool 
 {
     return (1u << 4) | (std::is_same<KT, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (mn_major ? 1u << 16 : 0u) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// One f32 row as two f16 rows in swizzled shared memory (row r of a tile and
+// of the tile behind it): x = (hi + lo) 2^-e, the largest |x| in [2^14, 2^15)
+// after the shift; 2^-e is returned.  A row that is not there: zeros.
+template <int D> __device__ __forceinline__ float split_row(const float *x, bool live, uint32_t tile, int r)
+{
+    float big = 0.f;
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < D; i += 4) {
+            const float4 v = *(const float4 *)(x + i);
+            big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+    }
+    const int e = min(max(14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127, -100), 100);
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < D; i += 8) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (live) {
+            const float4 y = *(const float4 *)(x + i), z = *(const float4 *)(x + i + 4);
+            v[0] = y.x * up; v[1] = y.y * up; v[2] = y.z * up; v[3] = y.w * up;
+            v[4] = z.x * up; v[5] = z.y * up; v[6] = z.z * up; v[7] = z.w * up;
+        }
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h[j] = pack2<__half>(v[2 * j], v[2 * j + 1]);
+            l[j] = pack2_rest(v[2 * j], v[2 * j + 1], h[j]);
+        }
+        const uint32_t to = tile + (uint32_t)(i / 64) * 16384u + (uint32_t)r * 128u + (uint32_t)((((i / 8) & 7) ^ (r & 7)) * 16);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 128u * D * 2u), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
+    }
+    return __uint_as_float((uint32_t)(127 - e) << 23);
+}
+
+// f32 keys and values as two f16 planes [part][token][kv_heads * D] and their
+// units (see TcMaps): the largest |x| of a row in [2^14, 2^15), so that values
+// down to 2^-17 of it keep 22 bits.  A warp a row.
+template <int D>
+__global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__restrict__ kp, __half *__restrict__ vp, float *__restrict__ key_unit,
+                                                       float *__restrict__ value_exp)
+{
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31, rows = a.tokens * a.kv_heads;
+    const size_t plane = (size_t)rows * D;
+    for (int w = blockIdx.x * 8 + (int)(threadIdx.x >> 5); w < 2 * rows; w += gridDim.x * 8) {
+        const bool value = w >= rows;
+        const int at = value ? w - rows : w, token = at / a.kv_heads, h = at - token * a.kv_heads;
+        const float *x = value ? (const float *)a.kv.v + (int64_t)token * a.kv.v_pos + h * D : (const float *)a.kv.k + (int64_t)token * a.kv.k_pos + h * D;
+        float v[E], big = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            v[i] = x[E * lane + i];
+            big = fmaxf(big, fabsf(v[i]));
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, d));
+        const int top = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+        const int e = value ? min(max(14 - top, -60), 60) : min(max(14 - top, -100), 100);
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        __half *to = (value ? vp : kp) + (size_t)at * D + E * lane;
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+            const uint32_t hi = pack2<__half>(v[i] * up, v[i + 1] * up);
+            *(uint32_t *)(to + i) = hi;
+            *(uint32_t *)(to + plane + i) = pack2_rest(v[i] * up, v[i + 1] * up, hi);
+        }
+        if (lane == 0) {
+            if (value)
+                value_exp[(size_t)h * a.tokens + token] = (float)-e;
+            else
+                key_unit[(size_t)h * a.tokens + token] = __uint_as_float((uint32_t)(127 - e) << 23);
+        }
+    }
 }
 
 // 32 values of a row, whole 32-byte sectors a store where rows allow.
@@ -434,24 +522,32 @@ struct TcSub {
 
 struct TcMaps {
     CUtensorMap q, k, v;
+    // f32 keys and values, rows [kv_head][token]: what a key's dot is times
+    // (2^-e), and the exponent of its value's row
+    const float *key_unit, *value_exp;
 };
+
 
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
 tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, const __grid_constant__ TcPlan plan,
                     float *__restrict__ partials, TcStart *__restrict__ starts)
 {
-    using C = Tc<D>;
-    constexpr int NS = C::kSlots;
-    constexpr float kLift = std::is_same<KT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
+    using C = Tc<T, KT, D>;
+    using MT = typename C::MT;
+    constexpr int NS = C::kSlots, kTcSubs = C::kSubs;
+    constexpr float kLift = std::is_same<MT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) unsigned long long bars[4 * NS + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ TcStart begin;
     __shared__ float row_q[8][D];
+    // of f32 keys and values: each key's unit and its value's exponent, a copy a
+    // warp, this block's and the next one's
+    __shared__ float2 key_of[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kTile, v_s = k_s + NS * C::kTile;
+    const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kQTile, v_s = k_s + NS * C::kKTile;
     const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
     const uint32_t k_full = bar0, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, q_full = v_empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
                    s_full = q_empty + 8 * kTcSubs, s_free = s_full + 8 * kTcSubs, p_full = s_free + 8 * kTcSubs,
@@ -465,7 +561,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             bar_init(v_empty + 8 * i, 1);
         }
         for (int x = 0; x < kTcSubs; ++x) {
-            bar_init(q_full + 8 * x, 1);
+            bar_init(q_full + 8 * x, C::kQ == 2 ? 4 : 1);
             bar_init(q_empty + 8 * x, 1);
             bar_init(s_full + 8 * x, 1);
             bar_init(s_free + 8 * x, 4);
@@ -507,15 +603,39 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
         const uint32_t s_t = lanes + C::s_col(x), p_t = lanes + C::p_col(x), o_t = lanes + C::o_col(x);
         uint32_t done = 0;  // blocks of this tile slot handed over so far
-        for (; ok && segment(&b1); it.next(plan)) {
+        // f32 keys: unit and exponent of this lane's keys (lane, lane + 32, ...) of block b
+        auto units_of = [&](int b, float2 u[4]) {
+            const int64_t at = (int64_t)it.h * a.tokens + it.q.row0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = b * kTcKeys + 32 * i + lane;
+                u[i] = j < it.q.keys ? make_float2(__ldg(maps.key_unit + at + j), __ldg(maps.value_exp + at + j)) : make_float2(0.f, 0.f);
+            }
+        };
+        for (; x < kTcSubs && ok && segment(&b1); it.next(plan)) {
             const TcSub me(plan, it, x);
             const int end = min(b1, me.blocks), token = r / a.group;
             const bool row = token < me.tokens;
             const int keys = it.q.keys - it.q.n + me.token0 + token + 1;
             // rows without a token run along unmasked and are never written
             const int lim = row ? max(keys, 0) : 0x7fffffff;
-            const float f = row ? a.scale * kLog2e : 0.f;
+            const int head = it.h * a.group + r - token * a.group, token_row = it.q.row0 + me.token0 + token;
+            float f = row ? a.scale * kLog2e : 0.f;
+            if constexpr (C::kQ == 2) {
+                // this thread's row of Q as two f16 rows; the QK products of
+                // the tile before have ended, since their scores were read
+                if (end > it.b0) {
+                    f *= split_row<D>((const float *)a.q + (int64_t)(row ? token_row : 0) * a.q_ld + (int64_t)(row ? head : 0) * D, row,
+                                      q_s + x * C::kQTile, r);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(q_full + 8 * x);
+                }
+            }
             float m = -INFINITY, l = 0.f;
+            float2 next_units[4];
+            if constexpr (C::kK == 2)
+                if (end > it.b0) units_of(it.b0, next_units);
             for (int b = it.b0; b < end; ++b) {
                 if (!(ok = warp_wait(s_full + 8 * x, done & 1))) break;
                 fence_after();
@@ -527,15 +647,26 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 __syncwarp();
                 if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
                 const int j0 = b * kTcKeys;
+                const float2 *unit = key_of[C::kK == 2 ? warp : 0][b & 1];
+                if constexpr (C::kK == 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) key_of[warp][b & 1][32 * i + lane] = next_units[i];
+                    __syncwarp();
+                    if (b + 1 < end) units_of(b + 1, next_units);
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] *= unit[i].x;
+                }
                 if (__any_sync(kFull, j0 + kTcKeys > lim)) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
                         if (j0 + i >= lim) s[i] = -INFINITY;
                 }
-                float top[4] = {s[0], s[1], s[2], s[3]};
+                // the largest exponent: of the weight, or, where values have
+                // exponents of their own, of the weight that meets the value
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+                for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], C::kK == 2 ? fmaf(s[i], f, unit[i].y) : s[i]);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (C::kK == 2 ? 1.f : f);
                 const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
                 // P and O as the block before this one left them
                 if (done > 0) {
@@ -563,15 +694,22 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32];
+                    uint32_t p[32], rest[C::kQ == 2 ? 32 : 1];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float2 e = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), f2, n2);
+                        const int j = 64 * h + 2 * i;
+                        const float2 of = C::kK == 2 ? make_float2(unit[j].y, unit[j + 1].y) : make_float2(0.f, 0.f);
+                        const float2 e = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, C::kK == 2 ? __fadd2_rn(n2, of) : n2);
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
-                        sum[i & 1] = __fadd2_rn(sum[i & 1], w);
-                        p[i] = pack2<KT>(w.x, w.y);
+                        if constexpr (C::kK == 2)
+                            sum[i & 1] = __ffma2_rn(w, make_float2(ex2(-of.x), ex2(-of.y)), sum[i & 1]);
+                        else
+                            sum[i & 1] = __fadd2_rn(sum[i & 1], w);
+                        p[i] = pack2<MT>(w.x, w.y);
+                        if constexpr (C::kQ == 2) rest[i] = pack2_rest(w.x, w.y, p[i]);
                     }
                     tmem_st32(p_t + 32 * h, p);
+                    if constexpr (C::kQ == 2) tmem_st32(p_t + 64 + 32 * h, rest);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 wait_st();
@@ -588,7 +726,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 fence_after();
             }
             const bool whole = it.b0 == 0 && b1 == it.blocks;
-            const int head = it.h * a.group + r - token * a.group, token_row = it.q.row0 + me.token0 + token;
             if (whole) {
                 const float inv = 1.f / l;
                 const bool none = keys <= 0;
@@ -615,7 +752,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
             } else {
                 // a partial that starts inside its pair goes to the first slot
-                float *part = partials + (size_t)(2 * blockIdx.x + (it.b0 == 0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / kTcSubs);
+                float *part = partials + (size_t)(2 * blockIdx.x + (it.b0 == 0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
                 if (any) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -643,16 +780,16 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         };
         if (warp == kTcQkWarp) {
             // ----------------------------------------------------- S = Q K^T
-            constexpr uint32_t kId = idesc<KT>(128, false);
+            constexpr uint32_t kId = idesc<MT>(128, false);
             const uint32_t tm = __shfl_sync(kFull, tmem, 0);
-            uint32_t q_phase[kTcSubs] = {0, 0}, s_phase[kTcSubs] = {1, 1};  // s_phase: of each S buffer
+            uint32_t q_phase[2] = {0, 0}, s_phase[2] = {1, 1};  // s_phase: of each S buffer
             for (; ok && segment(&b1); it.next(plan)) {
-                int end[kTcSubs];  // of the blocks of each tile
+                int end[2];  // of the blocks of each tile
 #pragma unroll
                 for (int x = 0; x < kTcSubs; ++x) end[x] = min(b1, TcSub(plan, it, x).blocks);
                 for (int b = it.b0; b < b1; ++b) {
                     if (!(ok = warp_wait(k_full + 8 * slot, phase))) break;
-                    const uint64_t kb = desc_k(k_s + __shfl_sync(kFull, slot, 0) * C::kTile);
+                    const uint64_t kb = desc_k(k_s + __shfl_sync(kFull, slot, 0) * C::kKTile);
 #pragma unroll
                     for (int x = 0; x < kTcSubs; ++x) {
                         if (!ok || b >= end[x]) continue;
@@ -664,10 +801,23 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         if (!ok || !(ok = warp_wait(s_free + 8 * (kBuf * x), s_phase[kBuf * x]))) continue;
                         s_phase[kBuf * x] ^= 1;
                         fence_after();
-                        const uint64_t qa = desc_k(q_s + x * C::kTile);
+                        const uint64_t qa = desc_k(q_s + x * C::kQTile);
+                        constexpr uint32_t part = C::kTile >> 4;
+                        // small products first: each addition rounds to the
+                        // sum so far
+                        if constexpr (C::kQ == 2) {
 #pragma unroll
-                        for (int k = 0; k < D / 64; ++k)
-                            mma_ss64(tm + C::s_col(x), qa + k * (C::kHalf >> 4), kb + k * (C::kHalf >> 4), kId, k != 0);
+                            for (int k = 0; k < D / 64; ++k) {
+                                const uint32_t at = k * (C::kHalf >> 4);
+                                mma_ss64(tm + C::s_col(x), qa + part + at, kb + at, kId, k != 0);
+                                if constexpr (C::kK == 2) mma_ss64(tm + C::s_col(x), qa + at, kb + part + at, kId, 1u);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k) {
+                            const uint32_t at = k * (C::kHalf >> 4);
+                            mma_ss64(tm + C::s_col(x), qa + at, kb + at, kId, C::kQ == 2 || k != 0);
+                        }
                         commit(s_full + 8 * x);
                         if (b + 1 == end[x]) commit(q_empty + 8 * x);
                     }
@@ -682,24 +832,30 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
         } else if (warp == kTcPvWarp) {
             // ------------------------------------------------------ O += P V
-            constexpr uint32_t kId = idesc<KT>(D, true);
+            constexpr uint32_t kId = idesc<MT>(D, true);
             const uint32_t tm = __shfl_sync(kFull, tmem, 0);
-            uint32_t p_phase[kTcSubs] = {0, 0};
+            uint32_t p_phase[2] = {0, 0};
             for (; ok && segment(&b1); it.next(plan)) {
-                int end[kTcSubs];
+                int end[2];
 #pragma unroll
                 for (int x = 0; x < kTcSubs; ++x) end[x] = min(b1, TcSub(plan, it, x).blocks);
                 for (int b = it.b0; b < b1; ++b) {
                     if (!(ok = warp_wait(v_full + 8 * slot, phase))) break;
-                    const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kTile);
+                    const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kKTile);
 #pragma unroll
                     for (int x = 0; x < kTcSubs; ++x) {
                         if (!ok || b >= end[x]) continue;
                         if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
                         p_phase[x] ^= 1;
                         fence_after();
-                        mma_ts64(tm + C::o_col(x), tm + C::p_col(x), vb, kId, b != it.b0);
-                        mma_ts64(tm + C::o_col(x), tm + C::p_col(x) + 32u, vb + (64 * 128 >> 4), kId, 1u);
+                        constexpr uint32_t part = C::kTile >> 4, rows64 = 64 * 128 >> 4;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t pt = tm + C::p_col(x) + 32u * h;
+                            mma_ts64(tm + C::o_col(x), pt, vb + h * rows64, kId, h != 0 || b != it.b0);
+                            if constexpr (C::kQ == 2) mma_ts64(tm + C::o_col(x), pt + 64u, vb + h * rows64, kId, 1u);
+                            if constexpr (C::kK == 2) mma_ts64(tm + C::o_col(x), pt, vb + part + h * rows64, kId, 1u);
+                        }
                         commit(pv_done + 8 * x);
                     }
                     if (!ok) break;
@@ -719,7 +875,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const bool paged = a.kv.table != nullptr;
             const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys, piece = min(page_size, kTcKeys), pieces = kTcKeys / piece;
             const uint32_t q_bytes = (uint32_t)(sub * a.group) * D * 2;
-            uint32_t issued = 0, q_phase[kTcSubs] = {1, 1}, tail_phase = 0;
+            uint32_t issued = 0, q_phase[2] = {1, 1}, tail_phase = 0;
             phase = 1;  // of the empty barriers
             // page of the piece that this lane copies of block b
             auto page_of = [&](int b) {
@@ -731,7 +887,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 return a.kv.page_count;  // outside the map: zeros
             };
             for (; ok && segment(&b1); it.next(plan)) {
-                if (!values) {
+                if (!values && C::kQ == 1) {
                     for (int x = 0; ok && x < kTcSubs; ++x) {
                         const TcSub me(plan, it, x);
                         if (min(b1, me.blocks) <= it.b0) continue;
@@ -741,7 +897,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                             bar_expect(q_full + 8 * x, q_bytes);
 #pragma unroll
                             for (int c = 0; c < D / 64; ++c)
-                                tma3(q_s + x * C::kTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
+                                tma3(q_s + x * C::kQTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
                         }
                     }
                 }
@@ -753,23 +909,24 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     // the rows behind the last value: zeros, so that no stale
                     // NaN meets a weight of 0
                     const bool tail = values && left < kTcKeys;
-                    const uint32_t bar = tail ? tail_bar : full + 8 * slot, dst = tiles + slot * C::kTile;
+                    const uint32_t bar = tail ? tail_bar : full + 8 * slot, dst = tiles + slot * C::kKTile;
                     const int live = paged ? min(pieces, max(0, (left + piece - 1) / piece)) : 1;
                     if (lane == 0) {
                         if (live > 0)
-                            bar_expect(bar, (uint32_t)(live * piece) * D * 2);
+                            bar_expect(bar, (uint32_t)(live * piece) * D * 2 * C::kK);
                         else if (!tail)
                             bar_arrive(bar);
                     }
                     __syncwarp();
                     if (lane < live) {
 #pragma unroll
-                        for (int c = 0; c < D / 64; ++c) {
+                        for (int c = 0; c < D / 64 * C::kK; ++c) {
                             const uint32_t to = dst + c * C::kHalf + (uint32_t)(lane * piece) * 128u;
+                            const int x0 = 64 * (c % (D / 64)), part = c / (D / 64);
                             if (paged)
-                                tma4(to, map, 64 * c, it.h, (j0 + lane * piece) & (page_size - 1), page, bar);
+                                tma4(to, map, x0, it.h, (j0 + lane * piece) & (page_size - 1), page, bar);
                             else
-                                tma4(to, map, 64 * c, it.h, it.q.row0 + j0, 0, bar);
+                                tma4(to, map, x0, it.h, it.q.row0 + j0, part, bar);
                         }
                     }
                     if (tail) {
@@ -779,7 +936,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         }
                         for (int row = max(0, left) + (lane >> 3); row < kTcKeys; row += 4)
 #pragma unroll
-                            for (int c = 0; c < D / 64; ++c)
+                            for (int c = 0; c < D / 64 * C::kK; ++c)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + c * C::kHalf + (uint32_t)row * 128u + (lane & 7) * 16u),
                                              "r"(0u)
                                              : "memory");
@@ -795,7 +952,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             if (!ok) {  // copies in flight land before the CTA ends
                 const uint32_t from = issued > NS ? issued - NS : 0;
                 for (uint32_t i = from; i < issued; ++i) bar_wait(full + 8 * (i % NS), (i / NS) & 1);
-                for (int x = 0; !values && x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
+                for (int x = 0; !values && C::kQ == 1 && x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
             }
         }
     }
@@ -818,7 +975,7 @@ template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials,
                                                                    const TcStart *__restrict__ starts, const __grid_constant__ TcPlan plan)
 {
-    using C = Tc<D>;
+    using C = Tc<T, KT, D>;
     __shared__ float row_q[kTcMergeThreads / 32][D];
     const int c = blockIdx.x + 1, x = blockIdx.y, warp = threadIdx.x >> 5;
     // also by CTAs with nothing to join: the next launch of the stream follows this one
@@ -843,7 +1000,7 @@ __global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_
         for (int i = 0; i < 16; ++i) o[i] = 0.f;
         for (int p = c0; live && p <= c1; ++p) {
             if (p > c0 && it.block_at(plan, starts[p].u0) == it.block_at(plan, starts[p].u1)) continue;  // no block of its own
-            const float *part = partials + (size_t)(2 * p + (p == c0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / kTcSubs);
+            const float *part = partials + (size_t)(2 * p + (p == c0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
             const float pm = part[kTcRows * D + r], pl = part[kTcRows * D + kTcRows + r];
             if (pm == -INFINITY) continue;
             const float mn = fmaxf(m, pm), fo = m == -INFINITY ? 0.f : ex2(m - mn), fn = ex2(pm - mn);
@@ -918,46 +1075,71 @@ cudaError_t make_map(CUtensorMap *map, const void *base, int rank, const cuuint6
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t s)
+template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t s)
 {
-    using C = Tc<D>;
+    using C = Tc<T, KT, D>;
+    using MT = typename C::MT;
     const int sub = kTcRows / a.group;
-    TcMaps maps;
-    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
-    const int64_t qs[2] = {D, a.q_ld};
-    const cuuint32_t qb[3] = {64, (cuuint32_t)a.group, (cuuint32_t)sub};
-    cudaError_t e = make_map<T>(&maps.q, a.q, 3, qd, qs, qb);
     const bool paged = a.kv.table != nullptr;
-    const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys;
-    const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.kv_heads, paged ? (cuuint64_t)page_size : (cuuint64_t)a.tokens,
-                              paged ? (cuuint64_t)a.kv.page_count : 1};
-    const int64_t ks[3] = {a.kv.head, a.kv.k_pos, paged ? a.kv.page : a.kv.k_pos}, vs[3] = {a.kv.head, a.kv.v_pos, paged ? a.kv.page : a.kv.v_pos};
-    const cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
-    if (e == cudaSuccess) e = make_map<T>(&maps.k, a.kv.k, 4, kd, ks, kb);
-    if (e == cudaSuccess) e = make_map<T>(&maps.v, a.kv.v, 4, kd, vs, kb);
     int dev = 0, sms = 0;
-    if (e == cudaSuccess) e = cudaGetDevice(&dev);
+    cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_attention_kernel<T, T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(tc_attention_kernel<T, KT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
     if (e != cudaSuccess) return e;
     const int64_t keys = paged ? (int64_t)a.kv.max_pages << a.kv.page_shift : a.tokens, blocks = (keys + kTcKeys - 1) / kTcKeys;
-    const int64_t pairs = a.tokens / (sub * kTcSubs) + a.sequences, most = pairs * a.kv_heads * blocks;
+    const int64_t pairs = a.tokens / (sub * C::kSubs) + a.sequences, most = pairs * a.kv_heads * blocks;
     const int ctas = (int)(most < sms ? most : sms);
     const bool split = ctas > 1 && blocks > 1;
-    float *partials = nullptr;
-    const size_t bytes = (size_t)2 * ctas * C::kPartial * sizeof(float);
-    if (split) e = stream_alloc((void **)&partials, bytes + (size_t)ctas * sizeof(TcStart), s);
+    // scratch: partials | share starts | f16 planes of K and V | their units
+    const size_t part_bytes = split ? (size_t)2 * ctas * C::kPartial * sizeof(float) : 0, start_bytes = split ? (size_t)ctas * sizeof(TcStart) : 0;
+    const size_t plane_at = (part_bytes + start_bytes + 127) & ~(size_t)127, rows = (size_t)a.tokens * a.kv_heads;
+    const size_t plane_bytes = C::kK == 2 ? rows * D * 4 : 0;  // two parts
+    char *scratch = nullptr;
+    if (split || C::kK == 2) e = stream_alloc((void **)&scratch, plane_at + 2 * plane_bytes + (C::kK == 2 ? rows * 8 : 0), s);
     if (e != cudaSuccess) return e;
-    TcStart *starts = split ? (TcStart *)((char *)partials + bytes) : nullptr;
+    float *partials = split ? (float *)scratch : nullptr;
+    TcStart *starts = split ? (TcStart *)(scratch + part_bytes) : nullptr;
+    TcMaps maps{};
+    const void *k = a.kv.k, *v = a.kv.v;
+    if constexpr (C::kK == 2) {
+        __half *kp = (__half *)(scratch + plane_at), *vp = kp + 2 * rows * D;
+        float *units = (float *)(vp + 2 * rows * D);
+        const size_t want = (2 * rows + 7) / 8, cap = (size_t)sms * 8;
+        split_kv_kernel<D><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a, kp, vp, units, units + rows);
+        e = cudaGetLastError();
+        k = kp;
+        v = vp;
+        maps.key_unit = units;
+        maps.value_exp = units + rows;
+    }
+    if constexpr (C::kQ == 1) {
+        const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
+        const int64_t qs[2] = {D, a.q_ld};
+        const cuuint32_t qb[3] = {64, (cuuint32_t)a.group, (cuuint32_t)sub};
+        if (e == cudaSuccess) e = make_map<MT>(&maps.q, a.q, 3, qd, qs, qb);
+    }
+    const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys;
+    const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.kv_heads, paged ? (cuuint64_t)page_size : (cuuint64_t)a.tokens,
+                              paged ? (cuuint64_t)a.kv.page_count : (cuuint64_t)C::kK};
+    int64_t ks[3] = {a.kv.head, a.kv.k_pos, paged ? a.kv.page : a.kv.k_pos}, vs[3] = {a.kv.head, a.kv.v_pos, paged ? a.kv.page : a.kv.v_pos};
+    if constexpr (C::kK == 2) {
+        ks[0] = vs[0] = D;
+        ks[1] = vs[1] = (int64_t)a.kv_heads * D;
+        ks[2] = vs[2] = (int64_t)rows * D;
+    }
+    const cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
+    if (e == cudaSuccess) e = make_map<MT>(&maps.k, k, 4, kd, ks, kb);
+    if (e == cudaSuccess) e = make_map<MT>(&maps.v, v, 4, kd, vs, kb);
     auto divisor = [](int d) { return Divisor{d > 1 ? ~0ull / (unsigned long long)d + 1 : ~0ull, d}; };
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
-                      sub, divisor(sub * kTcSubs), divisor(ctas)};
-    tc_attention_kernel<T, T, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, starts);
-    e = cudaGetLastError();
-    if (!split) return e;
+                      sub, divisor(sub * C::kSubs), divisor(ctas)};
     if (e == cudaSuccess) {
+        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, starts);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess && split) {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)ctas - 1, kTcSubs);
+        cfg.gridDim = dim3((unsigned)ctas - 1, C::kSubs);
         cfg.blockDim = dim3(kTcMergeThreads);
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
@@ -965,9 +1147,9 @@ template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t 
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, T, D>, a, (const float *)partials, (const TcStart *)starts, plan);
+        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, KT, D>, a, (const float *)partials, (const TcStart *)starts, plan);
     }
-    const cudaError_t f = stream_free(partials, s);
+    const cudaError_t f = stream_free(scratch, s);
     return e != cudaSuccess ? e : f;
 }
 
@@ -975,9 +1157,12 @@ template <typename T, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t 
 
 cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s)
 {
-    if (a.type != a.kv_type) return cudaErrorInvalidValue;
-    if (a.type == kTypeF16) return a.head_dim == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
-    if (a.type == kTypeBF16) return a.head_dim == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+    const bool wide = a.head_dim == 128;
+    if (a.type == kTypeF32 && a.kv_type == kTypeF32) return wide ? launch<float, float, 128>(a, s) : launch<float, float, 64>(a, s);
+    if (a.type == kTypeF32 && a.kv_type == kTypeF16) return wide ? launch<float, __half, 128>(a, s) : launch<float, __half, 64>(a, s);
+    if (a.type == kTypeF16 && a.kv_type == kTypeF16) return wide ? launch<__half, __half, 128>(a, s) : launch<__half, __half, 64>(a, s);
+    if (a.type == kTypeBF16 && a.kv_type == kTypeBF16)
+        return wide ? launch<__nv_bfloat16, __nv_bfloat16, 128>(a, s) : launch<__nv_bfloat16, __nv_bfloat16, 64>(a, s);
     return cudaErrorInvalidValue;
 }
 
