@@ -13,6 +13,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "qmv_attention.cuh"
 #include "qmv_internal.h"
 
@@ -130,8 +132,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(AttnArgs
 // cost nothing.  Each of the 4 warps takes 16 keys of every unit, streams
 // them through its own cp.async ring (the rings together keep 128 KB an SM in
 // flight, with no barrier between warps) and holds its own running maximum,
-// sum and output in registers; the warps meet once per item.  An item that ends up in more than one CTA leaves partials (maximum,
-// sum, unnormalised output) that decode_merge_kernel joins in order.
+// sum and output in registers; the warps meet once per item.
 // tcgen05 is not used: its M of 64 or more would be mostly empty rows here,
 // and the tensor work is a tenth of the time the bytes take.
 
@@ -195,73 +196,12 @@ template <typename KT> __device__ __forceinline__ void mma16816(float d[4], cons
 struct DcPlan {
     const int *start, *length;
     int sequences, tokens, max_keys, kv_heads, group;
+    Divisor ctas;
     __device__ __forceinline__ Seq seq(int s) const { return load_sequence(start, length, s, tokens, max_keys); }
     __device__ __forceinline__ int tiles(const Seq &q) const { return (q.n * group + kDcRows - 1) / kDcRows; }
     __device__ __forceinline__ int blocks(const Seq &q) const { return q.keys > 0 ? (q.keys + kDcUnit - 1) / kDcUnit : 1; }
     __device__ __forceinline__ long long cost(const Seq &q) const { return (long long)tiles(q) * kv_heads * (blocks(q) + kDcItemCost); }
 };
-
-// Sum over the CTA of one value a thread, and the exclusive prefix.
-__device__ __forceinline__ long long block_scan(long long v, long long *total, long long *scratch)
-{
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(kFull, x, d);
-        if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) scratch[warp] = x;
-    __syncthreads();
-    long long before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kDcWarps; ++w) {
-        if (w < warp) before += scratch[w];
-        all += scratch[w];
-    }
-    *total = all;
-    return before + x - v;
-}
-
-// How `total` is dealt to `ctas` CTAs in order: the first total % ctas get
-// one more.
-struct Deal {
-    long long each, more;
-    __device__ __forceinline__ Deal(long long total, int ctas) : each(total / ctas), more(total - each * ctas) {}
-    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
-    __device__ __forceinline__ int holder(long long u) const
-    {
-        const long long big = more * (each + 1);
-        return u < big ? (int)(u / (each + 1)) : (int)(more + (u - big) / each);
-    }
-};
-
-struct Found {
-    int s;          // sequence
-    long long rel;  // place within it
-};
-
-// The cost of the whole launch, and the sequence in which place share(total)
-// falls (by every thread of the CTA together; a thread takes a run of
-// sequences).
-template <typename F> __device__ Found find_place(const DcPlan &p, long long *scratch, long long *total, const F &share)
-{
-    __shared__ Found found;
-    const int per = (p.sequences + kDcThreads - 1) / kDcThreads, s0 = (int)threadIdx.x * per, s1 = min(s0 + per, p.sequences);
-    long long v = 0;
-    for (int s = s0; s < s1; ++s) v += p.cost(p.seq(s));
-    if (threadIdx.x == 0) found = Found{p.sequences, 0};
-    long long before = block_scan(v, total, scratch);
-    const long long want = share(*total);
-    if (want >= before && want < before + v) {
-        int s = s0;
-        for (long long c; want >= before + (c = p.cost(p.seq(s))); ++s) before += c;
-        found = Found{s, want - before};
-    }
-    __syncthreads();
-    return found;
-}
 
 // Walks units in order: sequence, head, row tile, key block.  A unit's place
 // is its item's first place + kDcItemCost + blk; a CTA has the units whose
@@ -269,6 +209,7 @@ template <typename F> __device__ Found find_place(const DcPlan &p, long long *sc
 struct DcIter {
     Seq q;
     int s, h, rt, blk, rts, blks;
+    long long u;  // the unit's place
     __device__ __forceinline__ void enter(const DcPlan &p)
     {
         rts = blks = 0;
@@ -280,31 +221,36 @@ struct DcIter {
             ++s;
         }
     }
-    // The first unit at or behind place rel of sequence s_; how far behind.
-    __device__ __forceinline__ int begin(const DcPlan &p, int s_, long long rel)
+    // The first unit at or behind place rel of sequence s_ (one with tiles),
+    // and its own place, where rel is place u0.
+    __device__ __forceinline__ void begin(const DcPlan &p, int s_, const Seq &q_, long long rel, long long u0)
     {
         s = s_;
-        enter(p);
-        blk = h = rt = 0;
-        if (rts == 0) return 0;
-        const int span = blks + kDcItemCost, item = (int)(rel / span), at = (int)(rel - (long long)item * span);
+        q = q_;
+        rts = p.tiles(q);
+        blks = p.blocks(q);
+        const int span = blks + kDcItemCost;
+        int item = (int)((float)rel / (float)span);  // an estimate, then exactly
+        while ((long long)item * span > rel) --item;
+        while ((long long)(item + 1) * span <= rel) ++item;
+        const int at = (int)(rel - (long long)item * span);
         blk = max(0, at - kDcItemCost);
-        rt = item % rts;
         h = item / rts;
-        return kDcItemCost + blk - at;
+        rt = item - h * rts;
+        u = u0 + kDcItemCost + blk - at;
     }
-    // To the next unit; the places between.
-    __device__ __forceinline__ int next(const DcPlan &p)
+    __device__ __forceinline__ void next(const DcPlan &p)
     {
-        if (++blk < blks) return 1;
+        ++u;
+        if (++blk < blks) return;
+        u += kDcItemCost;
         blk = 0;
-        if (++rt < rts) return 1 + kDcItemCost;
+        if (++rt < rts) return;
         rt = 0;
-        if (++h < p.kv_heads) return 1 + kDcItemCost;
+        if (++h < p.kv_heads) return;
         h = 0;
         ++s;
         enter(p);
-        return 1 + kDcItemCost;
     }
 };
 
@@ -320,7 +266,8 @@ template <typename T> __device__ __forceinline__ bool store4(T *out, const float
 }
 
 template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ partials)
+__global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ DcPlan plan,
+                                                                                 float *partials, unsigned long long *flags, unsigned long long launch)
 {
     using C = Dc<D>;
     constexpr int NQ = sizeof(T) == 4 ? 2 : 1;  // f16 pairs for f32 activations
@@ -328,25 +275,17 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
     // the weights' exponent offset: f16 weights down to 2^-22 stay normal
     constexpr float kLift = std::is_same<KT, __half>::value ? 8.f : 0.f;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long scratch[kDcWarps];
     __shared__ unsigned bad_rows;
+    __shared__ Start<DcIter> begin;
     float *merge = (float *)(smem + C::kRing);
     float2 *ml = (float2 *)(smem + C::kRing + C::kMerge);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, grp = lane >> 2;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
     if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
     if (tid == 0) bad_rows = 0u;
-    long long total;
-    const Found f = find_place(plan, scratch, &total, [&](long long n) { return Deal(n, gridDim.x).first(blockIdx.x); });
-    const Deal deal(total, gridDim.x);
-    long long u = deal.first(blockIdx.x);
-    const long long u1 = deal.first(blockIdx.x + 1);
-    if (u >= u1) return;
-
-    DcIter pf, it;
-    u += it.begin(plan, f.s, f.rel);
-    pf = it;
+    find_start<kDcThreads>(plan, &begin);
+    const long long u1 = begin.u1;
+    DcIter it = begin.it, pf = it;
+    if (it.s >= plan.sequences || it.u >= u1) return;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + (uint32_t)warp * C::kStep * C::kStages;
     const int mask = (1 << a.kv.page_shift) - 1;
 
@@ -355,11 +294,10 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
         const int j0 = i.blk * kDcUnit + warp * kDcKeys;
         return j0 < i.q.keys ? __ldg(a.kv.table + (int64_t)i.s * a.kv.max_pages + (j0 >> a.kv.page_shift)) : -1;
     };
-    long long ahead = u;     // place of the next unit to fetch
     uint32_t to_stage = 0u;  // its stage
     int page = page_of(pf);
     auto issue = [&]() {
-        if (ahead < u1) {
+        if (pf.u < u1) {
             const int j0 = pf.blk * kDcUnit + warp * kDcKeys;
             if (j0 < pf.q.keys) {
                 const bool good = page >= 0 && page < a.kv.page_count;
@@ -380,8 +318,8 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                 }
             }
             to_stage = to_stage + 1 == C::kStages ? 0u : to_stage + 1;
-            ahead += pf.next(plan);
-            if (ahead < u1) page = page_of(pf);
+            pf.next(plan);
+            if (pf.u < u1) page = page_of(pf);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -394,7 +332,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
     uint32_t stage = 0u;
     bool fresh = true;  // at the first unit of a segment, this CTA's part of an item
     int first_blk = 0;  // its key block
-    while (u < u1) {
+    while (it.u < u1) {
         if (fresh) {
             fresh = false;
             first_blk = it.blk;
@@ -532,10 +470,18 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
         }
         stage = stage + 1 == C::kStages ? 0u : stage + 1;
         const bool last_block = it.blk + 1 == it.blks;
-        if (last_block || u + 1 >= u1) {
+        if (last_block || it.u + 1 >= u1) {
             // the warps' shares of the segment meet in shared memory, 8 rows
             // at a time
-            const bool whole = last_block && first_blk == 0;
+            // a segment that starts inside its item leaves a partial; one that
+            // starts it joins the shares share + 1 .. last that hold the rest
+            const bool leaves = first_blk > 0;
+            const int share = my_share(), last = last_block ? share : begin.deal.holder(it.u + (it.blks - 1 - it.blk));
+            if (!leaves && !last_block) {
+                bool good = true;
+                for (int p = share + 1 + tid; p <= last; p += kDcThreads) good &= flag_take(flags + p, launch);
+                if (!good) report(a.status, kStatusAttentionWait);
+            }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 l[half] += __shfl_xor_sync(kFull, l[half], 1);
@@ -544,8 +490,6 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             }
             __syncthreads();
             const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
-            // a partial that starts inside its item goes to the first slot
-            float *part = partials + (size_t)(2 * blockIdx.x + (first_blk == 0 ? 1 : 0)) * C::kPartial;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 if (8 * half >= rows) break;
@@ -572,16 +516,42 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                         const float2 y = ml[w * kDcRows + r];
                         den += y.x == -INFINITY ? 0.f : y.y * ex2(y.x - big);
                     }
-                    if (whole) {
+                    if (!leaves) {
+                        for (int p = share + 1; p <= last; p += 8) {
+                            float pm[8], pl[8];
+                            float4 v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const float *part = partials + (size_t)(p + k) * C::kPartial;
+                                const bool live = p + k <= last;
+                                pm[k] = live ? __ldcg(part + kDcRows * D + r) : -INFINITY;
+                                pl[k] = live ? __ldcg(part + kDcRows * D + kDcRows + r) : 0.f;
+                                v[k] = live ? __ldcg((const float4 *)(part + r * D + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            }
+                            float top = big;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) top = fmaxf(top, pm[k]);
+                            const float fo = big == -INFINITY ? 0.f : ex2(big - top);
+                            den *= fo;
+                            sum = make_float4(sum.x * fo, sum.y * fo, sum.z * fo, sum.w * fo);
+                            big = top;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const float fn = pm[k] == -INFINITY ? 0.f : ex2(pm[k] - top);
+                                den += pl[k] * fn;
+                                sum = make_float4(sum.x + v[k].x * fn, sum.y + v[k].y * fn, sum.z + v[k].z * fn, sum.w + v[k].w * fn);
+                            }
+                        }
                         const int row = it.rt * kDcRows + r, token = row / a.group;
                         const bool none = it.q.keys - it.q.n + token + 1 <= 0;
                         const float inv = 1.f / den;
-                        const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        const float4 y = none ? make_float4(0.f, 0.f, 0.f, 0.f)
                                               : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
                         T *out = (T *)a.out + (int64_t)(it.q.row0 + token) * a.out_ld +
                                  (int64_t)(it.h * a.group + row - token * a.group) * D + c;
-                        if (store4<T>(out, v)) atomicOr(&bad_rows, 1u << r);
+                        if (store4<T>(out, y)) atomicOr(&bad_rows, 1u << r);
                     } else {
+                        float *part = partials + (size_t)share * C::kPartial;
                         *(float4 *)(part + r * D + c) = sum;
                         if (c == 0) {
                             part[kDcRows * D + r] = big;
@@ -591,6 +561,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                 }
                 __syncthreads();
             }
+            if (leaves && tid == 0) flag_set(flags + share, launch);
             const unsigned bad = bad_rows;
             if (bad) {  // a masked NaN or infinity met the sums: those rows again, without it
                 for (int r = warp; r < rows; r += kDcWarps) {
@@ -605,81 +576,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             }
             fresh = true;
         }
-        u += it.next(plan);
-    }
-}
-
-// Joins the partials of items split between CTAs.  Boundary c (CTA c's first
-// unit) lies inside an item or at its start; the boundaries inside one item
-// share its join, each taking a slice of the output.  Partials are added in
-// order, so the result does not depend on timing.
-template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kDcThreads) decode_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials, int ctas)
-{
-    using C = Dc<D>;
-    __shared__ long long scratch[kDcWarps];
-    __shared__ float qs[kDcWarps][D];
-    const int tid = threadIdx.x, c = blockIdx.x + 1;
-    const DcPlan plan{a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv), a.kv_heads, a.group};
-    long long total;
-    const Found f = find_place(plan, scratch, &total, [&](long long n) { return Deal(n, ctas).first(c); });
-    // every CTA waits for the partials, also those with nothing to join: the
-    // next launch of the stream follows this one
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Deal deal(total, ctas);
-    const long long u = deal.first(c);
-    if (u >= total) return;  // an empty share
-    DcIter it;
-    const int behind = it.begin(plan, f.s, f.rel);
-    if (it.blk == 0) return;  // the item starts here
-    // CTAs c0 .. c1 hold the item, and the boundaries c0 + 1 .. c1 join it
-    const long long begin = u + behind - it.blk;  // place of its first unit
-    const int c0 = deal.holder(begin), c1 = deal.holder(begin + it.blks - 1), slice = c - c0 - 1, slices = c1 - c0;
-    const int rows = min(kDcRows, it.q.n * a.group - it.rt * kDcRows);
-    const int positions = rows * (D / 4), p0 = (int)((long long)positions * slice / slices);
-    const int p1 = (int)((long long)positions * (slice + 1) / slices);
-    int width = 1;  // lanes that share a position
-    while (width < 32 && (p1 - p0) * width * 2 <= kDcThreads) width *= 2;
-    const int lane = tid % width;
-    for (int i0 = p0; i0 < p1; i0 += kDcThreads / width) {
-        const int i = i0 + tid / width;
-        const bool live = i < p1;
-        const int r = live ? i / (D / 4) : 0, col = live ? (i % (D / 4)) * 4 : 0;
-        auto slot = [&](int x) { return partials + (size_t)(2 * x + (x == c0 ? 1 : 0)) * C::kPartial; };
-        float big = -INFINITY, den = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int x = c0 + lane; x <= c1; x += width) {
-            const float *p = slot(x);
-            const float mx = p[kDcRows * D + r];
-            if (mx == -INFINITY) continue;
-            const float4 v = *(const float4 *)(p + r * D + col);
-            const float nb = fmaxf(big, mx), fo = big == -INFINITY ? 0.f : ex2(big - nb), fn = ex2(mx - nb);
-            den = den * fo + p[kDcRows * D + kDcRows + r] * fn;
-            sum = make_float4(sum.x * fo + v.x * fn, sum.y * fo + v.y * fn, sum.z * fo + v.z * fn, sum.w * fo + v.w * fn);
-            big = nb;
-        }
-        for (int d = width >> 1; d; d >>= 1) {
-            const float ob = __shfl_xor_sync(kFull, big, d), od = __shfl_xor_sync(kFull, den, d);
-            const float4 ov = make_float4(__shfl_xor_sync(kFull, sum.x, d), __shfl_xor_sync(kFull, sum.y, d),
-                                          __shfl_xor_sync(kFull, sum.z, d), __shfl_xor_sync(kFull, sum.w, d));
-            const float nb = fmaxf(big, ob), fo = big == -INFINITY ? 0.f : ex2(big - nb), fn = ob == -INFINITY ? 0.f : ex2(ob - nb);
-            den = den * fo + od * fn;
-            sum = make_float4(sum.x * fo + ov.x * fn, sum.y * fo + ov.y * fn, sum.z * fo + ov.z * fn, sum.w * fo + ov.w * fn);
-            big = nb;
-        }
-        bool bad = false;
-        const int row = it.rt * kDcRows + r, token = row / a.group, head = it.h * a.group + row - token * a.group;
-        if (live && lane == 0) {
-            const bool none = it.q.keys - it.q.n + token + 1 <= 0;
-            const float inv = 1.f / den;
-            const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-            bad = store4<T>((T *)a.out + (int64_t)(it.q.row0 + token) * a.out_ld + (int64_t)head * D + col, v);
-        }
-        for (unsigned left = __ballot_sync(kFull, bad); left; left &= left - 1) {
-            const int who = __ffs(left) - 1;
-            const int wt = __shfl_sync(kFull, token, who), wh = __shfl_sync(kFull, head, who), wc = __shfl_sync(kFull, col, who);
-            attention_row<T, KT, D>(a, it.q.row0 + wt, wh, it.s, it.q, qs[tid >> 5], wc, wc + 4);
-        }
+        it.next(plan);
     }
 }
 
@@ -728,6 +625,18 @@ cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s)
     });
 }
 
+// A number for a launch's flags that no other launch has and scratch does
+// not hold by chance (splitmix64 of a counter; not 0).
+unsigned long long launch_number()
+{
+    static std::atomic<unsigned long long> count{0x243f6a8885a308d3ull};
+    unsigned long long z = count.fetch_add(0x9e3779b97f4a7c15ull);
+    z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+    z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+    z ^= z >> 31;
+    return z ? z : 1;
+}
+
 cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
 {
     return by_type(a.type, a.kv_type, a.head_dim, [&](auto t, auto kt, auto d) {
@@ -750,25 +659,15 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
             const int64_t most = tiles * a.kv_heads * blocks;
             const int ctas = (int)(most < kDcPerSm * sms ? most : kDcPerSm * sms);
             const bool split = ctas > 1 && blocks > 1;
-            float *partials = nullptr;
-            if (e == cudaSuccess && split) e = stream_alloc((void **)&partials, (size_t)2 * ctas * C::kPartial * sizeof(float), s);
+            const size_t bytes = (size_t)ctas * C::kPartial * sizeof(float);
+            char *scratch = nullptr;  // a partial and a flag a share
+            if (e == cudaSuccess && split) e = stream_alloc((void **)&scratch, bytes + (size_t)ctas * 8, s);
             if (e != cudaSuccess) return e;
-            decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, partials);
+            const DcPlan plan{a.start, a.length, a.sequences, a.tokens, a.kv.max_pages << a.kv.page_shift, a.kv_heads, a.group, divisor(ctas)};
+            decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, plan, (float *)scratch, (unsigned long long *)(scratch + bytes),
+                                                                                            launch_number());
             e = cudaGetLastError();
-            if (!split) return e;
-            if (e == cudaSuccess) {
-                cudaLaunchConfig_t cfg{};
-                cfg.gridDim = dim3((unsigned)ctas - 1);
-                cfg.blockDim = dim3(kDcThreads);
-                cfg.stream = s;
-                cudaLaunchAttribute attr[1];
-                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-                attr[0].val.programmaticStreamSerializationAllowed = 1;
-                cfg.attrs = attr;
-                cfg.numAttrs = 1;
-                e = cudaLaunchKernelEx(&cfg, decode_merge_kernel<T, KT, D>, a, (const float *)partials, ctas);
-            }
-            const cudaError_t f = stream_free(partials, s);
+            const cudaError_t f = stream_free(scratch, s);
             return e != cudaSuccess ? e : f;
         }
     });

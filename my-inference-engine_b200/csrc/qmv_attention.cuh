@@ -166,6 +166,147 @@ __device__ __forceinline__ void check_metadata(unsigned int *status, const int *
     if (bad) report(status, kStatusBadMetadata);
 }
 
+// ------------------------------------------------------ shares of the work
+//
+// A launch's work is a line of places, dealt to its CTAs in equal shares in
+// order.  Where a share's border falls inside an item, the share that holds
+// the item's beginning joins it: the others leave what they have (maximum, sum,
+// unnormalised output) in scratch and set a flag; it ends its own part last, so
+// as a rule it finds them there, adds them in order and writes the output.
+// CTA b has share gridDim.x - 1 - b: a share waits only for later shares,
+// whose CTAs were dispatched before its own, so every wait ends however
+// many CTAs are resident.  (A second kernel for the join took 4 to 10 us.)
+//
+// Flags carry a number of the launch's own, so scratch needs no clearing; who
+// waited for a flag clears it, for the next replay of a captured launch.
+
+// Division by a number the host knows: its floor(2^64 / d) + 1 (exact for
+// dividends below 2^31; within 1 above, and corrected).
+struct Divisor {
+    unsigned long long magic;
+    int d;
+};
+
+inline Divisor divisor(int d) { return Divisor{d > 1 ? ~0ull / (unsigned long long)d + 1 : ~0ull, d}; }
+
+struct Deal {
+    long long each;
+    int more, shares;  // the first `more` shares get one place more
+    static __device__ __forceinline__ Deal of(long long total, const Divisor &d)
+    {
+        Deal t;
+        t.each = (long long)__umul64hi((unsigned long long)total, d.magic);
+        if (t.each * d.d > total) --t.each;
+        t.more = (int)(total - t.each * d.d);
+        t.shares = d.d;
+        return t;
+    }
+    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
+    // The share that place u falls to: an estimate, then exactly.
+    __device__ __forceinline__ int holder(long long u) const
+    {
+        int c = min(shares - 1, (int)((float)u / ((float)each + (float)more / (float)shares)));
+        while (first(c) > u) --c;
+        while (c + 1 < shares && first(c + 1) <= u) ++c;
+        return c;
+    }
+};
+
+__device__ __forceinline__ int my_share() { return (int)(gridDim.x - 1 - blockIdx.x); }
+
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+__device__ __forceinline__ unsigned long long now_ns()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+__device__ __forceinline__ void flag_set(unsigned long long *flag, unsigned long long launch)
+{
+    __threadfence();
+    asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(launch) : "memory");
+}
+
+// Waits (bounded) for a flag and clears it; false when the wait expired.
+__device__ __forceinline__ bool flag_take(unsigned long long *flag, unsigned long long launch)
+{
+    unsigned long long v, t0 = 0;
+    for (uint32_t n = 0;; ++n) {
+        asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(flag) : "memory");
+        if (v == launch) break;
+        if (n == 0) t0 = now_ns();
+        if ((n & 63u) == 63u && now_ns() - t0 > kWaitLimitNs) return false;
+    }
+    *flag = 0ull;
+    return true;
+}
+
+// Sum over the CTA's NT threads of one value each, and the exclusive prefix.
+template <int NT> __device__ __forceinline__ long long block_scan(long long v, long long *total)
+{
+    __shared__ long long scratch[NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) scratch[warp] = x;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += scratch[w];
+        all += scratch[w];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+// Where this CTA's share begins: Iter at its first unit, places [u0, u1), by
+// all threads of the CTA together.  A thread sums the cost of a run of
+// sequences, and the one whose run holds the place walks to it.
+template <typename Iter> struct Start {
+    Iter it;  // it.s == sequences: nothing
+    long long u0, u1;
+    Deal deal;
+};
+
+template <int NT, typename Plan, typename Iter> __device__ __forceinline__ void find_start(const Plan &p, Start<Iter> *out)
+{
+    const int per = p.sequences <= NT ? 1 : (p.sequences + NT - 1) / NT, s0 = min((int)threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
+    long long v = 0, all;
+    Seq q{0, 0, 0};
+    for (int s = s0; s < s1; ++s) {
+        q = p.seq(s);
+        v += p.cost(q);
+    }
+    long long at = block_scan<NT>(v, &all);
+    const Deal deal = Deal::of(all, p.ctas);
+    const int c = my_share();
+    const long long u0 = deal.first(c), u1 = deal.first(c + 1);
+    if (u0 >= u1) {
+        if (threadIdx.x == 0) {
+            out->it.s = p.sequences;
+            out->u0 = out->u1 = 0;
+        }
+    } else if (u0 >= at && u0 < at + v) {
+        int s = s0;
+        if (per > 1)
+            for (long long cost; u0 >= at + (cost = p.cost(q = p.seq(s))); ++s) at += cost;
+        Iter it;
+        it.begin(p, s, q, u0 - at, u0);
+        out->it = it;
+        out->u0 = u0;
+        out->u1 = u1;
+        out->deal = deal;
+    }
+    __syncthreads();
+}
+
 // ------------------------------------------------------ attention by rows
 //
 // One warp computes one (token, query head) in f32 on the CUDA cores: a lane

@@ -55,6 +55,8 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s);
 cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s);
 cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s);
 
+unsigned long long launch_number();
+
 // Status bits of the attention kernels on the current device.
 enum : unsigned int { kStatusBadMetadata = 32u, kStatusAttentionWait = 64u };
 cudaError_t attention_status_word(unsigned int **word);

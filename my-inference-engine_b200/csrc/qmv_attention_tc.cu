@@ -27,8 +27,8 @@
 // weights do not care), so O is rescaled a few times a row at most.
 //
 // Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
-// the launch in order are cut into one equal share per SM at multiples of 128 keys,
-// and a tile that is cut leaves partials (m, l, O) that tc_merge_kernel joins.
+// the launch in order are cut into one equal share per SM at multiples of 128
+// keys, and a tile that is cut is joined by the share that holds its beginning.
 // So ragged lengths, causal triangles and single long chunks load every SM alike.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -46,7 +46,6 @@ constexpr int kTcRows = 128;     // rows of a tile
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; then
 constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 
 // T, KT: types of the activations and of the keys and values.  f32 operands
 // meet the tensor cores as pairs of f16, x = hi + lo to 22 bits of the largest
@@ -76,13 +75,6 @@ template <typename T, typename KT, int D> struct Tc {
 };
 
 // ------------------------------------------------------------------- PTX
-
-__device__ __forceinline__ unsigned long long now_ns()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
 {
@@ -343,13 +335,6 @@ template <typename T> __device__ __forceinline__ void store32(T *out, const floa
 
 // ------------------------------------------------------------------ work
 
-// Division by a number the host knows: its floor(2^64 / d) + 1 (exact for
-// dividends below 2^31; within 1 above, and corrected).
-struct Divisor {
-    unsigned long long magic;
-    int d;
-};
-
 struct TcPlan {
     const int *start, *length;
     int sequences, tokens, max_keys, kv_heads, over;
@@ -366,22 +351,6 @@ struct TcPlan {
     }
     __device__ __forceinline__ int pairs(const Seq &q) const { return (int)__umul64hi((unsigned long long)(q.n + wide.d - 1), wide.magic); }
     __device__ __forceinline__ long long cost(const Seq &q) const { return before(q, pairs(q)) * kv_heads; }
-};
-
-// How `total` places are dealt to the CTAs in order: the first total % ctas
-// get one more.
-struct TcDeal {
-    long long each;
-    int more;
-    static __device__ __forceinline__ TcDeal of(long long total, const Divisor &d)
-    {
-        TcDeal t;
-        t.each = (long long)__umul64hi((unsigned long long)total, d.magic);
-        if (t.each * d.d > total) --t.each;
-        t.more = (int)(total - t.each * d.d);
-        return t;
-    }
-    __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
 };
 
 // Walks the pairs of tiles in order: sequence, head, pair.  Key block b of a
@@ -453,60 +422,6 @@ struct TcIter {
     }
 };
 
-// Where CTA c's share of the whole launch begins, and its places [u0, u1), by
-// all threads of the CTA together: a thread sums the cost of a run of
-// sequences, and the one whose run holds the place walks to it.
-struct TcStart {
-    TcIter it;  // it.s == sequences: nothing
-    long long u0, u1;
-};
-
-template <int NT> __device__ __forceinline__ void tc_find(const TcPlan &p, int c, TcStart *out)
-{
-    __shared__ long long scratch[NT / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = p.sequences <= NT ? 1 : (p.sequences + NT - 1) / NT, s0 = min((int)threadIdx.x * per, p.sequences), s1 = min(s0 + per, p.sequences);
-    long long v = 0;
-    Seq q{0, 0, 0};
-    for (int s = s0; s < s1; ++s) {
-        q = p.seq(s);
-        v += p.cost(q);
-    }
-    long long x = v;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long y = __shfl_up_sync(kFull, x, d);
-        if (lane >= d) x += y;
-    }
-    if (lane == 31) scratch[warp] = x;
-    __syncthreads();
-    long long base = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) base += scratch[w];
-        all += scratch[w];
-    }
-    const TcDeal deal = TcDeal::of(all, p.ctas);
-    const long long u0 = deal.first(c), u1 = deal.first(c + 1);
-    long long at = base + x - v;
-    if (u0 >= u1) {
-        if (threadIdx.x == 0) {
-            out->it.s = p.sequences;
-            out->u0 = out->u1 = 0;
-        }
-    } else if (u0 >= at && u0 < at + v) {
-        int s = s0;
-        if (per > 1)
-            for (long long cost; u0 >= at + (cost = p.cost(q = p.seq(s))); ++s) at += cost;
-        TcIter it;
-        it.begin(p, s, q, u0 - at, u0);
-        out->it = it;
-        out->u0 = u0;
-        out->u1 = u1;
-    }
-    __syncthreads();
-}
-
 // One tile of a pair: its tokens and key blocks.
 struct TcSub {
     int token0, tokens;  // within the sequence's new tokens
@@ -531,7 +446,7 @@ struct TcMaps {
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
 tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, const __grid_constant__ TcPlan plan,
-                    float *__restrict__ partials, TcStart *__restrict__ starts)
+                    float *partials, unsigned long long *flags, unsigned long long launch)
 {
     using C = Tc<T, KT, D>;
     using MT = typename C::MT;
@@ -540,7 +455,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) unsigned long long bars[4 * NS + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
-    __shared__ TcStart begin;
+    __shared__ Start<TcIter> begin;
     __shared__ float row_q[8][D];
     // of f32 keys and values: each key's unit and its value's exponent, a copy a
     // warp, this block's and the next one's
@@ -579,13 +494,11 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
-    tc_find<kTcThreads>(plan, blockIdx.x, &begin);
+    find_start<kTcThreads>(plan, &begin);
     fence_after();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = tmem_slot;
     const long long u1 = begin.u1;
     TcIter it = begin.it;
-    if (starts != nullptr && tid == 0) starts[blockIdx.x] = begin;  // for the joining of partials
     const int sub = plan.sub;
     // the next segment of this CTA: blocks [it.b0, b1) of the pair
     auto segment = [&](int *b1) {
@@ -725,10 +638,33 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
                 fence_after();
             }
-            const bool whole = it.b0 == 0 && b1 == it.blocks;
-            if (whole) {
-                const float inv = 1.f / l;
+            const int share = my_share();
+            unsigned long long *flag = flags + 4 * x + quarter;  // of share 0; a warp's rows are joined by the same warp
+            if (it.b0 == 0) {
+                // shares share + 1 .. last hold the rest of the pair
+                const int last = b1 == it.blocks ? share : begin.deal.holder(it.origin + plan.over + (long long)kTcKeys * (it.blocks - 1));
+                auto part_of = [&](int p) { return partials + (size_t)p * C::kPartial + (size_t)x * (C::kPartial / C::kSubs); };
+                auto has_blocks = [&](int p) { return it.block_at(plan, begin.deal.first(p)) < it.block_at(plan, begin.deal.first(p + 1)); };
+                float mine = 1.f;
+                if (last > share) {
+                    float top = m;
+                    for (int p = share + 1; p <= last; ++p) {
+                        if (!has_blocks(p)) continue;
+                        if (lane == 0 && !flag_take(flag + (size_t)p * (4 * kTcSubs), launch)) report(a.status, kStatusAttentionWait);
+                        __syncwarp();
+                        top = fmaxf(top, __ldcg(part_of(p) + kTcRows * D + r));
+                    }
+                    mine = m == -INFINITY ? 0.f : ex2(m - top);
+                    m = top;
+                    l *= mine;
+                    for (int p = share + 1; p <= last; ++p) {
+                        if (!has_blocks(p)) continue;
+                        const float pm = __ldcg(part_of(p) + kTcRows * D + r);
+                        l += __ldcg(part_of(p) + kTcRows * D + kTcRows + r) * (pm == -INFINITY ? 0.f : ex2(pm - m));
+                    }
+                }
                 const bool none = keys <= 0;
+                const float inv = 1.f / l;
                 const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
                 T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D;
                 bool bad = false;
@@ -737,6 +673,25 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     float o[32];
                     tmem_ld32(o_t + c, o);
                     wait_ld();
+                    if (last > share) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= mine;
+#pragma unroll 1
+                        for (int p = share + 1; p <= last; ++p) {
+                            if (!has_blocks(p)) continue;
+                            const float *part = part_of(p);
+                            const float pm = __ldcg(part + kTcRows * D + r), f = pm == -INFINITY ? 0.f : ex2(pm - m);
+                            if (pm == -INFINITY) continue;  // no block of this tile: nothing was written
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 v = __ldcg((const float4 *)(part + ((c + i) / 4 * kTcRows + r) * 4));
+                                o[i] = fmaf(v.x, f, o[i]);
+                                o[i + 1] = fmaf(v.y, f, o[i + 1]);
+                                o[i + 2] = fmaf(v.z, f, o[i + 2]);
+                                o[i + 3] = fmaf(v.w, f, o[i + 3]);
+                            }
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         o[i] = none ? 0.f : o[i] * inv;
@@ -751,8 +706,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     attention_row<T, KT, D>(a, __shfl_sync(kFull, token_row, who), __shfl_sync(kFull, head, who), it.s, it.q, row_q[warp], 0, D);
                 }
             } else {
-                // a partial that starts inside its pair goes to the first slot
-                float *part = partials + (size_t)(2 * blockIdx.x + (it.b0 == 0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
+                float *part = partials + (size_t)share * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
                 if (any) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
@@ -766,6 +720,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
                 part[kTcRows * D + r] = m;
                 part[kTcRows * D + kTcRows + r] = l;
+                __syncwarp();
+                if (lane == 0) flag_set(flag + (size_t)share * (4 * kTcSubs), launch);
             }
             fence_before();
         }
@@ -967,77 +923,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
 }
 
-// Joins the partials of pairs cut between CTAs; the boundaries inside one
-// pair share its rows.  Partials are added in order.
-constexpr int kTcMergeThreads = 256;
-
-template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kTcMergeThreads) tc_merge_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ partials,
-                                                                   const TcStart *__restrict__ starts, const __grid_constant__ TcPlan plan)
-{
-    using C = Tc<T, KT, D>;
-    __shared__ float row_q[kTcMergeThreads / 32][D];
-    const int c = blockIdx.x + 1, x = blockIdx.y, warp = threadIdx.x >> 5;
-    // also by CTAs with nothing to join: the next launch of the stream follows this one
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TcIter it = starts[c].it;
-    if (it.s >= plan.sequences || it.b0 == 0) return;  // no pair is cut here
-    // CTAs c0 .. c1 hold the pair
-    int c0 = c, c1 = c;
-    while (starts[c0].u0 > it.origin + plan.over) --c0;
-    const long long last = it.origin + plan.over + (long long)kTcKeys * (it.blocks - 1);
-    while (c1 + 1 < plan.ctas.d && starts[c1 + 1].u0 <= last && starts[c1 + 1].it.s < plan.sequences) ++c1;
-    const int slice = c - c0 - 1, slices = c1 - c0;
-    const TcSub me(plan, it, x);
-    constexpr int G = D / 16;  // 16-column pieces of a row
-    const int rows = me.tokens * a.group, work = kTcRows * G;
-    const int w0 = (int)((long long)work * slice / slices), w1 = (int)((long long)work * (slice + 1) / slices);
-    for (int first = (w0 & ~31) + 32 * warp; first < w1; first += kTcMergeThreads) {
-        const int w = first + (int)(threadIdx.x & 31), r = w % kTcRows, g = w / kTcRows;
-        const bool live = w >= w0 && w < w1 && r < rows;
-        float m = -INFINITY, l = 0.f, o[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = 0.f;
-        for (int p = c0; live && p <= c1; ++p) {
-            if (p > c0 && it.block_at(plan, starts[p].u0) == it.block_at(plan, starts[p].u1)) continue;  // no block of its own
-            const float *part = partials + (size_t)(2 * p + (p == c0 ? 1 : 0)) * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
-            const float pm = part[kTcRows * D + r], pl = part[kTcRows * D + kTcRows + r];
-            if (pm == -INFINITY) continue;
-            const float mn = fmaxf(m, pm), fo = m == -INFINITY ? 0.f : ex2(m - mn), fn = ex2(pm - mn);
-            m = mn;
-            l = l * fo + pl * fn;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 v = *(const float4 *)(part + ((4 * g + i) * kTcRows + r) * 4);
-                o[4 * i] = o[4 * i] * fo + v.x * fn;
-                o[4 * i + 1] = o[4 * i + 1] * fo + v.y * fn;
-                o[4 * i + 2] = o[4 * i + 2] * fo + v.z * fn;
-                o[4 * i + 3] = o[4 * i + 3] * fo + v.w * fn;
-            }
-        }
-        const int token = r / a.group, head = it.h * a.group + r - token * a.group, token_row = it.q.row0 + me.token0 + token;
-        bool bad = false;
-        if (live) {
-            const bool none = it.q.keys - it.q.n + me.token0 + token + 1 <= 0;
-            const float inv = 1.f / l;
-            T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D + 16 * g;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                o[i] = none ? 0.f : o[i] * inv;
-                bad |= !isfinite(o[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i += Elem<T>::kVec) Elem<T>::store(out + i, o + i);
-        }
-        for (unsigned left = __ballot_sync(kFull, bad); left; left &= left - 1) {
-            const int who = __ffs(left) - 1;
-            const int row = __shfl_sync(kFull, token_row, who), hd = __shfl_sync(kFull, head, who), col = 16 * __shfl_sync(kFull, g, who);
-            __syncwarp();
-            attention_row<T, KT, D>(a, row, hd, it.s, it.q, row_q[warp], col, col + 16);
-        }
-    }
-}
-
 // ---------------------------------------------------------------- launch
 
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
@@ -1090,15 +975,15 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     const int64_t pairs = a.tokens / (sub * C::kSubs) + a.sequences, most = pairs * a.kv_heads * blocks;
     const int ctas = (int)(most < sms ? most : sms);
     const bool split = ctas > 1 && blocks > 1;
-    // scratch: partials | share starts | f16 planes of K and V | their units
-    const size_t part_bytes = split ? (size_t)2 * ctas * C::kPartial * sizeof(float) : 0, start_bytes = split ? (size_t)ctas * sizeof(TcStart) : 0;
-    const size_t plane_at = (part_bytes + start_bytes + 127) & ~(size_t)127, rows = (size_t)a.tokens * a.kv_heads;
+    // scratch: a partial a share | flags | f16 planes of K and V | their units
+    const size_t part_bytes = split ? (size_t)ctas * C::kPartial * sizeof(float) : 0, flag_bytes = split ? (size_t)ctas * 4 * C::kSubs * 8 : 0;
+    const size_t plane_at = (part_bytes + flag_bytes + 127) & ~(size_t)127, rows = (size_t)a.tokens * a.kv_heads;
     const size_t plane_bytes = C::kK == 2 ? rows * D * 4 : 0;  // two parts
     char *scratch = nullptr;
     if (split || C::kK == 2) e = stream_alloc((void **)&scratch, plane_at + 2 * plane_bytes + (C::kK == 2 ? rows * 8 : 0), s);
     if (e != cudaSuccess) return e;
     float *partials = split ? (float *)scratch : nullptr;
-    TcStart *starts = split ? (TcStart *)(scratch + part_bytes) : nullptr;
+    unsigned long long *flags = (unsigned long long *)(scratch + part_bytes);
     TcMaps maps{};
     const void *k = a.kv.k, *v = a.kv.v;
     if constexpr (C::kK == 2) {
@@ -1130,24 +1015,11 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     const cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
     if (e == cudaSuccess) e = make_map<MT>(&maps.k, k, 4, kd, ks, kb);
     if (e == cudaSuccess) e = make_map<MT>(&maps.v, v, 4, kd, vs, kb);
-    auto divisor = [](int d) { return Divisor{d > 1 ? ~0ull / (unsigned long long)d + 1 : ~0ull, d}; };
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
                       sub, divisor(sub * C::kSubs), divisor(ctas)};
     if (e == cudaSuccess) {
-        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, starts);
+        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, flags, launch_number());
         e = cudaGetLastError();
-    }
-    if (e == cudaSuccess && split) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)ctas - 1, C::kSubs);
-        cfg.blockDim = dim3(kTcMergeThreads);
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, tc_merge_kernel<T, KT, D>, a, (const float *)partials, (const TcStart *)starts, plan);
     }
     const cudaError_t f = stream_free(scratch, s);
     return e != cudaSuccess ? e : f;
