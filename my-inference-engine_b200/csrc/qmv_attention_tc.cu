@@ -211,6 +211,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r)
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+        : "memory");
+}
+
 // Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 rows x 128
 // bytes, 1024 bytes apart along the rows).  K-major (Q, K): the contiguous
 // 64 elements run along the reduction.  MN-major (V): they run along the
@@ -232,40 +241,62 @@ template <typename KT> __host__ __device__ constexpr uint32_t idesc(int n, bool 
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// One f32 row as two f16 rows in swizzled shared memory (row r of a tile and
-// of the tile behind it): x = (hi + lo) 2^-e, the largest |x| in [2^14, 2^15)
-// after the shift; 2^-e is returned.  A row that is not there: zeros.
-template <int D> __device__ __forceinline__ float split_row(const float *x, bool live, uint32_t tile, int r)
+// Two keys' units and exponents; volatile, so that 128 of them are not held in
+// registers between the passes over a row.
+__device__ __forceinline__ float4 lds4(const float2 *p)
 {
-    float big = 0.f;
-    if (live) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    return v;
+}
+
+// 2^n for a whole number |n| <= 60 held in a float.
+__device__ __forceinline__ float power(float n) { return __uint_as_float(__float_as_uint(n + 12583039.f) << 23); }
+
+// A warp's 32 f32 rows of Q (rows 32 * quarter .. of the tile) as two f16 rows
+// each in swizzled shared memory, the second in the tile behind: x = (hi + lo)
+// 2^-e, the largest |x| of a row in [2^14, 2^15) after the shift.  2^-e of each
+// lane's own row is returned.  D / 4 lanes take a row, 16 bytes each; rows
+// without a token are zeros.
+template <int D> __device__ __forceinline__ float split_rows(const AttnArgs &a, int token_row0, int tokens, int head0, uint32_t tile, int quarter)
+{
+    constexpr int L = D / 4, R = 32 / L, N = 8;  // lanes a row, rows a load, loads in flight
+    const int lane = threadIdx.x & 31, l = lane % L;
+    float unit = 1.f;
+#pragma unroll 1
+    for (int g = 0; g < 32 / R; g += N) {
+        float4 v[N];
 #pragma unroll
-        for (int i = 0; i < D; i += 4) {
-            const float4 v = *(const float4 *)(x + i);
-            big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        for (int i = 0; i < N; ++i) {
+            const int r = 32 * quarter + (g + i) * R + lane / L, token = r / a.group;
+            v[i] = token < tokens ? *(const float4 *)((const float *)a.q + (int64_t)(token_row0 + token) * a.q_ld +
+                                                       (int64_t)(head0 + r - token * a.group) * D + 4 * l)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = 32 * quarter + (g + i) * R + lane / L;
+            float big = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+#pragma unroll
+            for (int d = L / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, d));
+            const int e = min(max(14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127, -100), 100);
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+            const uint32_t h0 = pack2<__half>(v[i].x * up, v[i].y * up), h1 = pack2<__half>(v[i].z * up, v[i].w * up);
+            const uint32_t l0 = pack2_rest(v[i].x * up, v[i].y * up, h0), l1 = pack2_rest(v[i].z * up, v[i].w * up, h1);
+            const uint32_t to = tile + (uint32_t)(l / 16) * 16384u + (uint32_t)r * 128u + (uint32_t)((((l / 2) & 7) ^ (r & 7)) * 16 + (l & 1) * 8);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(h0), "r"(h1) : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + 128u * D * 2u), "r"(l0), "r"(l1) : "memory");
+            // to the lane whose row it is: row (g + i) R + k of the warp is lane L k's
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float u = __shfl_sync(kFull, __uint_as_float((uint32_t)(127 - e) << 23), L * k);
+                if (lane == (g + i) * R + k) unit = u;
+            }
         }
     }
-    const int e = min(max(14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127, -100), 100);
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-    for (int i = 0; i < D; i += 8) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            const float4 y = *(const float4 *)(x + i), z = *(const float4 *)(x + i + 4);
-            v[0] = y.x * up; v[1] = y.y * up; v[2] = y.z * up; v[3] = y.w * up;
-            v[4] = z.x * up; v[5] = z.y * up; v[6] = z.z * up; v[7] = z.w * up;
-        }
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            h[j] = pack2<__half>(v[2 * j], v[2 * j + 1]);
-            l[j] = pack2_rest(v[2 * j], v[2 * j + 1], h[j]);
-        }
-        const uint32_t to = tile + (uint32_t)(i / 64) * 16384u + (uint32_t)r * 128u + (uint32_t)((((i / 8) & 7) ^ (r & 7)) * 16);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 128u * D * 2u), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
-    }
-    return __uint_as_float((uint32_t)(127 - e) << 23);
+    return unit;
 }
 
 // f32 keys and values as two f16 planes [part][token][kv_heads * D] and their
@@ -459,7 +490,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     __shared__ float row_q[8][D];
     // of f32 keys and values: each key's unit and its value's exponent, a copy a
     // warp, this block's and the next one's
-    __shared__ float2 key_of[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];
+    __shared__ __align__(16) float2 key_of[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kQTile, v_s = k_s + NS * C::kKTile;
@@ -522,7 +553,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = b * kTcKeys + 32 * i + lane;
-                u[i] = j < it.q.keys ? make_float2(__ldg(maps.key_unit + at + j), __ldg(maps.value_exp + at + j)) : make_float2(0.f, 0.f);
+                u[i] = j < it.q.keys ? make_float2(__ldg(maps.key_unit + at + j), __ldg(maps.value_exp + at + j)) : make_float2(1.f, 0.f);
             }
         };
         for (; x < kTcSubs && ok && segment(&b1); it.next(plan)) {
@@ -538,8 +569,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 // this thread's row of Q as two f16 rows; the QK products of
                 // the tile before have ended, since their scores were read
                 if (end > it.b0) {
-                    f *= split_row<D>((const float *)a.q + (int64_t)(row ? token_row : 0) * a.q_ld + (int64_t)(row ? head : 0) * D, row,
-                                      q_s + x * C::kQTile, r);
+                    f *= split_rows<D>(a, it.q.row0 + me.token0, me.tokens, it.h * a.group, q_s + x * C::kQTile, quarter);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) bar_arrive(q_full + 8 * x);
@@ -566,8 +596,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     for (int i = 0; i < 4; ++i) key_of[warp][b & 1][32 * i + lane] = next_units[i];
                     __syncwarp();
                     if (b + 1 < end) units_of(b + 1, next_units);
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] *= unit[i].x;
                 }
                 if (__any_sync(kFull, j0 + kTcKeys > lim)) {
 #pragma unroll
@@ -578,7 +606,16 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 // exponents of their own, of the weight that meets the value
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], C::kK == 2 ? fmaf(s[i], f, unit[i].y) : s[i]);
+                for (int i = 0; i < 128; i += 2) {
+                    float y = s[i], z = s[i + 1];
+                    if constexpr (C::kK == 2) {
+                        const float4 u = lds4(unit + i);
+                        y = fmaf(y * u.x, f, u.y);
+                        z = fmaf(z * u.z, f, u.w);
+                    }
+                    top[i & 3] = fmaxf(top[i & 3], y);
+                    top[(i + 1) & 3] = fmaxf(top[(i + 1) & 3], z);
+                }
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (C::kK == 2 ? 1.f : f);
                 const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
                 // P and O as the block before this one left them
@@ -605,24 +642,34 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 const float base = m == -INFINITY ? 0.f : m - kLift;
                 const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                constexpr int W = C::kQ == 2 ? 16 : 32;  // columns of P a store
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t p[32], rest[C::kQ == 2 ? 32 : 1];
+                for (int h = 0; h < 64 / W; ++h) {
+                    uint32_t p[W], rest[C::kQ == 2 ? W : 1];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int j = 64 * h + 2 * i;
-                        const float2 of = C::kK == 2 ? make_float2(unit[j].y, unit[j + 1].y) : make_float2(0.f, 0.f);
-                        const float2 e = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, C::kK == 2 ? __fadd2_rn(n2, of) : n2);
+                    for (int i = 0; i < W; ++i) {
+                        const int j = 2 * (W * h + i);
+                        float2 at = make_float2(s[j], s[j + 1]), of = make_float2(0.f, 0.f);
+                        if constexpr (C::kK == 2) {
+                            const float4 u = lds4(unit + j);
+                            at = __fmul2_rn(at, make_float2(u.x, u.z));
+                            of = make_float2(u.y, u.w);
+                        }
+                        const float2 e = __ffma2_rn(at, f2, C::kK == 2 ? __fadd2_rn(n2, of) : n2);
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         if constexpr (C::kK == 2)
-                            sum[i & 1] = __ffma2_rn(w, make_float2(ex2(-of.x), ex2(-of.y)), sum[i & 1]);
+                            sum[i & 1] = __ffma2_rn(w, make_float2(power(-of.x), power(-of.y)), sum[i & 1]);
                         else
                             sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                         p[i] = pack2<MT>(w.x, w.y);
                         if constexpr (C::kQ == 2) rest[i] = pack2_rest(w.x, w.y, p[i]);
                     }
-                    tmem_st32(p_t + 32 * h, p);
-                    if constexpr (C::kQ == 2) tmem_st32(p_t + 64 + 32 * h, rest);
+                    if constexpr (C::kQ == 2) {
+                        tmem_st16(p_t + W * h, p);
+                        tmem_st16(p_t + 64 + W * h, rest);
+                    } else {
+                        tmem_st32(p_t + W * h, p);
+                    }
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 wait_st();
