@@ -56,9 +56,10 @@ template <typename T, typename KT, int D> struct Tc {
     static constexpr int kK = sizeof(KT) == 4 ? 2 : 1;  // parts of K and V
     using MT = typename std::conditional<kQ == 2, __half, T>::type;
     static constexpr int kSubs = kQ == 2 && D == 128 ? 1 : 2;  // tiles of a CTA: what tensor memory holds
-    // What a pair of tiles costs beside its keys, in keys: 4600 cycles at
-    // head_dim 64 and 6700 at 128, where 128 keys take 2560 and 2300.
-    static constexpr int kOver = D == 64 ? 256 : 384;
+    // What a pair of tiles costs beside its keys, in keys, from measured cycles
+    // of a pair and of a block: 16 bits 4600 / 2560 (head_dim 64), 6700 / 2300
+    // (128); f32 over f16 keys 14500 / 2700, over f32 keys 16300 / 6800 (64).
+    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 256 : 384;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
@@ -262,15 +263,16 @@ __device__ __forceinline__ float power(float n) { return __uint_as_float(__float
 // without a token are zeros.
 template <int D> __device__ __forceinline__ float split_rows(const AttnArgs &a, int token_row0, int tokens, int head0, uint32_t tile, int quarter)
 {
-    constexpr int L = D / 4, R = 32 / L, N = 8;  // lanes a row, rows a load, loads in flight
+    constexpr int L = D / 4, R = 32 / L, N = 16;  // lanes a row, rows a load, loads in flight
     const int lane = threadIdx.x & 31, l = lane % L;
+    const float per_head = 1.f / (float)a.group;  // (r + 1/2) times it, cut: r / group for r < 128 and groups to 64
     float unit = 1.f;
 #pragma unroll 1
     for (int g = 0; g < 32 / R; g += N) {
         float4 v[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r = 32 * quarter + (g + i) * R + lane / L, token = r / a.group;
+            const int r = 32 * quarter + (g + i) * R + lane / L, token = (int)(((float)r + 0.5f) * per_head);
             v[i] = token < tokens ? *(const float4 *)((const float *)a.q + (int64_t)(token_row0 + token) * a.q_ld +
                                                        (int64_t)(head0 + r - token * a.group) * D + 4 * l)
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -499,6 +501,11 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                    s_full = q_empty + 8 * kTcSubs, s_free = s_full + 8 * kTcSubs, p_full = s_free + 8 * kTcSubs,
                    pv_done = p_full + 8 * kTcSubs, tail_bar = pv_done + 8 * kTcSubs, drain_bar = tail_bar + 8;
 
+    if (tid == 32 * kTcLoadVWarp) {
+        if (C::kQ == 1) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             bar_init(k_full + 8 * i, 1);
