@@ -194,6 +194,7 @@ template <typename KT> __device__ __forceinline__ void mma16816(float d[4], cons
 // What a sequence costs, in blocks of keys: row tiles x heads items, each of
 // its key blocks and of kDcItemCost for its beginning and end.
 struct DcPlan {
+    static constexpr int kLeast = 2;  // units: one takes as long, for its latencies
     const int *start, *length;
     int sequences, tokens, max_keys, kv_heads, group;
     Divisor ctas;

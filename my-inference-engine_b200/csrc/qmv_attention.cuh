@@ -192,13 +192,20 @@ inline Divisor divisor(int d) { return Divisor{d > 1 ? ~0ull / (unsigned long lo
 struct Deal {
     long long each;
     int more, shares;  // the first `more` shares get one place more
-    static __device__ __forceinline__ Deal of(long long total, const Divisor &d)
+    // No share below `least` places (but the only one): a join costs more than a
+    // short share saves.
+    static __device__ __forceinline__ Deal of(long long total, const Divisor &d, int least)
     {
         Deal t;
-        t.each = (long long)__umul64hi((unsigned long long)total, d.magic);
-        if (t.each * d.d > total) --t.each;
-        t.more = (int)(total - t.each * d.d);
-        t.shares = d.d;
+        if (total >= (long long)least * d.d) {
+            t.each = (long long)__umul64hi((unsigned long long)total, d.magic);
+            if (t.each * d.d > total) --t.each;
+            t.shares = d.d;
+        } else {
+            t.shares = max(1, (int)total / least);
+            t.each = (int)total / t.shares;
+        }
+        t.more = (int)(total - t.each * t.shares);
         return t;
     }
     __device__ __forceinline__ long long first(int c) const { return each * c + (c < more ? c : more); }
@@ -285,10 +292,10 @@ template <int NT, typename Plan, typename Iter> __device__ __forceinline__ void 
         v += p.cost(q);
     }
     long long at = block_scan<NT>(v, &all);
-    const Deal deal = Deal::of(all, p.ctas);
+    const Deal deal = Deal::of(all, p.ctas, Plan::kLeast);
     const int c = my_share();
     const long long u0 = deal.first(c), u1 = deal.first(c + 1);
-    if (u0 >= u1) {
+    if (c >= deal.shares || u0 >= u1) {
         if (threadIdx.x == 0) {
             out->it.s = p.sequences;
             out->u0 = out->u1 = 0;

@@ -369,6 +369,7 @@ template <typename T> __device__ __forceinline__ void store32(T *out, const floa
 // ------------------------------------------------------------------ work
 
 struct TcPlan {
+    static constexpr int kLeast = 512;  // keys
     const int *start, *length;
     int sequences, tokens, max_keys, kv_heads, over;
     int sub;       // tokens of a tile
@@ -475,6 +476,167 @@ struct TcMaps {
     const float *key_unit, *value_exp;
 };
 
+
+// The output of an uncut pair's row: O from tensor memory times inv (0: a row
+// without keys), written where the row has a token (token_row >= 0).  This and
+// tc_join are not inlined: their registers would be taken from the softmax
+// loop (440 and not 400 us for a prompt of 8192 tokens).
+template <typename T, typename KT, int D>
+__device__ __noinline__ void tc_store(const AttnArgs &a, uint32_t o_t, float inv, int token_row, int head, int s, Seq q, float *row_q)
+{
+    const bool row = token_row >= 0, wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
+    T *out = (T *)a.out + (int64_t)(row ? token_row : 0) * a.out_ld + (int64_t)head * D;
+    bool bad = false;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+        float o[32];
+        tmem_ld32(o_t + c, o);
+        wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            o[i] = inv == 0.f ? 0.f : o[i] * inv;
+            bad |= !isfinite(o[i]);
+        }
+        if (row) store32<T>(out + c, o, wide);
+    }
+    // a masked NaN or infinity met the sums: those rows again, without it
+    for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
+        const int who = __ffs(left) - 1;
+        __syncwarp();
+        attention_row<T, KT, D>(a, __shfl_sync(kFull, token_row, who), __shfl_sync(kFull, head, who), s, q, row_q, 0, D);
+    }
+}
+
+// What a softmax thread has of its row when its segment ends.
+struct TcRow {
+    float m, l;
+    int keys, token_row, head;
+    bool row;  // a row with a token
+    bool any;  // the segment holds blocks of this tile
+};
+
+// Ends a segment of a cut pair, tile x: the output, or a partial.  Of the shares c0 ..
+// last that hold a cut pair, every eighth (c0 + 8 k) joins the seven behind
+// it, and c0 joins its seven and the joined eighths: a share waits for later
+// ones only, and 37 shares of one long context take 11 + 7 steps and not 36.
+constexpr int kJoin = 8;
+
+template <typename T, typename KT, int D>
+__device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, const TcIter &it, const Deal &deal, int x, uint32_t o_t, TcRow w,
+                                     float *partials, unsigned long long *flags, unsigned long long launch, float *row_q)
+{
+    using C = Tc<T, KT, D>;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, r = 32 * quarter + lane, share = my_share();
+    const long long first_place = it.origin + plan.over, last_place = first_place + (long long)kTcKeys * (it.blocks - 1);
+    const int c0 = it.b0 == 0 ? share : deal.holder(first_place), last = deal.holder(last_place);
+    // the shares that this one joins
+    const int mine8 = (share - c0) % kJoin == 0 ? min(kJoin - 1, last - share) : 0;
+    const int sources = mine8 + (share == c0 ? (last - c0) / kJoin : 0);
+    auto source = [&](int k) { return k < mine8 ? share + 1 + k : share + kJoin * (k - mine8 + 1); };
+    auto part_of = [&](int p) { return partials + (size_t)p * C::kPartial + (size_t)x * (C::kPartial / C::kSubs); };
+    // (every one of them has blocks of the pair: it is kLeast places long, or the
+    // last)
+    static_assert(TcPlan::kLeast >= kTcKeys, "a share between two block borders would have none");
+    unsigned long long *flag = flags + 4 * x + quarter;  // of share 0; a warp's rows are joined by the same warp
+    float mine = 1.f;
+    if (sources > 0) {
+        bool good = true;
+        for (int k = lane; k < sources; k += 32) good &= flag_take(flag + (size_t)source(k) * (4 * C::kSubs), launch);
+        if (!good) report(a.status, kStatusAttentionWait);
+        __syncwarp();
+        float top = w.m, sum = 0.f;
+        for (int k0 = 0; k0 < sources; k0 += 4) {
+            float pm[4], pl[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float *stat = part_of(source(min(k0 + k, sources - 1))) + kTcRows * D + r;
+                pm[k] = k0 + k < sources ? __ldcg(stat) : -INFINITY;
+                pl[k] = __ldcg(stat + kTcRows);
+            }
+            const float before = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, pm[k]);
+            sum *= before == -INFINITY ? 0.f : ex2(before - top);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum += pm[k] == -INFINITY ? 0.f : pl[k] * ex2(pm[k] - top);
+        }
+        mine = w.m == -INFINITY ? 0.f : ex2(w.m - top);
+        w.m = top;
+        w.l = w.l * mine + sum;
+    }
+    const bool whole = share == c0, none = w.keys <= 0;
+    const float scale = whole ? (none ? 0.f : 1.f / w.l) : 1.f;
+    const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
+    T *out = (T *)a.out + (int64_t)w.token_row * a.out_ld + (int64_t)w.head * D;
+    float *part = part_of(share);
+    float check = 0.f;  // 0 times a value is 0, or NaN where the value is not finite
+    if (w.any || sources > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            float o[32];
+            if (w.any) {
+                tmem_ld32(o_t + c, o);
+                wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            }
+            if (sources > 0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= mine;
+#pragma unroll 1
+                for (int k0 = 0; k0 < sources; k0 += 2) {
+                    float f[2];
+                    float4 v[2][8];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float *from = part_of(source(min(k0 + k, sources - 1)));
+                        const float pm = k0 + k < sources ? __ldcg(from + kTcRows * D + r) : -INFINITY;
+                        f[k] = pm == -INFINITY ? 0.f : ex2(pm - w.m);
+                        // (where the source has no block of this tile, nothing was written)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            v[k][i] = pm == -INFINITY ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg((const float4 *)(from + ((c / 4 + i) * kTcRows + r) * 4));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            o[4 * i] = fmaf(v[k][i].x, f[k], o[4 * i]);
+                            o[4 * i + 1] = fmaf(v[k][i].y, f[k], o[4 * i + 1]);
+                            o[4 * i + 2] = fmaf(v[k][i].z, f[k], o[4 * i + 2]);
+                            o[4 * i + 3] = fmaf(v[k][i].w, f[k], o[4 * i + 3]);
+                        }
+                }
+            }
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    o[i] = none ? 0.f : o[i] * scale;
+                    check = fmaf(o[i], 0.f, check);
+                }
+                if (w.row) store32<T>(out + c, o, wide);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *(float4 *)(part + ((c + i) / 4 * kTcRows + r) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+        }
+    }
+    if (whole) {
+        // a masked NaN or infinity met the sums: those rows again, without it
+        for (unsigned left = __ballot_sync(kFull, w.row && !(check == 0.f)); left; left &= left - 1) {
+            const int who = __ffs(left) - 1;
+            __syncwarp();
+            attention_row<T, KT, D>(a, __shfl_sync(kFull, w.token_row, who), __shfl_sync(kFull, w.head, who), it.s, it.q, row_q, 0, D);
+        }
+    } else {
+        part[kTcRows * D + r] = w.any || sources > 0 ? w.m : -INFINITY;
+        part[kTcRows * D + kTcRows + r] = w.l;
+        __syncwarp();
+        if (lane == 0) flag_set(flag + (size_t)share * (4 * C::kSubs), launch);
+    }
+}
 
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -692,90 +854,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
                 fence_after();
             }
-            const int share = my_share();
-            unsigned long long *flag = flags + 4 * x + quarter;  // of share 0; a warp's rows are joined by the same warp
-            if (it.b0 == 0) {
-                // shares share + 1 .. last hold the rest of the pair
-                const int last = b1 == it.blocks ? share : begin.deal.holder(it.origin + plan.over + (long long)kTcKeys * (it.blocks - 1));
-                auto part_of = [&](int p) { return partials + (size_t)p * C::kPartial + (size_t)x * (C::kPartial / C::kSubs); };
-                auto has_blocks = [&](int p) { return it.block_at(plan, begin.deal.first(p)) < it.block_at(plan, begin.deal.first(p + 1)); };
-                float mine = 1.f;
-                if (last > share) {
-                    float top = m;
-                    for (int p = share + 1; p <= last; ++p) {
-                        if (!has_blocks(p)) continue;
-                        if (lane == 0 && !flag_take(flag + (size_t)p * (4 * kTcSubs), launch)) report(a.status, kStatusAttentionWait);
-                        __syncwarp();
-                        top = fmaxf(top, __ldcg(part_of(p) + kTcRows * D + r));
-                    }
-                    mine = m == -INFINITY ? 0.f : ex2(m - top);
-                    m = top;
-                    l *= mine;
-                    for (int p = share + 1; p <= last; ++p) {
-                        if (!has_blocks(p)) continue;
-                        const float pm = __ldcg(part_of(p) + kTcRows * D + r);
-                        l += __ldcg(part_of(p) + kTcRows * D + kTcRows + r) * (pm == -INFINITY ? 0.f : ex2(pm - m));
-                    }
-                }
-                const bool none = keys <= 0;
-                const float inv = 1.f / l;
-                const bool wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
-                T *out = (T *)a.out + (int64_t)token_row * a.out_ld + (int64_t)head * D;
-                bool bad = false;
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    tmem_ld32(o_t + c, o);
-                    wait_ld();
-                    if (last > share) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] *= mine;
-#pragma unroll 1
-                        for (int p = share + 1; p <= last; ++p) {
-                            if (!has_blocks(p)) continue;
-                            const float *part = part_of(p);
-                            const float pm = __ldcg(part + kTcRows * D + r), f = pm == -INFINITY ? 0.f : ex2(pm - m);
-                            if (pm == -INFINITY) continue;  // no block of this tile: nothing was written
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                const float4 v = __ldcg((const float4 *)(part + ((c + i) / 4 * kTcRows + r) * 4));
-                                o[i] = fmaf(v.x, f, o[i]);
-                                o[i + 1] = fmaf(v.y, f, o[i + 1]);
-                                o[i + 2] = fmaf(v.z, f, o[i + 2]);
-                                o[i + 3] = fmaf(v.w, f, o[i + 3]);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        o[i] = none ? 0.f : o[i] * inv;
-                        bad |= !isfinite(o[i]);
-                    }
-                    if (row) store32<T>(out + c, o, wide);
-                }
-                // a masked NaN or infinity met the sums: those rows again, without it
-                for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
-                    const int who = __ffs(left) - 1;
-                    __syncwarp();
-                    attention_row<T, KT, D>(a, __shfl_sync(kFull, token_row, who), __shfl_sync(kFull, head, who), it.s, it.q, row_q[warp], 0, D);
-                }
+            if (it.b0 > 0 || b1 < it.blocks) {
+                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, launch, row_q[warp]);
             } else {
-                float *part = partials + (size_t)share * C::kPartial + (size_t)x * (C::kPartial / C::kSubs);
-                if (any) {
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        tmem_ld32(o_t + c, o);
-                        wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *(float4 *)(part + ((c + i) / 4 * kTcRows + r) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    }
-                }
-                part[kTcRows * D + r] = m;
-                part[kTcRows * D + kTcRows + r] = l;
-                __syncwarp();
-                if (lane == 0) flag_set(flag + (size_t)share * (4 * kTcSubs), launch);
+                tc_store<T, KT, D>(a, o_t, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, it.s, it.q, row_q[warp]);
             }
             fence_before();
         }
