@@ -26,97 +26,111 @@ __device__ unsigned int g_attention_status;
 
 // ------------------------------------------------------ rope and append
 //
-// One CTA a token.  Its angles are formed once, in fixed point: position *
+// One CTA a token, or two neighbours where there are many, so that the chain
+// from the sequence over its length and page to the first store is paid once
+// for both.  Each token's angles are formed once, in fixed point: position *
 // base^(-2i / D) / 2 pi turns, the factor held as 64 bits of a turn, so the
 // product modulo one turn is exact to position * 2^-65 turns and no position
 // is too far for the f32 sine.  Threads then take 16-byte pieces of the
 // first half of a head together with the pieces of the second half that they
-// turn with, for all query and key heads, and the value pieces.
-// Bound by bytes: q, k and v are read once and written once.
+// turn with, for all query and key heads, and the value pieces; a thread's
+// first piece is on its way while the sequence, the page and the angles are found.
+// Bound by bytes, q, k and v being read once and written once, and by that
+// chain: 6789 tokens (bf16, 28/4/128; 125 MB) take 31 us, 4.1 TB/s; with four
+// or eight tokens a CTA registers cost more than the chain saves (45, 59 us at 9600).
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 512;  // at most: a thread a piece, as far as they go
 
 struct Turns {
     unsigned long long f[64];  // fraction of a turn a position, times 2^64
 };
 
-template <typename T, typename KT, int D>
+template <typename T, typename KT, int D, int R>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs a, const __grid_constant__ Turns turns)
 {
     constexpr int V = Elem<T>::kVec, H = D / 2, U = H / V;  // pieces of a half head
-    __shared__ float cs[H], sn[H];
-    const int row = blockIdx.x;
-    if (row == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
-    const int s = find_sequence(a.start, a.sequences, row);
-    const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
-    const int i = row - sq.row0, pos = sq.keys - sq.n + i;
-    if (i < 0 || i >= sq.n || pos < 0) return;  // the same for the whole CTA
-    const int page = __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (pos >> a.kv.page_shift));
-    const bool stored = page >= 0 && page < a.kv.page_count;
-    if (!stored && threadIdx.x == 0) report(a.status, kStatusBadMetadata);
+    __shared__ float cs[R][H], sn[R][H];
+    __shared__ int position[R];  // -1: not a token to append
+    __shared__ int64_t slot[R];  // its place in a page's keys, -1: nowhere
+    const int row0 = (int)blockIdx.x * R, warp = threadIdx.x >> 5;
+    const int nq = a.q_out ? a.heads * U : 0, nk = a.kv_heads * U, total = nq + 2 * nk;
+    uint4 raw_x[R], raw_y[R];
+    auto fetch = [&](int i, int u) {
+        const int row = row0 + i;
+        if (row >= a.tokens) return;
+        const bool is_q = u < nq, is_v = u >= nq + nk;
+        const int w = is_q ? u : is_v ? u - nq - nk : u - nq;
+        const T *src = is_q ? (const T *)a.q + (int64_t)row * a.q_ld : is_v ? (const T *)a.v + (int64_t)row * a.v_ld : (const T *)a.k + (int64_t)row * a.k_ld;
+        src += w / U * D + (w % U) * V;
+        raw_x[i] = *(const uint4 *)src;
+        raw_y[i] = *(const uint4 *)(src + H);
+    };
+    if ((int)threadIdx.x < total) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) fetch(i, threadIdx.x);
+    }
+    if (row0 == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
+    for (int i = warp; i < R; i += (int)(blockDim.x >> 5)) {  // a warp a token
+        const int row = row0 + i;
+        const int s = find_sequence(a.start, a.sequences, row);
+        const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
+        const int at = row - sq.row0, pos = sq.keys - sq.n + at;
+        const bool live = at >= 0 && at < sq.n && pos >= 0;
+        const int page = live ? __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (pos >> a.kv.page_shift)) : -1;
+        const bool stored = page >= 0 && page < a.kv.page_count;
+        if ((threadIdx.x & 31) == 0) {
+            if (live && !stored) report(a.status, kStatusBadMetadata);
+            position[i] = live ? pos : -1;
+            slot[i] = stored ? (int64_t)page * a.kv.page + (int64_t)(pos & ((1 << a.kv.page_shift) - 1)) * a.kv.k_pos : -1;
+        }
+    }
+    __syncthreads();
     const bool rope = a.rope_base > 0.f;
     if (rope) {
-        for (int e = threadIdx.x; e < H; e += kAppendThreads) {
+        for (int e = threadIdx.x; e < R * H; e += (int)blockDim.x) {
             // the signed fraction of a turn in [-1/2, 1/2): angle / pi = 2 * fraction
-            const long long frac = (long long)((unsigned long long)pos * turns.f[e]);
-            sincospif((float)frac * 1.0842021724855044e-19f, &sn[e], &cs[e]);  // 2^-63
+            const long long frac = (long long)((unsigned long long)position[e / H] * turns.f[e % H]);
+            sincospif((float)frac * 1.0842021724855044e-19f, &sn[e / H][e % H], &cs[e / H][e % H]);  // 2^-63
         }
         __syncthreads();
     }
-    const int64_t slot = (int64_t)page * a.kv.page + (int64_t)(pos & ((1 << a.kv.page_shift) - 1)) * a.kv.k_pos;
-    KT *kc = (KT *)const_cast<void *>(a.kv.k) + slot, *vc = (KT *)const_cast<void *>(a.kv.v) + slot;
-    const T *q = (const T *)a.q + (int64_t)row * a.q_ld, *k = (const T *)a.k + (int64_t)row * a.k_ld;
-    const T *v = (const T *)a.v + (int64_t)row * a.v_ld;
-    T *qo = (T *)a.q_out + (int64_t)row * a.q_out_ld, *ko = (T *)a.k_out + (int64_t)row * a.k_out_ld;
-    const int nq = a.q_out ? a.heads * U : 0, nk = a.kv_heads * U, total = nq + 2 * nk;
-    for (int u = threadIdx.x; u < total; u += kAppendThreads) {
+    for (int u = threadIdx.x; u < total; u += (int)blockDim.x) {
         const bool is_q = u < nq, is_v = u >= nq + nk;
         const int w = is_q ? u : is_v ? u - nq - nk : u - nq;
         const int head = w / U, e = (w % U) * V;
-        const T *src = (is_q ? q : is_v ? v : k) + head * D + e;
-        float x[V], y[V];
-        Elem<T>::load(src, x);
-        Elem<T>::load(src + H, y);
-        if (rope && !is_v) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float c = cs[e + j], n = sn[e + j], xr = x[j] * c - y[j] * n, yr = x[j] * n + y[j] * c;
-                x[j] = xr;
-                y[j] = yr;
+        for (int i = 0; i < R; ++i) {
+            if (position[i] < 0) continue;
+            if (u != (int)threadIdx.x) fetch(i, u);
+            float x[V], y[V];
+            Elem<T>::unpack(raw_x[i], x);
+            Elem<T>::unpack(raw_y[i], y);
+            if (rope && !is_v) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float c = cs[i][e + j], n = sn[i][e + j], xr = x[j] * c - y[j] * n, yr = x[j] * n + y[j] * c;
+                    x[j] = xr;
+                    y[j] = yr;
+                }
             }
-        }
-        T *out = is_q ? qo + head * D + e : ko + head * D + e;
-        if (is_q || (!is_v && a.k_out)) {
-            Elem<T>::store(out, x);
-            Elem<T>::store(out + H, y);
-        }
-        if (!is_q && stored) {
-            KT *dst = (is_v ? vc : kc) + head * a.kv.head + e;
-            if constexpr (sizeof(T) == sizeof(KT)) {
-                Elem<KT>::store(dst, x);
-                Elem<KT>::store(dst + H, y);
-            } else {
-                __half2 p[4] = {__floats2half2_rn(x[0], x[1]), __floats2half2_rn(x[2], x[3]), __floats2half2_rn(y[0], y[1]),
-                                __floats2half2_rn(y[2], y[3])};
-                *(uint2 *)dst = *(const uint2 *)&p[0];
-                *(uint2 *)(dst + H) = *(const uint2 *)&p[2];
+            if (is_q || (!is_v && a.k_out)) {
+                T *out = is_q ? (T *)a.q_out + (int64_t)(row0 + i) * a.q_out_ld : (T *)a.k_out + (int64_t)(row0 + i) * a.k_out_ld;
+                out += head * D + e;
+                Elem<T>::store(out, x);
+                Elem<T>::store(out + H, y);
+            }
+            if (!is_q && slot[i] >= 0) {
+                KT *dst = (KT *)const_cast<void *>(is_v ? a.kv.v : a.kv.k) + slot[i] + head * a.kv.head + e;
+                if constexpr (sizeof(T) == sizeof(KT)) {
+                    Elem<KT>::store(dst, x);
+                    Elem<KT>::store(dst + H, y);
+                } else {
+                    *(uint2 *)dst = make_uint2(pack2<KT>(x[0], x[1]), pack2<KT>(x[2], x[3]));
+                    *(uint2 *)(dst + H) = make_uint2(pack2<KT>(y[0], y[1]), pack2<KT>(y[2], y[3]));
+                }
             }
         }
     }
-}
-
-constexpr int kRowWarps = 4;
-
-template <typename T, typename KT, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) attention_rows_kernel(AttnArgs a)
-{
-    __shared__ float qs[kRowWarps][D];
-    if (blockIdx.x == 0 && blockIdx.y == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
-    const int row = blockIdx.x, warp = threadIdx.x >> 5, head = blockIdx.y * kRowWarps + warp;
-    const int s = find_sequence(a.start, a.sequences, row);
-    const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
-    if (row < sq.row0 || row >= sq.row0 + sq.n || head >= a.heads) return;
-    attention_row<T, KT, D>(a, row, head, s, sq, qs[warp], 0, D);
 }
 
 // ------------------------------------------------- paged decode attention
@@ -601,10 +615,9 @@ const Turns &turns_of(float base, int d)
     return t;
 }
 
+// Activations with the 16-bit caches they go with.
 template <typename F> cudaError_t by_type(uint32_t type, uint32_t kv_type, int d, const F &f)
 {
-    if (type == kTypeF32 && kv_type == kTypeF32)
-        return d == 64 ? f(float{}, float{}, std::integral_constant<int, 64>{}) : f(float{}, float{}, std::integral_constant<int, 128>{});
     if (type == kTypeF32 && kv_type == kTypeF16)
         return d == 64 ? f(float{}, __half{}, std::integral_constant<int, 64>{}) : f(float{}, __half{}, std::integral_constant<int, 128>{});
     if (type == kTypeF16 && kv_type == kTypeF16)
@@ -621,7 +634,15 @@ cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s)
 {
     const Turns &turns = turns_of(a.rope_base, a.head_dim);
     return by_type(a.type, a.kv_type, a.head_dim, [&](auto t, auto kt, auto d) {
-        paged_append_kernel<decltype(t), decltype(kt), d.value><<<(unsigned)a.tokens, kAppendThreads, 0, s>>>(a, turns);
+        using T = decltype(t);
+        const int pieces = ((a.q_out ? a.heads : 0) + 2 * a.kv_heads) * (d.value / 2 / Elem<T>::kVec), threads = (pieces + 31) / 32 * 32;
+        const int block = threads < 64 ? 64 : threads < kAppendThreads ? threads : kAppendThreads;
+        // two tokens a CTA from 2048 on: 9600 tokens (bf16, 28/4/128) 41 and not
+        // 43 us, (f32, 14/2/64) 16 and not 19; below, one is as fast or faster
+        if (a.tokens >= 2048)
+            paged_append_kernel<T, decltype(kt), d.value, 2><<<(unsigned)(a.tokens + 1) / 2, block, 0, s>>>(a, turns);
+        else
+            paged_append_kernel<T, decltype(kt), d.value, 1><<<(unsigned)a.tokens, block, 0, s>>>(a, turns);
         return cudaGetLastError();
     });
 }
@@ -644,42 +665,29 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
         using T = decltype(t);
         using KT = decltype(kt);
         constexpr int D = d.value;
-        if constexpr (sizeof(KT) == 4) {
-            return cudaErrorInvalidValue;
-        } else {
-            using C = Dc<D>;
-            int dev = 0, sms = 0;
-            cudaError_t e = cudaGetDevice(&dev);
-            if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(decode_attention_kernel<T, KT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
-            // no more CTAs than units there can be, and no partials where an
-            // item has one unit at most
-            const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.page_shift) + kDcUnit - 1) / kDcUnit;
-            const int64_t tiles = ((int64_t)a.tokens * a.group + kDcRows - 1) / kDcRows + a.sequences;
-            const int64_t most = tiles * a.kv_heads * blocks;
-            const int ctas = (int)(most < kDcPerSm * sms ? most : kDcPerSm * sms);
-            const bool split = ctas > 1 && blocks > 1;
-            const size_t bytes = (size_t)ctas * C::kPartial * sizeof(float);
-            char *scratch = nullptr;  // a partial and a flag a share
-            if (e == cudaSuccess && split) e = stream_alloc((void **)&scratch, bytes + (size_t)ctas * 8, s);
-            if (e != cudaSuccess) return e;
-            const DcPlan plan{a.start, a.length, a.sequences, a.tokens, a.kv.max_pages << a.kv.page_shift, a.kv_heads, a.group, divisor(ctas)};
-            decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, plan, (float *)scratch, (unsigned long long *)(scratch + bytes),
-                                                                                            launch_number());
-            e = cudaGetLastError();
-            const cudaError_t f = stream_free(scratch, s);
-            return e != cudaSuccess ? e : f;
-        }
-    });
-}
-
-cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s)
-{
-    return by_type(a.type, a.kv_type, a.head_dim, [&](auto t, auto kt, auto d) {
-        const dim3 grid((unsigned)a.tokens, (unsigned)((a.heads + kRowWarps - 1) / kRowWarps));
-        attention_rows_kernel<decltype(t), decltype(kt), d.value><<<grid, kRowWarps * 32, 0, s>>>(a);
-        return cudaGetLastError();
+        using C = Dc<D>;
+        int dev = 0, sms = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(decode_attention_kernel<T, KT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+        // no more CTAs than units there can be, and no partials where an
+        // item has one unit at most
+        const int64_t blocks = (((int64_t)a.kv.max_pages << a.kv.page_shift) + kDcUnit - 1) / kDcUnit;
+        const int64_t tiles = ((int64_t)a.tokens * a.group + kDcRows - 1) / kDcRows + a.sequences;
+        const int64_t most = tiles * a.kv_heads * blocks;
+        const int ctas = (int)(most < kDcPerSm * sms ? most : kDcPerSm * sms);
+        const bool split = ctas > 1 && blocks > 1;
+        const size_t bytes = (size_t)ctas * C::kPartial * sizeof(float);
+        char *scratch = nullptr;  // a partial and a flag a share
+        if (e == cudaSuccess && split) e = stream_alloc((void **)&scratch, bytes + (size_t)ctas * 8, s);
+        if (e != cudaSuccess) return e;
+        const DcPlan plan{a.start, a.length, a.sequences, a.tokens, a.kv.max_pages << a.kv.page_shift, a.kv_heads, a.group, divisor(ctas)};
+        decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, plan, (float *)scratch, (unsigned long long *)(scratch + bytes),
+                                                                                        launch_number());
+        e = cudaGetLastError();
+        const cudaError_t f = stream_free(scratch, s);
+        return e != cudaSuccess ? e : f;
     });
 }
 

@@ -53,10 +53,9 @@ __device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t hi)
 template <typename T> struct Elem;
 template <> struct Elem<float> {
     static constexpr int kVec = 4;
-    static __device__ __forceinline__ void load(const float *p, float v[4])
+    static __device__ __forceinline__ void unpack(const uint4 &x, float v[4])
     {
-        const float4 x = *(const float4 *)p;
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        v[0] = __uint_as_float(x.x); v[1] = __uint_as_float(x.y); v[2] = __uint_as_float(x.z); v[3] = __uint_as_float(x.w);
     }
     static __device__ __forceinline__ void store(float *p, const float v[4]) { *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]); }
     static __device__ __forceinline__ float to_float(float x) { return x; }
@@ -64,9 +63,8 @@ template <> struct Elem<float> {
 };
 template <> struct Elem<__half> {
     static constexpr int kVec = 8;
-    static __device__ __forceinline__ void load(const __half *p, float v[8])
+    static __device__ __forceinline__ void unpack(const uint4 &x, float v[8])
     {
-        const uint4 x = *(const uint4 *)p;
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -87,9 +85,8 @@ template <> struct Elem<__half> {
 };
 template <> struct Elem<__nv_bfloat16> {
     static constexpr int kVec = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float v[8])
+    static __device__ __forceinline__ void unpack(const uint4 &x, float v[8])
     {
-        const uint4 x = *(const uint4 *)p;
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -368,7 +365,7 @@ __device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head,
             float acc = 0.f;
             for (int e = 0; e < D; e += V) {
                 float x[V];
-                Elem<KT>::load(k + e, x);
+                Elem<KT>::unpack(*(const uint4 *)(k + e), x);
 #pragma unroll
                 for (int t = 0; t < V; ++t) acc = fmaf(x[t], qs[e + t], acc);
             }

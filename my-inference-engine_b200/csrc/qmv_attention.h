@@ -51,9 +51,8 @@ struct AppendArgs {
 cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s);
 // Paged, 16-bit cache: for few rows a sequence over many keys.
 cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s);
-// f16 and bf16: prompts and chunks, on tcgen05.
+// Prompts and chunks, on tcgen05.
 cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s);
-cudaError_t launch_attention_rows(const AttnArgs &a, cudaStream_t s);
 
 unsigned long long launch_number();
 
