@@ -309,8 +309,6 @@ __global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__res
                                                        float *__restrict__ value_exp)
 {
     constexpr int E = D / 32;
-    // the attention launched behind may begin; it waits for these planes itself
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, rows = a.tokens * a.kv_heads;
     const size_t plane = (size_t)rows * D;
     for (int w = blockIdx.x * 8 + (int)(threadIdx.x >> 5); w < 2 * rows; w += gridDim.x * 8) {
@@ -748,10 +746,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
             float m = -INFINITY, l = 0.f;
             float2 next_units[4];
-            if constexpr (C::kK == 2) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");  // for split_kv_kernel
+            if constexpr (C::kK == 2)
                 if (end > it.b0) units_of(it.b0, next_units);
-            }
             for (int b = it.b0; b < end; ++b) {
                 if (!(ok = warp_wait(s_full + 8 * x, done & 1))) break;
                 fence_after();
@@ -972,7 +968,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys, piece = min(page_size, kTcKeys), pieces = kTcKeys / piece;
             const uint32_t q_bytes = (uint32_t)(sub * a.group) * D * 2;
             uint32_t issued = 0, q_phase[2] = {1, 1}, tail_phase = 0;
-            if constexpr (C::kK == 2) asm volatile("griddepcontrol.wait;" ::: "memory");  // for the planes
             phase = 1;  // of the empty barriers
             // page of the piece that this lane copies of block b
             auto page_of = [&](int b) {
@@ -1159,17 +1154,8 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
                       sub, divisor(sub * C::kSubs), divisor(ctas)};
     if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(kTcThreads);
-        cfg.dynamicSmemBytes = C::kSmem;
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = C::kK == 2 ? 1 : 0;  // behind split_kv_kernel only
-        e = cudaLaunchKernelEx(&cfg, tc_attention_kernel<T, KT, D>, a, maps, plan, partials, flags, launch_number());
+        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, flags, launch_number());
+        e = cudaGetLastError();
     }
     const cudaError_t f = stream_free(scratch, s);
     return e != cudaSuccess ? e : f;

@@ -168,6 +168,88 @@ def test_paged_long_decode(qmv, t, page):
     b.check(False)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+def test_paged_chunk_over_a_long_cache(qmv, t, heads, kv_heads, d):
+    """Few tiles over many keys: every tile is cut into dozens of shares."""
+    b = Batch(qmv, t, heads, kv_heads, d, [45, 1], [20011, 9000], page=64, layout="head")
+    b.run_paged()
+    b.check(False)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_many_sequences(qmv, t):
+    """More sequences than a CTA has threads, empty ones among them."""
+    new = [(i * 7) % 5 for i in range(900)]
+    kv = [n + (i * 13) % 40 if i % 11 else n for i, n in enumerate(new)]
+    for hint in (1, 1000):
+        b = Batch(qmv, t, 4, 2, 64, new, kv, page=16)
+        b.run_paged(max_query=hint)
+        torch.cuda.synchronize()
+        for s in list(range(0, 900, 37)) + [896, 897, 898, 899]:
+            a = sum(new[:s])
+            if new[s]:
+                k, v = b.kv_of(s, False)
+                want, tol = reference(b.q[a:a + new[s]].double().view(new[s], 4, 64), k, v, 0.125, t)
+                assert bool(((b.out[a:a + new[s]].double().view_as(want) - want).abs() <= tol).all()), (hint, s)
+        assert not torch.any(b.out == SENTINEL)
+    b = Batch(qmv, t, 4, 2, 64, new)
+    b.run_packed()
+    torch.cuda.synchronize()
+    for s in range(0, 900, 37):
+        a = sum(new[:s])
+        if new[s]:
+            k, v = b.kv_of(s, True)
+            want, tol = reference(b.q[a:a + new[s]].double().view(new[s], 4, 64), k, v, 0.125, t)
+            assert bool(((b.out[a:a + new[s]].double().view_as(want) - want).abs() <= tol).all()), s
+    assert not torch.any(b.out == SENTINEL)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 60])
+def test_output_rows_apart(qmv, t, new):
+    """Output rows on 16-byte boundaries only, with room between them that
+    stays as it was."""
+    b = Batch(qmv, t, 6, 2, 64, [new, 2], [new + 90, 77])
+    extra = 4 if t == "f32" else 8
+    wide = torch.full((b.tokens, 6 * 64 + extra), SENTINEL, dtype=b.dtype, device="cuda")
+    qmv.paged_attention(b.cache, b.batch(new), b.id, 6, b.q, b.ld, wide, 6 * 64 + extra)
+    torch.cuda.synchronize()
+    assert torch.all(wide[:, 6 * 64:] == SENTINEL)
+    b.out.copy_(wide[:, :6 * 64])
+    b.check(False)
+    qmv.packed_attention(b.id, 6, 2, 64, b.start, 2, b.tokens, b.q, b.ld, b.k, b.ld, b.v, b.ld, wide, 6 * 64 + extra)
+    torch.cuda.synchronize()
+    assert torch.all(wide[:, 6 * 64:] == SENTINEL)
+    b.out.copy_(wide[:, :6 * 64])
+    b.check(True)
+
+
+def test_offsets_past_32_bits(qmv):
+    """Pages 2^31 elements apart, positions and heads with room between them."""
+    hk, d, page, apart = 2, 64, 16, 2 ** 31 + 64
+    size = apart + page * (hk * (d + 8) + 24) + 64
+    keys, values = (torch.zeros(size, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = qmv.PagedCache(keys, values, 30, hk, d, page, 2, apart, hk * (d + 8) + 24, d + 8)
+    view = [x.as_strided((2, page, hk, d), (apart, hk * (d + 8) + 24, d + 8, 1)) for x in (keys, values)]
+    for new in (1, 20):
+        b = Batch(qmv, "bf16", 8, hk, d, [new], [32], page=page)
+        order = [1, 0]
+        b.table[0, :2] = torch.tensor(order, dtype=torch.int32)
+        qmv.paged_append(cache, b.batch(), b.id, 8, b.q, b.ld, b.k, b.ld, b.v, b.ld, 0.0)
+        at = torch.arange(32 - new, 32, device="cuda")
+        for x, rows in zip(view, (b.k, b.v)):
+            assert torch.equal(x[torch.tensor(order, device="cuda")[at // page], at % page], rows[:new].view(new, hk, d))
+            x.copy_(torch.randn(x.shape, device="cuda"))
+        for hint in (1, 1000):
+            b.out.fill_(SENTINEL)
+            qmv.paged_attention(cache, b.batch(hint), b.id, 8, b.q, b.ld, b.out, 8 * d)
+            torch.cuda.synchronize()
+            k, v = (x[order].reshape(32, hk, d).double() for x in view)
+            want, tol = reference(b.q[:new].double().view(new, 8, d), k, v, 0.125, "bf16")
+            assert bool(((b.out[:new].double().view_as(want) - want).abs() <= tol).all()), (new, hint)
+
+
 @pytest.mark.parametrize("hint", [1, 1000])
 def test_max_query_is_only_a_hint(qmv, hint):
     b = Batch(qmv, "bf16", 14, 2, 64, [70, 1, 20], [300, 77, 20])
