@@ -486,19 +486,28 @@ __device__ __noinline__ void tc_store(const AttnArgs &a, uint32_t o_t, float inv
 {
     const bool row = token_row >= 0, wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
     T *out = (T *)a.out + (int64_t)(row ? token_row : 0) * a.out_ld + (int64_t)head * D;
-    bool bad = false;
+    // 0 times a value is 0, or NaN where the value is not finite
+    float2 check[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-        float o[32];
+    for (int c = 0; c < D; c += 64) {
+        float o[64];
         tmem_ld32(o_t + c, o);
+        tmem_ld32(o_t + c + 32, o + 32);
         wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            o[i] = inv == 0.f ? 0.f : o[i] * inv;
-            bad |= !isfinite(o[i]);
+        for (int i = 0; i < 64; i += 2) {
+            float2 y = __fmul2_rn(make_float2(o[i], o[i + 1]), make_float2(inv, inv));
+            if (inv == 0.f) y = make_float2(0.f, 0.f);
+            check[i / 2 & 1] = __ffma2_rn(y, make_float2(0.f, 0.f), check[i / 2 & 1]);
+            o[i] = y.x;
+            o[i + 1] = y.y;
         }
-        if (row) store32<T>(out + c, o, wide);
+        if (row) {
+            store32<T>(out + c, o, wide);
+            store32<T>(out + c + 32, o + 32, wide);
+        }
     }
+    const bool bad = !((check[0].x + check[0].y) + (check[1].x + check[1].y) == 0.f);
     // a masked NaN or infinity met the sums: those rows again, without it
     for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
         const int who = __ffs(left) - 1;
