@@ -35,9 +35,10 @@ __device__ unsigned int g_attention_status;
 // first half of a head together with the pieces of the second half that they
 // turn with, for all query and key heads, and the value pieces; a thread's
 // first piece is on its way while the sequence, the page and the angles are found.
-// Bound by bytes, q, k and v being read once and written once, and by that
-// chain: 6789 tokens (bf16, 28/4/128; 125 MB) take 31 us, 4.1 TB/s; with four
-// or eight tokens a CTA registers cost more than the chain saves (45, 59 us at 9600).
+// Bound by bytes, q, k and v being read once and written once, and below some
+// thousand tokens by that chain: 6789 tokens (bf16, 28/4/128; 125 MB) take 26 us,
+// 4.8 TB/s, 20000 5.5 TB/s.  With four or eight tokens a CTA registers cost more
+// than the chain saves.
 
 constexpr int kAppendThreads = 512;  // at most: a thread a piece, as far as they go
 
@@ -70,30 +71,32 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(AppendArgs
         for (int i = 0; i < R; ++i) fetch(i, threadIdx.x);
     }
     if (row0 == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, max_keys_of(a.kv));
-    for (int i = warp; i < R; i += (int)(blockDim.x >> 5)) {  // a warp a token
-        const int row = row0 + i;
-        const int s = find_sequence(a.start, a.sequences, row);
-        const Seq sq = load_sequence(a.start, a.length, s, a.tokens, max_keys_of(a.kv));
-        const int at = row - sq.row0, pos = sq.keys - sq.n + at;
-        const bool live = at >= 0 && at < sq.n && pos >= 0;
-        const int page = live ? __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (pos >> a.kv.page_shift)) : -1;
-        const bool stored = page >= 0 && page < a.kv.page_count;
-        if ((threadIdx.x & 31) == 0) {
-            if (live && !stored) report(a.status, kStatusBadMetadata);
-            position[i] = live ? pos : -1;
-            slot[i] = stored ? (int64_t)page * a.kv.page + (int64_t)(pos & ((1 << a.kv.page_shift) - 1)) * a.kv.k_pos : -1;
-        }
+    static_assert(R <= 2, "a warp a token, and two warps at least");
+    int page = -1, pos = -1;  // of token `warp`
+    if (warp < R) {
+        const int row = row0 + warp;
+        Seq sq;
+        const int s = find_sequence(a.start, a.length, a.sequences, row, a.tokens, max_keys_of(a.kv), &sq);
+        const int at = row - sq.row0;
+        if (at >= 0 && at < sq.n) pos = sq.keys - sq.n + at;
+        if (pos >= 0) page = __ldg(a.kv.table + (int64_t)s * a.kv.max_pages + (pos >> a.kv.page_shift));
+        if ((threadIdx.x & 31) == 0) position[warp] = pos < 0 ? -1 : pos;
     }
     __syncthreads();
     const bool rope = a.rope_base > 0.f;
-    if (rope) {
+    if (rope) {  // while the pages' numbers are on their way
         for (int e = threadIdx.x; e < R * H; e += (int)blockDim.x) {
             // the signed fraction of a turn in [-1/2, 1/2): angle / pi = 2 * fraction
             const long long frac = (long long)((unsigned long long)position[e / H] * turns.f[e % H]);
             sincospif((float)frac * 1.0842021724855044e-19f, &sn[e / H][e % H], &cs[e / H][e % H]);  // 2^-63
         }
-        __syncthreads();
     }
+    if (warp < R && (threadIdx.x & 31) == 0) {
+        const bool stored = page >= 0 && page < a.kv.page_count;
+        if (pos >= 0 && !stored) report(a.status, kStatusBadMetadata);
+        slot[warp] = stored ? (int64_t)page * a.kv.page + (int64_t)(pos & ((1 << a.kv.page_shift) - 1)) * a.kv.k_pos : -1;
+    }
+    __syncthreads();
     for (int u = threadIdx.x; u < total; u += (int)blockDim.x) {
         const bool is_q = u < nq, is_v = u >= nq + nk;
         const int w = is_q ? u : is_v ? u - nq - nk : u - nq;
@@ -637,8 +640,8 @@ cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s)
         using T = decltype(t);
         const int pieces = ((a.q_out ? a.heads : 0) + 2 * a.kv_heads) * (d.value / 2 / Elem<T>::kVec), threads = (pieces + 31) / 32 * 32;
         const int block = threads < 64 ? 64 : threads < kAppendThreads ? threads : kAppendThreads;
-        // two tokens a CTA from 2048 on: 9600 tokens (bf16, 28/4/128) 41 and not
-        // 43 us, (f32, 14/2/64) 16 and not 19; below, one is as fast or faster
+        // two tokens a CTA from 2048 on: 9600 tokens (bf16, 28/4/128) take 0.95 of
+        // what they take with one, (f32, 14/2/64) 0.82; below, one is as fast or faster
         if (a.tokens >= 2048)
             paged_append_kernel<T, decltype(kt), d.value, 2><<<(unsigned)(a.tokens + 1) / 2, block, 0, s>>>(a, turns);
         else

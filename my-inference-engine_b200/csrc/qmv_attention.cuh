@@ -107,25 +107,6 @@ template <> struct Elem<__nv_bfloat16> {
 
 // ------------------------------------------------------------ metadata
 
-// The last s in [0, n) with start[s] <= row (0 when there is none), by the
-// 32 lanes of a warp together: 32 splits a step.
-__device__ __forceinline__ int find_sequence(const int *__restrict__ start, int n, int row)
-{
-    const int lane = threadIdx.x & 31;
-    int lo = 0, len = n;
-    while (len > 1) {
-        const int step = (len + 31) / 32;
-        const int s = lo + lane * step;
-        const bool below = s < lo + len && __ldg(start + s) <= row;
-        const unsigned m = __ballot_sync(kFull, below);
-        const int k = m ? 31 - __clz(m) : 0;
-        const int end = lo + len;
-        lo += k * step;
-        len = min(step, end - lo);
-    }
-    return lo;
-}
-
 struct Seq {
     int row0;  // first row
     int n;     // new tokens (0: left out)
@@ -147,6 +128,28 @@ __device__ __forceinline__ Seq load_sequence(const int *__restrict__ start, cons
 }
 
 __device__ __forceinline__ int max_keys_of(const KvView &kv) { return kv.table ? kv.max_pages << kv.page_shift : 0x7fffffff; }
+
+// The sequence that owns a row (the last s with start[s] <= row; 0 when there
+// is none) by the 32 lanes of a warp together: 32 splits a step, and the last
+// step's lanes bring the candidates' metadata along.
+__device__ __forceinline__ int find_sequence(const int *__restrict__ start, const int *__restrict__ length, int n, int row, int tokens, int max_keys,
+                                             Seq *found)
+{
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = n;
+    while (len > 32) {
+        const int step = (len + 31) / 32, s = lo + lane * step, end = lo + len;
+        const unsigned m = __ballot_sync(kFull, s < end && __ldg(start + s) <= row);
+        lo += (m ? 31 - __clz(m) : 0) * step;
+        len = min(step, end - lo);
+    }
+    Seq q{0x7fffffff, 0, 0};
+    if (lane < len) q = load_sequence(start, length, lo + lane, tokens, max_keys);
+    const unsigned m = __ballot_sync(kFull, lane < len && q.row0 <= row);
+    const int k = m ? 31 - __clz(m) : 0;
+    *found = Seq{__shfl_sync(kFull, q.row0, k), __shfl_sync(kFull, q.n, k), __shfl_sync(kFull, q.keys, k)};
+    return lo + k;
+}
 
 // Reports metadata out of range (one CTA of a launch calls it).
 __device__ __forceinline__ void check_metadata(unsigned int *status, const int *__restrict__ start, const int *__restrict__ length, int n, int tokens, int max_keys)

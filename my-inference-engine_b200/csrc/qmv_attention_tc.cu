@@ -56,10 +56,12 @@ template <typename T, typename KT, int D> struct Tc {
     static constexpr int kK = sizeof(KT) == 4 ? 2 : 1;  // parts of K and V
     using MT = typename std::conditional<kQ == 2, __half, T>::type;
     static constexpr int kSubs = kQ == 2 && D == 128 ? 1 : 2;  // tiles of a CTA: what tensor memory holds
-    // What a pair of tiles costs beside its keys, in keys, from measured cycles
-    // of a pair and of a block: 16 bits 4600 / 2560 (head_dim 64), 6700 / 2300
-    // (128); f32 over f16 keys 14500 / 2700, over f32 keys 16300 / 6800 (64).
-    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 256 : 384;
+    // What a pair of tiles costs beside its keys, in keys.  Tried on each kind:
+    // 16 bits, head_dim 128: a prompt of 8192 tokens takes 446, 409, 397, 388 us
+    // with 256, 384, 512, 640 (390 with 768); head_dim 64: ragged prompts 141,
+    // 125, 124, 125 us with 128, 256, 288, 384; f32: 640 over f16 keys, 320
+    // over f32 keys, both a few per cent better than half and one and a half of it.
+    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 288 : 640;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
