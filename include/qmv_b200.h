@@ -422,8 +422,9 @@ typedef struct QmvPagedCache {
 /* The new tokens of a step.  length[s] counts the cached positions of
  * sequence s with its new tokens, so token i of its n tokens has position
  * length[s] - n + i; position p lives in page
- * page_table[s * max_pages + p / page_size].  max_query: about how many new
- * tokens the longest sequence has (chooses the kernel; any value gives the same function). */
+ * page_table[s * max_pages + p / page_size]; max_pages * page_size is at most
+ * 2^30.  max_query: about how many new tokens the longest sequence has
+ * (chooses the kernel; any value gives the same function). */
 typedef struct QmvPagedBatch {
     const int *query_start; /* device, sequences + 1 */
     const int *length;      /* device, sequences */

@@ -3,7 +3,6 @@
 // message on failure; nothing is launched for a refused call.
 #include <cuda_runtime.h>
 
-#include <limits.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdint.h>
@@ -94,7 +93,8 @@ int check_batch(const QmvPagedBatch *b, qmv::KvView *kv)
     if (b->sequences == 0 || b->tokens == 0) return 1;
     if (b->query_start == nullptr || b->length == nullptr || b->page_table == nullptr)
         return fail("query_start, length or page_table is null");
-    if (b->max_pages <= 0 || b->max_pages > (INT_MAX >> kv->page_shift)) return fail("max_pages is out of range");
+    // (key counts are rounded up to blocks in 32 bits)
+    if (b->max_pages <= 0 || b->max_pages > ((1 << 30) >> kv->page_shift)) return fail("max_pages is out of range (2^30 positions at most)");
     if (b->max_query <= 0) return fail("max_query must be positive");
     kv->table = b->page_table;
     kv->max_pages = b->max_pages;

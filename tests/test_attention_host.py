@@ -111,3 +111,13 @@ def test_nothing_to_do_is_no_work(qmv):
     _append(qmv, batch=_batch(qmv, sequences=0))
     _packed(qmv, sequences=0)
     _packed(qmv, tokens=0)
+
+
+@pytest.mark.parametrize("page_size", [16, 256])
+@pytest.mark.parametrize("call", [_paged, _append])
+def test_positions_that_pass_32_bits_once_rounded_are_refused(qmv, call, page_size):
+    """A length of 2^31 - 16 keys is a length in 32 bits, but its blocks of 128
+    keys are not."""
+    for pages in (2 ** 30 // page_size + 1, (2 ** 31 - 16) // page_size):
+        with pytest.raises(qmv.QmvError, match="2\\^30 positions"):
+            call(qmv, cache=_cache(qmv, page_size=page_size), batch=_batch(qmv, max_pages=pages))
