@@ -101,6 +101,12 @@ int check_batch(const QmvPagedBatch *b, qmv::KvView *kv)
     return 1;
 }
 
+int check_metadata_device(const QmvPagedBatch *b, int dev)
+{
+    return check_device("query_start", b->query_start, dev) && check_device("length", b->length, dev) &&
+           check_device("page_table", b->page_table, dev);
+}
+
 int check_scale(float *scale, int head_dim)
 {
     if (!(*scale >= 0.f) || !isfinite(*scale)) return fail("scale must be finite and not negative");
@@ -141,7 +147,8 @@ QMV_EXPORT int qmv_paged_append(const QmvPagedCache *cache, const QmvPagedBatch 
     unsigned int *status = nullptr;
     if (!current_device(&dev, &status) || !check_device("keys", cache->keys, dev) ||
         !check_device("values", cache->values, dev) || !check_device("k", k, dev) || !check_device("v", v, dev) ||
-        (q_out != nullptr && !check_device("q_out", q_out, dev)) || !check_device("query_start", batch->query_start, dev))
+        (q_out != nullptr && (!check_device("q", q, dev) || !check_device("q_out", q_out, dev))) ||
+        (k_out != nullptr && !check_device("k_out", k_out, dev)) || !check_metadata_device(batch, dev))
         return 0;
     const qmv::AppendArgs a{type, cache->type, q, k, v, q_out, k_out, q_ld, k_ld, v_ld, q_out_ld, k_out_ld, kv,
                             batch->query_start, batch->length, batch->sequences, batch->tokens, heads, cache->kv_heads, d,
@@ -189,7 +196,8 @@ QMV_EXPORT int qmv_paged_attention(const QmvPagedCache *cache, const QmvPagedBat
     int dev = 0;
     unsigned int *status = nullptr;
     if (!current_device(&dev, &status) || !check_device("keys", cache->keys, dev) ||
-        !check_device("values", cache->values, dev) || !check_device("q", q, dev) || !check_device("out", out, dev) || !check_device("query_start", batch->query_start, dev))
+        !check_device("values", cache->values, dev) || !check_device("q", q, dev) || !check_device("out", out, dev) ||
+        !check_metadata_device(batch, dev))
         return 0;
     const qmv::AttnArgs a{type, cache->type, q, out, q_ld, out_ld, kv, batch->query_start, batch->length,
                           batch->sequences, batch->tokens, heads, cache->kv_heads, heads / cache->kv_heads, d,

@@ -437,6 +437,28 @@ def test_host_memory_is_refused(qmv):
         b.run_packed(out=host)
 
 
+@pytest.mark.parametrize("which", ["keys", "values", "query_start", "length", "page_table", "q", "k", "v", "q_out", "k_out"])
+def test_host_memory_is_refused_wherever_it_is_passed(qmv, which):
+    """Every pointer is looked at before the launch; nothing runs."""
+    b = Batch(qmv, "f16", 2, 1, 64, [3])
+    host = torch.zeros(4096, dtype=torch.float16)
+    cache, batch, at = b.cache, b.batch(), {n: host if n == which else x for n, x in dict(q=b.q, k=b.k, v=b.v, q_out=b.q, k_out=b.k).items()}
+    if hasattr(cache.c, which):
+        cache = qmv.PagedCache(*(host if which == n else x for n, x in (("keys", b.keys), ("values", b.values))), b.cache_id, 1, 64, b.page, b.count,
+                               b.page * 64, 64, 64)
+    elif hasattr(batch.c, which):
+        meta = {n: host if n == which else x for n, x in dict(query_start=b.start, length=b.length, page_table=b.table).items()}
+        batch = qmv.PagedBatch(**meta, sequences=1, tokens=b.tokens, max_pages=b.width)
+    with pytest.raises(qmv.QmvError, match=which + " is not device memory"):
+        qmv.paged_append(cache, batch, b.id, 2, at["q"], b.ld, at["k"], b.ld, at["v"], b.ld, 1e4, at["q_out"], b.ld, at["k_out"], b.ld)
+    if which in ("keys", "values", "query_start", "length", "page_table", "q"):
+        with pytest.raises(qmv.QmvError, match=which + " is not device memory"):
+            qmv.paged_attention(cache, batch, b.id, 2, at["q"], b.ld, b.out, 128)
+    if which in ("q", "k", "v", "query_start"):
+        with pytest.raises(qmv.QmvError, match=("start" if which == "query_start" else which) + " is not device memory"):
+            qmv.packed_attention(b.id, 2, 1, 64, host if which == "query_start" else b.start, 1, b.tokens, at["q"], b.ld, at["k"], b.ld, at["v"], b.ld, b.out, 128)
+
+
 # ----------------------------------------------------- metadata out of range
 
 @pytest.mark.parametrize("new", [1, 40])
