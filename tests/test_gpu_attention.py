@@ -314,6 +314,24 @@ def test_masked_places_may_hold_anything(qmv, t, what):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lengths", [[700, 1500], [130, 65, 1029]], ids=str)
+def test_not_a_number_from_a_token_on(qmv, t, lengths):
+    """What a NaN token leaves behind it: tokens that are NaN all over, behind
+    tokens that are not; and a value with one NaN element, which reaches that
+    column only."""
+    b = Batch(qmv, t, 14, 2, 64, lengths)
+    at = b.used - lengths[-1]
+    b.rows[at + 400:b.used] = math.nan
+    b.v[at - 40, 5] = math.nan
+    b.v[at + 3, 64 + 7] = math.nan
+    b.run_packed()
+    b.check(True)
+    assert torch.isnan(b.out[at + 400:b.used]).all()
+    assert torch.isfinite(b.out[at + 40:at + 400, :7 * 64]).all()
+    assert int(torch.isnan(b.out[at + 40:at + 400, 7 * 64:]).sum()) == 360 * 7
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_large_and_small_magnitudes(qmv, t):
     """Scores of hundreds (one weight is 1, the rest vanish) and tiny ones."""
     for f in (30.0, 1e-3):
