@@ -26,6 +26,13 @@
 // maximum passes it by 8 (a factor of 256; f32 sums and 16-bit floating
 // weights do not care), so O is rescaled a few times a row at most.
 //
+// Where no row of a tile sees the second half of its last block (half of all
+// tiles, and every short prompt), 16-bit activations leave it out of the
+// softmax and of PV: 61 prompts of 1..64 tokens (f16, 32/8/128) took 34.2 us and
+// take 29.6, 13 ragged prompts (bf16, 14/2/64) 126 and 120, and a prompt of 8192
+// tokens (bf16, 28/4/128) pays 387 to 393 for the larger code.  f32, for which
+// that code took 3 to 9 per cent everywhere, does not.
+//
 // Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
 // the launch in order are cut into one equal share per SM at multiples of 128
 // keys, and a tile that is cut is joined by the share that holds its beginning.
@@ -57,11 +64,12 @@ template <typename T, typename KT, int D> struct Tc {
     using MT = typename std::conditional<kQ == 2, __half, T>::type;
     static constexpr int kSubs = kQ == 2 && D == 128 ? 1 : 2;  // tiles of a CTA: what tensor memory holds
     // What a pair of tiles costs beside its keys, in keys.  Tried on each kind:
-    // 16 bits, head_dim 128: a prompt of 8192 tokens takes 446, 409, 397, 388 us
-    // with 256, 384, 512, 640 (390 with 768); head_dim 64: ragged prompts 141,
-    // 125, 124, 125 us with 128, 256, 288, 384; f32: 640 over f16 keys, 320
-    // over f32 keys, both a few per cent better than half and one and a half of it.
-    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 288 : 640;
+    // 16 bits, head_dim 128: a prompt of 8192 tokens takes 400, 399, 393, 393 us
+    // with 384, 448, 512, 640, 61 prompts of 1..64 tokens 25.4, 26.3, 26.4,
+    // 29.6 us; head_dim 64: 13 ragged prompts 119, 120, 119, 127 us with 256, 288,
+    // 320, 384; f32: 640 over f16 keys, 320 over f32 keys, both a few per cent
+    // better than half and one and a half of it.
+    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 320 : 512;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
@@ -462,11 +470,14 @@ struct TcIter {
 struct TcSub {
     int token0, tokens;  // within the sequence's new tokens
     int blocks;          // that any of its rows sees (at least 1 when it has tokens)
+    int keys;            // that any of its rows sees
+    // no row sees the second half of block b
+    __device__ __forceinline__ bool half(int b) const { return keys - b * kTcKeys <= kTcKeys / 2; }
     __device__ __forceinline__ TcSub(const TcPlan &p, const TcIter &it, int x)
     {
         token0 = it.i * p.wide.d + x * p.sub;
         tokens = max(0, min(p.sub, it.q.n - token0));
-        const int keys = it.q.keys - it.q.n + token0 + tokens;
+        keys = it.q.keys - it.q.n + token0 + tokens;
         blocks = tokens == 0 ? 0 : keys > 0 ? (keys + kTcKeys - 1) / kTcKeys : 1;
     }
 };
@@ -759,12 +770,14 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             float2 next_units[4];
             if constexpr (C::kK == 2)
                 if (end > it.b0) units_of(it.b0, next_units);
-            for (int b = it.b0; b < end; ++b) {
-                if (!(ok = warp_wait(s_full + 8 * x, done & 1))) break;
+            // block b, of its keys the first N
+            auto block = [&](const int b, auto cols) {
+                constexpr int N = decltype(cols)::value;
+                if (!warp_wait(s_full + 8 * x, done & 1)) return false;
                 fence_after();
-                float s[128];
+                float s[N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld32(s_t + 32 * i, s + 32 * i);
+                for (int i = 0; i < N / 32; ++i) tmem_ld32(s_t + 32 * i, s + 32 * i);
                 wait_ld();
                 fence_before();
                 __syncwarp();
@@ -777,16 +790,16 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     __syncwarp();
                     if (b + 1 < end) units_of(b + 1, next_units);
                 }
-                if (__any_sync(kFull, j0 + kTcKeys > lim)) {
+                if (__any_sync(kFull, j0 + N > lim)) {
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
+                    for (int i = 0; i < N; ++i)
                         if (j0 + i >= lim) s[i] = -INFINITY;
                 }
                 // the largest exponent: of the weight, or, where values have
                 // exponents of their own, of the weight that meets the value
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < 128; i += 2) {
+                for (int i = 0; i < N; i += 2) {
                     float y = s[i], z = s[i + 1];
                     if constexpr (C::kK == 2) {
                         const float4 u = lds4(unit + i);
@@ -800,7 +813,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
                 // P and O as the block before this one left them
                 if (done > 0) {
-                    if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
+                    if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
                     fence_after();
                 }
                 if (raise) {
@@ -824,7 +837,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 constexpr int W = C::kQ == 2 ? 16 : 32;  // columns of P a store
 #pragma unroll
-                for (int h = 0; h < 64 / W; ++h) {
+                for (int h = 0; h < N / 2 / W; ++h) {
                     uint32_t p[W], rest[C::kQ == 2 ? W : 1];
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
@@ -857,7 +870,16 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 __syncwarp();
                 if (lane == 0) bar_arrive(p_full + 8 * x);
                 ++done;
-            }
+                return true;
+            };
+            // the last block may go by halves; in a loop of its own, since a branch
+            // within the loop cost a long prompt another 1 to 4 per cent
+            const bool half = C::kQ == 1 && end > it.b0 && me.half(end - 1);
+            const int full = end - (half ? 1 : 0);
+#pragma unroll 1
+            for (int b = it.b0; ok && b < full; ++b) ok = block(b, std::integral_constant<int, 128>{});
+            if constexpr (C::kQ == 1)
+                if (ok && half) ok = block(end - 1, std::integral_constant<int, 64>{});
             if (!ok) break;
             if (me.tokens == 0) continue;
             const bool any = end > it.b0;  // this segment holds blocks of this tile
@@ -940,8 +962,13 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             uint32_t p_phase[2] = {0, 0};
             for (; ok && segment(&b1); it.next(plan)) {
                 int end[2];
+                bool half[2];
 #pragma unroll
-                for (int x = 0; x < kTcSubs; ++x) end[x] = min(b1, TcSub(plan, it, x).blocks);
+                for (int x = 0; x < kTcSubs; ++x) {
+                    const TcSub me(plan, it, x);
+                    end[x] = min(b1, me.blocks);
+                    half[x] = me.half(end[x] - 1);
+                }
                 for (int b = it.b0; b < b1; ++b) {
                     if (!(ok = warp_wait(v_full + 8 * slot, phase))) break;
                     const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kKTile);
@@ -954,6 +981,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         constexpr uint32_t part = C::kTile >> 4, rows64 = 64 * 128 >> 4;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
+                            if (C::kQ == 1 && h == 1 && b + 1 == end[x] && half[x]) break;
                             const uint32_t pt = tm + C::p_col(x) + 32u * h;
                             mma_ts64(tm + C::o_col(x), pt, vb + h * rows64, kId, h != 0 || b != it.b0);
                             if constexpr (C::kQ == 2) mma_ts64(tm + C::o_col(x), pt + 64u, vb + h * rows64, kId, 1u);

@@ -477,6 +477,22 @@ def test_host_memory_is_refused_wherever_it_is_passed(qmv, which):
             qmv.packed_attention(b.id, 2, 1, 64, host if which == "query_start" else b.start, 1, b.tokens, at["q"], b.ld, at["k"], b.ld, at["v"], b.ld, b.out, 128)
 
 
+# --------------------------------------------- lengths about a half block
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (32, 8, 128), (2, 2, 128), (64, 1, 64)])
+@pytest.mark.parametrize("paged", [False, True])
+def test_lengths_about_half_a_block(qmv, t, heads, kv_heads, d, paged):
+    """Tiles whose last block of 128 keys ends about its half."""
+    if paged:
+        b = Batch(qmv, t, heads, kv_heads, d, [40, 33, 34, 50, 17, 64, 40], [63, 64, 65, 191, 192, 193, 320], page=32, layout="head")
+        b.run_paged(max_query=64)
+    else:
+        b = Batch(qmv, t, heads, kv_heads, d, [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 257], pad=5)
+        b.run_packed()
+    b.check(not paged)
+
+
 # ----------------------------------------------------- metadata out of range
 
 @pytest.mark.parametrize("new", [1, 40])
