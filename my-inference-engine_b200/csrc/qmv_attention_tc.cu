@@ -31,7 +31,7 @@
 // softmax and of PV: 61 prompts of 1..64 tokens (f16, 32/8/128) took 34.2 us and
 // take 29.6, 13 ragged prompts (bf16, 14/2/64) 126 and 120, and a prompt of 8192
 // tokens (bf16, 28/4/128) pays 387 to 393 for the larger code.  f32, for which
-// that code took 3 to 9 per cent everywhere, does not.
+// that code took 2 to 3 per cent everywhere, does not.
 //
 // Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
 // the launch in order are cut into one equal share per SM at multiples of 128
@@ -263,7 +263,14 @@ __device__ __forceinline__ float4 lds4(const float2 *p)
     return v;
 }
 
-// 2^n for a whole number |n| <= 60 held in a float.
+__device__ __forceinline__ float2 lds2(const float *p)
+{
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    return v;
+}
+
+// 2^n for a whole number |n| <= 80 held in a float.
 __device__ __forceinline__ float power(float n) { return __uint_as_float(__float_as_uint(n + 12583039.f) << 23); }
 
 // A warp's 32 f32 rows of Q (rows 32 * quarter .. of the tile) as two f16 rows
@@ -314,6 +321,7 @@ template <int D> __device__ __forceinline__ float split_rows(const AttnArgs &a, 
 // f32 keys and values as two f16 planes [part][token][kv_heads * D] and their
 // units (see TcMaps): the largest |x| of a row in [2^14, 2^15), so that values
 // down to 2^-17 of it keep 22 bits.  A warp a row.
+constexpr int kNear = 14;
 template <int D>
 __global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__restrict__ kp, __half *__restrict__ vp, float *__restrict__ key_unit,
                                                        float *__restrict__ value_exp)
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__res
         }
         if (lane == 0) {
             if (value)
-                value_exp[(size_t)h * a.tokens + token] = (float)-e;
+                value_exp[(size_t)h * a.tokens + token] = (float)(kNear - e);
             else
                 key_unit[(size_t)h * a.tokens + token] = __uint_as_float((uint32_t)(127 - e) << 23);
         }
@@ -485,7 +493,8 @@ struct TcSub {
 struct TcMaps {
     CUtensorMap q, k, v;
     // f32 keys and values, rows [kv_head][token]: what a key's dot is times
-    // (2^-e), and the exponent of its value's row
+    // (2^-e), and the exponent of its value's row, kNear - e, so that it is
+    // small for values about 1
     const float *key_unit, *value_exp;
 };
 
@@ -677,6 +686,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     // of f32 keys and values: each key's unit and its value's exponent, a copy a
     // warp, this block's and the next one's
     __shared__ __align__(16) float2 key_of[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];
+    __shared__ __align__(16) float key_scale[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];  // 2^-exponent
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kQTile, v_s = k_s + NS * C::kKTile;
@@ -784,9 +794,13 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
                 const int j0 = b * kTcKeys;
                 const float2 *unit = key_of[C::kK == 2 ? warp : 0][b & 1];
+                const float *key_l = key_scale[C::kK == 2 ? warp : 0][b & 1];
                 if constexpr (C::kK == 2) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) key_of[warp][b & 1][32 * i + lane] = next_units[i];
+                    for (int i = 0; i < 4; ++i) {
+                        key_of[warp][b & 1][32 * i + lane] = next_units[i];
+                        key_scale[warp][b & 1][32 * i + lane] = power(-next_units[i].y);
+                    }
                     __syncwarp();
                     if (b + 1 < end) units_of(b + 1, next_units);
                 }
@@ -796,18 +810,20 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         if (j0 + i >= lim) s[i] = -INFINITY;
                 }
                 // the largest exponent: of the weight, or, where values have
-                // exponents of their own, of the weight that meets the value
+                // exponents of their own, of the weight that meets the value (s
+                // is then that exponent: the second pass needs the keys' 2^-exponent
+                // only, for the sum; 3 f32 prompts of 400..2000 tokens 53.1 -> 48.2 us)
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < N; i += 2) {
-                    float y = s[i], z = s[i + 1];
                     if constexpr (C::kK == 2) {
                         const float4 u = lds4(unit + i);
-                        y = fmaf(y * u.x, f, u.y);
-                        z = fmaf(z * u.z, f, u.w);
+                        const float2 e = __ffma2_rn(__fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(u.x, u.z)), make_float2(f, f), make_float2(u.y, u.w));
+                        s[i] = e.x;
+                        s[i + 1] = e.y;
                     }
-                    top[i & 3] = fmaxf(top[i & 3], y);
-                    top[(i + 1) & 3] = fmaxf(top[(i + 1) & 3], z);
+                    top[i & 3] = fmaxf(top[i & 3], s[i]);
+                    top[(i + 1) & 3] = fmaxf(top[(i + 1) & 3], s[i + 1]);
                 }
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (C::kK == 2 ? 1.f : f);
                 const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
@@ -842,16 +858,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
                         const int j = 2 * (W * h + i);
-                        float2 at = make_float2(s[j], s[j + 1]), of = make_float2(0.f, 0.f);
-                        if constexpr (C::kK == 2) {
-                            const float4 u = lds4(unit + j);
-                            at = __fmul2_rn(at, make_float2(u.x, u.z));
-                            of = make_float2(u.y, u.w);
-                        }
-                        const float2 e = __ffma2_rn(at, f2, C::kK == 2 ? __fadd2_rn(n2, of) : n2);
+                        const float2 at = make_float2(s[j], s[j + 1]), e = C::kK == 2 ? __fadd2_rn(at, n2) : __ffma2_rn(at, f2, n2);
                         const float2 w = make_float2(ex2(e.x), ex2(e.y));
                         if constexpr (C::kK == 2)
-                            sum[i & 1] = __ffma2_rn(w, make_float2(power(-of.x), power(-of.y)), sum[i & 1]);
+                            sum[i & 1] = __ffma2_rn(w, lds2(key_l + j), sum[i & 1]);
                         else
                             sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                         p[i] = pack2<MT>(w.x, w.y);
@@ -882,6 +892,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 if (ok && half) ok = block(end - 1, std::integral_constant<int, 64>{});
             if (!ok) break;
             if (me.tokens == 0) continue;
+            if constexpr (C::kK == 2) l *= (float)(1 << kNear);  // as the values are 2^kNear times theirs
             const bool any = end > it.b0;  // this segment holds blocks of this tile
             if (any) {
                 if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
