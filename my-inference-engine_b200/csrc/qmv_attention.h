@@ -1,5 +1,6 @@
 // Internal interface between the attention entry points
-// (qmv_attention_capi.cpp) and their sm_100a kernels (qmv_attention.cu).
+// (qmv_attention_capi.cpp) and their sm_100a kernels (qmv_attention.cu and
+// qmv_attention_tc.cu).
 #pragma once
 
 #include <cuda_runtime.h>

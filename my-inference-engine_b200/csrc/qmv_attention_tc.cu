@@ -41,6 +41,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "qmv_attention.cuh"
 #include "qmv_internal.h"
 
@@ -1119,16 +1121,16 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 
 cudaError_t encode_tiled(EncodeTiled *fn)
 {
-    static EncodeTiled have = nullptr;  // the same for every thread that looks it up
-    if (have == nullptr) {
+    static std::atomic<EncodeTiled> have{nullptr};  // the same for every thread that looks it up
+    if (have.load(std::memory_order_relaxed) == nullptr) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult found;
         const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
         if (e != cudaSuccess) return e;
         if (found != cudaDriverEntryPointSuccess || p == nullptr) return cudaErrorNotSupported;
-        have = (EncodeTiled)p;
+        have.store((EncodeTiled)p, std::memory_order_relaxed);
     }
-    *fn = have;
+    *fn = have.load(std::memory_order_relaxed);
     return cudaSuccess;
 }
 

@@ -1,6 +1,7 @@
 """Append to a paged cache and causal attention of ragged batches on the GPU,
 against the formulas in 64 bits (attention_cases.py derives the tolerances)."""
 import math
+import threading
 
 import pytest
 
@@ -436,6 +437,30 @@ def test_two_streams_at_once(qmv):
             c.run_paged(stream=s.cuda_stream)
     for b in bs + cs:
         b.check(False)
+
+
+def test_two_threads_at_once(qmv):
+    """Calls from two host threads, each on its own stream."""
+    packed, paged = Batch(qmv, "bf16", 14, 2, 64, [300, 700]), Batch(qmv, "f16", 32, 8, 128, [1] * 9, [900] * 9, seed=1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(b, run, stream):
+        try:
+            for _ in range(50):
+                run(stream=stream.cuda_stream)
+        except Exception as e:  # noqa: BLE001 - handed to the test's thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((packed, packed.run_packed, streams[0]), (paged, paged.run_paged, streams[1]))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    packed.check(True)
+    paged.check(False)
 
 
 def test_same_inputs_same_bits(qmv):
