@@ -11,7 +11,7 @@
 //               swizzle), 128 x 128 f32 in tensor memory;
 //   softmax     one thread a row: the row of S in registers, running reference
 //               m and sum l; P = 2^(S f - m) rounded to the values' 16-bit type
-//               and stored to tensor memory;
+//               (f32: to two or three parts of it) and stored to tensor memory;
 //   O += P V    tcgen05.mma, P from tensor memory, V from shared memory.
 // S is needed only until it is in registers, so the next scores are multiplied
 // while the exponentials run: head_dim 128 has room for one S that the two
@@ -56,14 +56,23 @@ constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; t
 constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
 constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
 
-// T, KT: types of the activations and of the keys and values.  f32 operands
-// meet the tensor cores as pairs of f16, x = hi + lo to 22 bits of the largest
-// value of their row (scaled by a power of two), in the products hi hi, lo hi
-// and hi lo.
+// T, KT: types of the activations and of the keys and values.
+//
+// f32 queries and keys meet the tensor cores as pairs of f16, x = hi + lo,
+// each row scaled by a power of two that its largest |x| chooses (an element
+// is held to 22 bits, or to 2^-39 of that largest one), in the products hi hi,
+// lo hi and hi lo.  The weights over f16 pages are pairs of f16 too.  f32
+// values meet their weights as three bf16 each (24 bits), in the six products
+// above 2^-24: bf16 has f32's exponents, so that values of any size, side by
+// side in a row or a column, and weights of any size keep their bits.  (As f16
+// pairs scaled by rows, a value of 1e7 cost the other columns 11 of 22 bits.)
 template <typename T, typename KT, int D> struct Tc {
-    static constexpr int kQ = sizeof(T) == 4 ? 2 : 1;   // parts of Q and P
-    static constexpr int kK = sizeof(KT) == 4 ? 2 : 1;  // parts of K and V
-    using MT = typename std::conditional<kQ == 2, __half, T>::type;
+    static constexpr int kQ = sizeof(T) == 4 ? 2 : 1;   // parts of Q
+    static constexpr int kK = sizeof(KT) == 4 ? 2 : 1;  // parts of K
+    static constexpr int kV = sizeof(KT) == 4 ? 3 : 1;  // parts of V
+    static constexpr int kP = kV == 3 ? 3 : kQ;         // parts of P
+    using MT = typename std::conditional<kQ == 2, __half, T>::type;             // of Q K^T
+    using VT = typename std::conditional<kV == 3, __nv_bfloat16, MT>::type;     // of P V
     static constexpr int kSubs = kQ == 2 && D == 128 ? 1 : 2;  // tiles of a CTA: what tensor memory holds
     // What a pair of tiles costs beside its keys, in keys.  Tried on each kind:
     // 16 bits, head_dim 128: a prompt of 8192 tokens takes 400, 399, 393, 393 us
@@ -75,15 +84,21 @@ template <typename T, typename KT, int D> struct Tc {
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
-    // blocks of K, and of V, in flight
+    // blocks of K in flight, and pieces of V: a block, or 64 keys of one part
     static constexpr int kSlots = kKTile == 65536 ? 1 : kKTile == 32768 ? 2 : 4;
-    static constexpr uint32_t kSmem = kSubs * kQTile + 2 * kSlots * kKTile + 1024;
+    static constexpr int kVSlots = kV == 1 ? kSlots : D == 64 ? 10 : 5;
+    static constexpr uint32_t kVTile = kV == 1 ? kTile : kTile / 2;
+    static constexpr uint32_t kSmem = kSubs * kQTile + kSlots * kKTile + kVSlots * kVTile + 1024;
+    // P of a block at once, or of its halves of 64 keys one after another (three
+    // parts of 128 keys are more than tensor memory holds)
+    static constexpr int kHalves = kP == 3 ? 2 : 1;
+    static constexpr uint32_t kPCols = kP == 3 ? 96u : 64u * kP;
     // tensor memory columns
     static constexpr int kScores = D == 64 && kQ == 1 ? 2 : 1;  // S buffers
     static __host__ __device__ constexpr uint32_t s_col(int x) { return kScores == 2 ? 128u * x : 0u; }
-    static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + 64u * kQ * x; }
-    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + 64u * kQ * kSubs + (uint32_t)D * x; }
-    static_assert(128 * kScores + (64 * kQ + D) * kSubs <= 512, "tensor memory");
+    static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + kPCols * x; }
+    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + kPCols * kSubs + (uint32_t)D * x; }
+    static_assert(128 * kScores + ((int)kPCols + D) * kSubs <= 512, "tensor memory");
     static constexpr int kPartial = kSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
 };
 
@@ -236,14 +251,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r)
 // Shared-memory matrix descriptors, 128-byte swizzle (atoms of 8 rows x 128
 // bytes, 1024 bytes apart along the rows).  K-major (Q, K): the contiguous
 // 64 elements run along the reduction.  MN-major (V): they run along the
-// output columns, the second 64 columns one half tile (16 KB) further.
+// output columns, the second 64 columns `apart` bytes further.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr)
 {
     return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)1u << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr)
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t apart)
 {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(apart >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // Instruction descriptor: f32 accumulator, M = 128, N = n, A and B of the
@@ -254,9 +269,8 @@ template <typename KT> __host__ __device__ constexpr uint32_t idesc(int n, bool 
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-// Two keys' units and exponents; volatile, so that 128 of them are not held in
-// registers between the passes over a row.
-__device__ __forceinline__ float4 lds4(const float2 *p)
+// Four keys' units; volatile, so that 128 of them are not held in registers.
+__device__ __forceinline__ float4 lds4(const float *p)
 {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -265,15 +279,20 @@ __device__ __forceinline__ float4 lds4(const float2 *p)
     return v;
 }
 
-__device__ __forceinline__ float2 lds2(const float *p)
+// Two weights as three bf16 each, by cutting: 8 + 8 + 8 bits, exactly (of
+// weights above 2^-100).
+__device__ __forceinline__ void cut3(float a, float b, uint32_t part[3])
 {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"((uint32_t)__cvta_generic_to_shared(p)));
-    return v;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        part[k] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+        if (k == 2) break;
+        const float2 rest = __fadd2_rn(make_float2(a, b), make_float2(-__uint_as_float(__float_as_uint(a) & 0xffff0000u),
+                                                                     -__uint_as_float(__float_as_uint(b) & 0xffff0000u)));
+        a = rest.x;
+        b = rest.y;
+    }
 }
-
-// 2^n for a whole number |n| <= 80 held in a float.
-__device__ __forceinline__ float power(float n) { return __uint_as_float(__float_as_uint(n + 12583039.f) << 23); }
 
 // A warp's 32 f32 rows of Q (rows 32 * quarter .. of the tile) as two f16 rows
 // each in swizzled shared memory, the second in the tile behind: x = (hi + lo)
@@ -322,13 +341,11 @@ template <int D> __device__ __forceinline__ float split_rows(const AttnArgs &a, 
     return unit;
 }
 
-// f32 keys and values as two f16 planes [part][token][kv_heads * D] and their
-// units (see TcMaps): the largest |x| of a row in [2^14, 2^15), so that values
-// down to 2^-17 of it keep 22 bits.  A warp a row.
-constexpr int kNear = 14;
+// f32 keys as two f16 planes [part][token][kv_heads * D] and their units (see
+// TcMaps): the largest |x| of a row in [2^14, 2^15).  f32 values as three bf16
+// planes, each the rounding of what the ones before leave.  A warp a row.
 template <int D>
-__global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__restrict__ kp, __half *__restrict__ vp, float *__restrict__ key_unit,
-                                                       float *__restrict__ value_exp)
+__global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__restrict__ kp, __nv_bfloat16 *__restrict__ vp, float *__restrict__ key_unit)
 {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31, rows = a.tokens * a.kv_heads;
@@ -343,24 +360,34 @@ __global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__res
             v[i] = x[E * lane + i];
             big = fmaxf(big, fabsf(v[i]));
         }
+        if (value) {
+            __nv_bfloat16 *to = vp + (size_t)at * D + E * lane;
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                float2 rest = make_float2(v[i], v[i + 1]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    const uint32_t w2 = pack2<__nv_bfloat16>(rest.x, rest.y);
+                    *(uint32_t *)(to + k * plane + i) = w2;
+                    rest.x -= __uint_as_float(w2 << 16);
+                    rest.y -= __uint_as_float(w2 & 0xffff0000u);
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, d));
         const int top = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-        const int e = value ? min(max(14 - top, -60), 60) : min(max(14 - top, -100), 100);
+        const int e = min(max(14 - top, -100), 100);
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        __half *to = (value ? vp : kp) + (size_t)at * D + E * lane;
+        __half *to = kp + (size_t)at * D + E * lane;
 #pragma unroll
         for (int i = 0; i < E; i += 2) {
             const uint32_t hi = pack2<__half>(v[i] * up, v[i + 1] * up);
             *(uint32_t *)(to + i) = hi;
             *(uint32_t *)(to + plane + i) = pack2_rest(v[i] * up, v[i + 1] * up, hi);
         }
-        if (lane == 0) {
-            if (value)
-                value_exp[(size_t)h * a.tokens + token] = (float)(kNear - e);
-            else
-                key_unit[(size_t)h * a.tokens + token] = __uint_as_float((uint32_t)(127 - e) << 23);
-        }
+        if (lane == 0) key_unit[(size_t)h * a.tokens + token] = __uint_as_float((uint32_t)(127 - e) << 23);
     }
 }
 
@@ -496,10 +523,8 @@ struct TcSub {
 
 struct TcMaps {
     CUtensorMap q, k, v;
-    // f32 keys and values, rows [kv_head][token]: what a key's dot is times
-    // (2^-e), and the exponent of its value's row, kNear - e, so that it is
-    // small for values about 1
-    const float *key_unit, *value_exp;
+    // f32 keys, rows [kv_head][token]: what a key's dot is times (2^-e)
+    const float *key_unit;
 };
 
 
@@ -680,22 +705,21 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 {
     using C = Tc<T, KT, D>;
     using MT = typename C::MT;
-    constexpr int NS = C::kSlots, kTcSubs = C::kSubs;
-    constexpr float kLift = std::is_same<MT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
+    using VT = typename C::VT;
+    constexpr int NS = C::kSlots, NV = C::kVSlots, kTcSubs = C::kSubs;
+    constexpr float kLift = std::is_same<VT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[4 * NS + 6 * kTcSubs + 3];
+    __shared__ __align__(8) unsigned long long bars[2 * NS + 2 * NV + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ Start<TcIter> begin;
     __shared__ float row_q[8][D];
-    // of f32 keys and values: each key's unit and its value's exponent, a copy a
-    // warp, this block's and the next one's
-    __shared__ __align__(16) float2 key_of[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];
-    __shared__ __align__(16) float key_scale[C::kK == 2 ? 8 : 1][2][C::kK == 2 ? kTcKeys : 1];  // 2^-exponent
+    // of f32 keys: each key's unit, a copy a warp, this block's and the next one's
+    __shared__ __align__(16) float key_of[C::kK == 2 ? 4 * kTcSubs : 1][2][C::kK == 2 ? kTcKeys : 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_s = smem0, k_s = smem0 + kTcSubs * C::kQTile, v_s = k_s + NS * C::kKTile;
     const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t k_full = bar0, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NS, q_full = v_empty + 8 * NS, q_empty = q_full + 8 * kTcSubs,
+    const uint32_t k_full = bar0, k_empty = k_full + 8 * NS, v_full = k_empty + 8 * NS, v_empty = v_full + 8 * NV, q_full = v_empty + 8 * NV, q_empty = q_full + 8 * kTcSubs,
                    s_full = q_empty + 8 * kTcSubs, s_free = s_full + 8 * kTcSubs, p_full = s_free + 8 * kTcSubs,
                    pv_done = p_full + 8 * kTcSubs, tail_bar = pv_done + 8 * kTcSubs, drain_bar = tail_bar + 8;
 
@@ -708,6 +732,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         for (int i = 0; i < NS; ++i) {
             bar_init(k_full + 8 * i, 1);
             bar_init(k_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < NV; ++i) {
             bar_init(v_full + 8 * i, 1);
             bar_init(v_empty + 8 * i, 1);
         }
@@ -751,14 +777,14 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
         const uint32_t s_t = lanes + C::s_col(x), p_t = lanes + C::p_col(x), o_t = lanes + C::o_col(x);
-        uint32_t done = 0;  // blocks of this tile slot handed over so far
-        // f32 keys: unit and exponent of this lane's keys (lane, lane + 32, ...) of block b
-        auto units_of = [&](int b, float2 u[4]) {
+        uint32_t done = 0;  // blocks (or their halves) of this tile slot handed over so far
+        // f32 keys: units of this lane's keys (4 lane ..) of block b
+        auto units_of = [&](int b, float u[4]) {
             const int64_t at = (int64_t)it.h * a.tokens + it.q.row0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int j = b * kTcKeys + 32 * i + lane;
-                u[i] = j < it.q.keys ? make_float2(__ldg(maps.key_unit + at + j), __ldg(maps.value_exp + at + j)) : make_float2(1.f, 0.f);
+                const int j = b * kTcKeys + 4 * lane + i;
+                u[i] = j < it.q.keys ? __ldg(maps.key_unit + at + j) : 1.f;
             }
         };
         for (; x < kTcSubs && ok && segment(&b1); it.next(plan)) {
@@ -781,13 +807,13 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
             }
             float m = -INFINITY, l = 0.f;
-            float2 next_units[4];
+            float next_units[4];
             if constexpr (C::kK == 2)
                 if (end > it.b0) units_of(it.b0, next_units);
             // block b, of its keys the first N
             auto block = [&](const int b, auto cols) {
                 constexpr int N = decltype(cols)::value;
-                if (!warp_wait(s_full + 8 * x, done & 1)) return false;
+                if (!warp_wait(s_full + 8 * x, done / C::kHalves & 1)) return false;
                 fence_after();
                 float s[N];
 #pragma unroll
@@ -797,39 +823,30 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 __syncwarp();
                 if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
                 const int j0 = b * kTcKeys;
-                const float2 *unit = key_of[C::kK == 2 ? warp : 0][b & 1];
-                const float *key_l = key_scale[C::kK == 2 ? warp : 0][b & 1];
                 if constexpr (C::kK == 2) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        key_of[warp][b & 1][32 * i + lane] = next_units[i];
-                        key_scale[warp][b & 1][32 * i + lane] = power(-next_units[i].y);
-                    }
+                    float *unit = key_of[warp][b & 1];
+                    *(float4 *)(unit + 4 * lane) = make_float4(next_units[0], next_units[1], next_units[2], next_units[3]);
                     __syncwarp();
                     if (b + 1 < end) units_of(b + 1, next_units);
+#pragma unroll
+                    for (int i = 0; i < N; i += 4) {
+                        const float4 u = lds4(unit + i);
+                        const float2 lo = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(u.x, u.y)), hi = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(u.z, u.w));
+                        s[i] = lo.x;
+                        s[i + 1] = lo.y;
+                        s[i + 2] = hi.x;
+                        s[i + 3] = hi.y;
+                    }
                 }
                 if (__any_sync(kFull, j0 + N > lim)) {
 #pragma unroll
                     for (int i = 0; i < N; ++i)
                         if (j0 + i >= lim) s[i] = -INFINITY;
                 }
-                // the largest exponent: of the weight, or, where values have
-                // exponents of their own, of the weight that meets the value (s
-                // is then that exponent: the second pass needs the keys' 2^-exponent
-                // only, for the sum; 3 f32 prompts of 400..2000 tokens 53.1 -> 48.2 us)
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < N; i += 2) {
-                    if constexpr (C::kK == 2) {
-                        const float4 u = lds4(unit + i);
-                        const float2 e = __ffma2_rn(__fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(u.x, u.z)), make_float2(f, f), make_float2(u.y, u.w));
-                        s[i] = e.x;
-                        s[i + 1] = e.y;
-                    }
-                    top[i & 3] = fmaxf(top[i & 3], s[i]);
-                    top[(i + 1) & 3] = fmaxf(top[(i + 1) & 3], s[i + 1]);
-                }
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * (C::kK == 2 ? 1.f : f);
+                for (int i = 0; i < N; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
                 const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
                 // P and O as the block before this one left them
                 if (done > 0) {
@@ -855,35 +872,46 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 const float base = m == -INFINITY ? 0.f : m - kLift;
                 const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                constexpr int W = C::kQ == 2 ? 16 : 32;  // columns of P a store
+                constexpr int W = C::kP > 1 ? 16 : 32;  // columns of P a store
 #pragma unroll
-                for (int h = 0; h < N / 2 / W; ++h) {
-                    uint32_t p[W], rest[C::kQ == 2 ? W : 1];
+                for (int g = 0; g < C::kHalves; ++g) {
+                    if (g > 0) {  // the half before has left tensor memory
+                        if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
+                        fence_after();
+                    }
 #pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        const int j = 2 * (W * h + i);
-                        const float2 at = make_float2(s[j], s[j + 1]), e = C::kK == 2 ? __fadd2_rn(at, n2) : __ffma2_rn(at, f2, n2);
-                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
-                        if constexpr (C::kK == 2)
-                            sum[i & 1] = __ffma2_rn(w, lds2(key_l + j), sum[i & 1]);
-                        else
+                    for (int h = 0; h < N / 2 / W / C::kHalves; ++h) {
+                        uint32_t p[C::kP][W];
+#pragma unroll
+                        for (int i = 0; i < W; ++i) {
+                            const int j = N / C::kHalves * g + 2 * (W * h + i);
+                            const float2 e = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, n2), w = make_float2(ex2(e.x), ex2(e.y));
                             sum[i & 1] = __fadd2_rn(sum[i & 1], w);
-                        p[i] = pack2<MT>(w.x, w.y);
-                        if constexpr (C::kQ == 2) rest[i] = pack2_rest(w.x, w.y, p[i]);
+                            if constexpr (C::kP == 3) {
+                                uint32_t part[3];
+                                cut3(w.x, w.y, part);
+#pragma unroll
+                                for (int k = 0; k < 3; ++k) p[k][i] = part[k];
+                            } else {
+                                p[0][i] = pack2<VT>(w.x, w.y);
+                                if constexpr (C::kP == 2) p[1][i] = pack2_rest(w.x, w.y, p[0][i]);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < C::kP; ++k) {
+                            if constexpr (W == 16)
+                                tmem_st16(p_t + C::kPCols / C::kP * k + W * h, p[k]);
+                            else
+                                tmem_st32(p_t + W * h, p[k]);
+                        }
                     }
-                    if constexpr (C::kQ == 2) {
-                        tmem_st16(p_t + W * h, p);
-                        tmem_st16(p_t + 64 + W * h, rest);
-                    } else {
-                        tmem_st32(p_t + W * h, p);
-                    }
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(p_full + 8 * x);
+                    ++done;
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(p_full + 8 * x);
-                ++done;
                 return true;
             };
             // the last block may go by halves; in a loop of its own, since a branch
@@ -896,7 +924,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 if (ok && half) ok = block(end - 1, std::integral_constant<int, 64>{});
             if (!ok) break;
             if (me.tokens == 0) continue;
-            if constexpr (C::kK == 2) l *= (float)(1 << kNear);  // as the values are 2^kNear times theirs
             const bool any = end > it.b0;  // this segment holds blocks of this tile
             if (any) {
                 if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
@@ -912,8 +939,9 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         uint32_t slot = 0, phase = 0;  // of this warp's next block of K or V
+        const uint32_t slots = warp == kTcPvWarp || warp == kTcLoadVWarp ? NV : NS;
         auto step = [&]() {
-            if (++slot == NS) {
+            if (++slot == slots) {
                 slot = 0;
                 phase ^= 1;
             }
@@ -972,7 +1000,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
         } else if (warp == kTcPvWarp) {
             // ------------------------------------------------------ O += P V
-            constexpr uint32_t kId = idesc<MT>(D, true);
+            constexpr uint32_t kId = idesc<VT>(D, true);
             const uint32_t tm = __shfl_sync(kFull, tmem, 0);
             uint32_t p_phase[2] = {0, 0};
             for (; ok && segment(&b1); it.next(plan)) {
@@ -984,23 +1012,67 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     end[x] = min(b1, me.blocks);
                     half[x] = me.half(end[x] - 1);
                 }
-                for (int b = it.b0; b < b1; ++b) {
+                if constexpr (C::kV == 3) {
+                    for (int g = 2 * it.b0; ok && g < 2 * b1; ++g) {
+                        // 64 keys: their values' three parts, a slot each
+                        uint64_t vb[3];
+                        const int left = it.q.keys - 64 * g;
+                        uint32_t at[3];
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) {
+                            if (!ok || !(ok = warp_wait(v_full + 8 * slot, phase))) continue;
+                            at[c] = slot;
+                            const uint32_t to = v_s + __shfl_sync(kFull, slot, 0) * C::kVTile;
+                            vb[c] = desc_mn(to, 64 * 128);
+                            // the rows behind the last value: zeros, so that no NaN of
+                            // another sequence meets a weight of 0
+                            if (left < 64) {
+                                for (int row = max(0, left) + (lane >> 3); row < 64; row += 4)
+#pragma unroll
+                                    for (int i = 0; i < D / 64; ++i)
+                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + i * 8192u + (uint32_t)row * 128u + (lane & 7) * 16u), "r"(0u) : "memory");
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                            }
+                            step();
+                        }
+#pragma unroll
+                        for (int x = 0; x < kTcSubs; ++x) {
+                            if (!ok || g >= 2 * end[x]) continue;
+                            if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
+                            p_phase[x] ^= 1;
+                            fence_after();
+                            // the products of part c of the values and k of the weights above 2^-24, small ones first
+                            const uint32_t pt = tm + C::p_col(x), ot = tm + C::o_col(x);
+                            mma_ts64(ot, pt + 64u, vb[0], kId, g != 2 * it.b0);
+                            mma_ts64(ot, pt + 32u, vb[1], kId, 1u);
+                            mma_ts64(ot, pt, vb[2], kId, 1u);
+                            mma_ts64(ot, pt + 32u, vb[0], kId, 1u);
+                            mma_ts64(ot, pt, vb[1], kId, 1u);
+                            mma_ts64(ot, pt, vb[0], kId, 1u);
+                            commit(pv_done + 8 * x);
+                        }
+                        if (!ok) break;
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) commit(v_empty + 8 * at[c]);
+                    }
+                }
+                for (int b = it.b0; C::kV == 1 && b < b1; ++b) {
                     if (!(ok = warp_wait(v_full + 8 * slot, phase))) break;
-                    const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kKTile);
+                    const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kVTile, C::kHalf);
 #pragma unroll
                     for (int x = 0; x < kTcSubs; ++x) {
                         if (!ok || b >= end[x]) continue;
                         if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
                         p_phase[x] ^= 1;
                         fence_after();
-                        constexpr uint32_t part = C::kTile >> 4, rows64 = 64 * 128 >> 4;
+                        constexpr uint32_t rows64 = 64 * 128 >> 4;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             if (C::kQ == 1 && h == 1 && b + 1 == end[x] && half[x]) break;
                             const uint32_t pt = tm + C::p_col(x) + 32u * h;
                             mma_ts64(tm + C::o_col(x), pt, vb + h * rows64, kId, h != 0 || b != it.b0);
                             if constexpr (C::kQ == 2) mma_ts64(tm + C::o_col(x), pt + 64u, vb + h * rows64, kId, 1u);
-                            if constexpr (C::kK == 2) mma_ts64(tm + C::o_col(x), pt, vb + part + h * rows64, kId, 1u);
                         }
                         commit(pv_done + 8 * x);
                     }
@@ -1045,6 +1117,22 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                             for (int c = 0; c < D / 64; ++c)
                                 tma3(q_s + x * C::kQTile + c * C::kHalf, &maps.q, 64 * c, it.h * a.group, it.q.row0 + me.token0, q_full + 8 * x);
                         }
+                    }
+                }
+                if constexpr (C::kV == 3) {
+                    if (values) {  // 64 keys of one part after another
+                        for (int u = 6 * it.b0; ok && u < 6 * b1; ++u) {
+                            if (!(ok = warp_wait(empty + 8 * slot, phase))) break;
+                            if (lane == 0) {
+                                bar_expect(full + 8 * slot, C::kVTile);
+#pragma unroll
+                                for (int c = 0; c < D / 64; ++c)
+                                    tma4(tiles + slot * C::kVTile + c * 8192u, map, 64 * c, it.h, it.q.row0 + 64 * (u / 3), u % 3, full + 8 * slot);
+                            }
+                            ++issued;
+                            step();
+                        }
+                        continue;
                     }
                 }
                 int page = page_of(it.b0);
@@ -1096,8 +1184,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
             }
             if (!ok) {  // copies in flight land before the CTA ends
-                const uint32_t from = issued > NS ? issued - NS : 0;
-                for (uint32_t i = from; i < issued; ++i) bar_wait(full + 8 * (i % NS), (i / NS) & 1);
+                const uint32_t from = issued > slots ? issued - slots : 0;
+                for (uint32_t i = from; i < issued; ++i) bar_wait(full + 8 * (i % slots), (i / slots) & 1);
                 for (int x = 0; !values && C::kQ == 1 && x < kTcSubs; ++x) bar_wait(q_full + 8 * x, q_phase[x]);
             }
         }
@@ -1154,6 +1242,7 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
 {
     using C = Tc<T, KT, D>;
     using MT = typename C::MT;
+    using VT = typename C::VT;
     const int sub = kTcRows / a.group;
     const bool paged = a.kv.table != nullptr;
     int dev = 0, sms = 0;
@@ -1165,27 +1254,27 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     const int64_t pairs = a.tokens / (sub * C::kSubs) + a.sequences, most = pairs * a.kv_heads * blocks;
     const int ctas = (int)(most < sms ? most : sms);
     const bool split = ctas > 1 && blocks > 1;
-    // scratch: a partial a share | flags | f16 planes of K and V | their units
+    // scratch: a partial a share | flags | planes of K | of V | units of K
     const size_t part_bytes = split ? (size_t)ctas * C::kPartial * sizeof(float) : 0, flag_bytes = split ? (size_t)ctas * 4 * C::kSubs * 8 : 0;
     const size_t plane_at = (part_bytes + flag_bytes + 127) & ~(size_t)127, rows = (size_t)a.tokens * a.kv_heads;
-    const size_t plane_bytes = C::kK == 2 ? rows * D * 4 : 0;  // two parts
+    const size_t key_bytes = rows * D * 2 * C::kK, value_bytes = rows * D * 2 * C::kV;
     char *scratch = nullptr;
-    if (split || C::kK == 2) e = stream_alloc((void **)&scratch, plane_at + 2 * plane_bytes + (C::kK == 2 ? rows * 8 : 0), s);
+    if (split || C::kK == 2) e = stream_alloc((void **)&scratch, plane_at + (C::kK == 2 ? key_bytes + value_bytes + rows * 4 : 0), s);
     if (e != cudaSuccess) return e;
     float *partials = split ? (float *)scratch : nullptr;
     unsigned long long *flags = (unsigned long long *)(scratch + part_bytes);
     TcMaps maps{};
     const void *k = a.kv.k, *v = a.kv.v;
     if constexpr (C::kK == 2) {
-        __half *kp = (__half *)(scratch + plane_at), *vp = kp + 2 * rows * D;
-        float *units = (float *)(vp + 2 * rows * D);
+        __half *kp = (__half *)(scratch + plane_at);
+        __nv_bfloat16 *vp = (__nv_bfloat16 *)(scratch + plane_at + key_bytes);
+        float *units = (float *)(scratch + plane_at + key_bytes + value_bytes);
         const size_t want = (2 * rows + 7) / 8, cap = (size_t)sms * 8;
-        split_kv_kernel<D><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a, kp, vp, units, units + rows);
+        split_kv_kernel<D><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a, kp, vp, units);
         e = cudaGetLastError();
         k = kp;
         v = vp;
         maps.key_unit = units;
-        maps.value_exp = units + rows;
     }
     if constexpr (C::kQ == 1) {
         const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
@@ -1194,17 +1283,21 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
         if (e == cudaSuccess) e = make_map<MT>(&maps.q, a.q, 3, qd, qs, qb);
     }
     const int page_size = paged ? 1 << a.kv.page_shift : kTcKeys;
-    const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.kv_heads, paged ? (cuuint64_t)page_size : (cuuint64_t)a.tokens,
-                              paged ? (cuuint64_t)a.kv.page_count : (cuuint64_t)C::kK};
+    cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)a.kv_heads, paged ? (cuuint64_t)page_size : (cuuint64_t)a.tokens,
+                        paged ? (cuuint64_t)a.kv.page_count : (cuuint64_t)C::kK};
     int64_t ks[3] = {a.kv.head, a.kv.k_pos, paged ? a.kv.page : a.kv.k_pos}, vs[3] = {a.kv.head, a.kv.v_pos, paged ? a.kv.page : a.kv.v_pos};
     if constexpr (C::kK == 2) {
         ks[0] = vs[0] = D;
         ks[1] = vs[1] = (int64_t)a.kv_heads * D;
         ks[2] = vs[2] = (int64_t)rows * D;
     }
-    const cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
+    cuuint32_t kb[4] = {64, 1, (cuuint32_t)(page_size < kTcKeys ? page_size : kTcKeys), 1};
     if (e == cudaSuccess) e = make_map<MT>(&maps.k, k, 4, kd, ks, kb);
-    if (e == cudaSuccess) e = make_map<MT>(&maps.v, v, 4, kd, vs, kb);
+    if constexpr (C::kV == 3) {
+        kd[3] = 3;
+        kb[2] = 64;
+    }
+    if (e == cudaSuccess) e = make_map<VT>(&maps.v, v, 4, kd, vs, kb);
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
                       sub, divisor(sub * C::kSubs), divisor(ctas)};
     if (e == cudaSuccess) {

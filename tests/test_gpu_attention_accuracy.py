@@ -1,0 +1,139 @@
+"""How exact attention is on inputs whose rows, weights or values differ widely
+in magnitude: the root of the mean square error against a model of it, which a
+lost part of an operand passes by far (the worst-case bounds of
+attention_cases.py do not notice one).
+
+Per output element, with A = sum_j w_j |v_j|, o the output and n the row's keys:
+ * weights and values meet in parts that hold 22 bits each: 2^-22 A twice;
+ * a score is summed over 3 D / 16 steps of 16 products, each of which rounds
+   the sum so far by up to 2^-23 of it.  The sum is of the size of
+   c_j = scale sqrt(sum_e (q_e k_je)^2), and the steps are independent, so a
+   score is off by sqrt(3 D / 16) 2^-23 c_j, and a normalised weight by twice
+   that at most: sqrt(3 D / 16) 2^-22 (sum_j w_j c_j) A.  (A score that is one
+   exact product has no such error.)
+ * the output is summed over 48 steps each 128 keys at most, each of which
+   rounds the sum so far, of the size of o: sqrt(48 n / 128) 2^-23 |o|.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from attention_cases import Batch, reference  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def healthy(cuda, qmv):
+    qmv.device_status(clear=True)
+    yield
+    assert qmv.device_status(clear=True) == 0
+
+
+def model(q, k, v, scale, one_product=()):
+    """(out, A, modelled error / A), 64 bits; one_product: keys whose scores are
+    one exact product."""
+    n, heads, d = q.shape
+    keys, kv_heads = k.shape[0], k.shape[1]
+    live = torch.arange(keys, device=q.device)[None, :] <= torch.arange(n, device=q.device)[:, None] + keys - n
+    out, mass, err = (torch.zeros(n, heads, d, dtype=torch.float64, device=q.device) for _ in range(3))
+    for a in range(heads):
+        h = a // (heads // kv_heads)
+        w = torch.softmax(torch.where(live, scale * (q[:, a] @ k[:, h].T), -math.inf), -1)
+        out[:, a], mass[:, a] = w @ v[:, h], w @ v[:, h].abs()
+        c = scale * ((q[:, a] ** 2) @ (k[:, h] ** 2).T).sqrt()
+        for j in one_product:
+            c[:, j] = 0.0
+        score = math.sqrt(3 * d / 16) * 2.0 ** -22 * (w * c).sum(-1, keepdim=True)
+        steps = (48 * live.sum(-1, keepdim=True).double() / 128).sqrt() * 2.0 ** -23
+        part = (out[:, a].abs() / mass[:, a].clamp_min(1e-300)) * steps
+        err[:, a] = (2 * 2.0 ** -44 + score ** 2 + part ** 2).sqrt()
+    return out, mass, err
+
+
+def rms_of(b, packed, one_product=()):
+    """Worst ratio of the measured to the modelled root mean square error of a
+    sequence's columns."""
+    torch.cuda.synchronize()
+    worst, a = 0.0, 0
+    for s, n in enumerate(b.new):
+        k, v = b.kv_of(s, packed)
+        q = b.q[a:a + n].double().view(n, b.heads, b.d)
+        out, mass, err = model(q, k, v, 1.0 / math.sqrt(b.d), one_product)
+        got = b.out[a:a + n].double().view_as(out)
+        a += n
+        assert torch.isfinite(got).all()
+        use = mass > 0
+        assert torch.equal(got[~use], out[~use])
+        rel = torch.where(use, (got - out) / mass.clamp_min(1e-300), 0.0)
+        err = torch.where(use, err, 0.0)
+        # of a column over all rows and heads, so that one bad column shows
+        ratio = rel.square().mean((0, 1)).sqrt() / err.square().mean((0, 1)).sqrt().clamp_min(2.0 ** -22)
+        worst = max(worst, float(ratio.max()))
+    return worst
+
+
+# -------------------------------------------------- values of f32 prompts
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e10, 1e30])
+@pytest.mark.parametrize("token", [2, 127, 300, 511])
+def test_one_large_value_reaches_its_column_only(qmv, heads, kv_heads, d, size, token):
+    """One element of one value row is large: the other columns, that token's
+    own too, and the earlier tokens are as exact as without it."""
+    b = Batch(qmv, "f32", heads, kv_heads, d, [512, 40])
+    b.v[token, 5] = size
+    b.run_packed()
+    b.check(True)
+    assert rms_of(b, True) <= 1.0
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("what", ["as they are", "small", "tiny", "large", "rows apart", "elements apart"])
+def test_values_of_any_size(qmv, heads, kv_heads, d, what):
+    b = Batch(qmv, "f32", heads, kv_heads, d, [700, 65, 1, 130])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    if what in ("small", "tiny", "large"):
+        b.v.mul_({"small": 2.0 ** -74, "tiny": 1e-30, "large": 1e35}[what])
+    elif what == "rows apart":
+        b.v.mul_(torch.exp2(torch.randint(-40, 41, (b.tokens, 1), generator=g, device="cuda").float()))
+    elif what == "elements apart":
+        b.v.mul_(torch.exp2(torch.randint(-30, 31, b.v.shape, generator=g, device="cuda").float()))
+    b.run_packed()
+    b.check(True)
+    assert rms_of(b, True) <= 1.0
+
+
+# ------------------------------------------------------- a sink's neighbours
+
+def sink_batch(qmv, t, heads, kv_heads, d, log2_weight, new=(20, 1), kv=(1000, 9000), packed=False):
+    """The first key has 2^log2_weight times a middling key's weight and a value
+    of 0, so that the output is made of small weights.  Its score is one exact
+    product: channel 0 of every query is 4, of every other key 0."""
+    b = Batch(qmv, t, heads, kv_heads, d, new, new if packed else kv, poison=False)
+    b.rows[:, 0:heads * d:d] = 4.0
+    size = log2_weight * math.log(2.0) * math.sqrt(d) / 4.0
+    first = torch.zeros(1, kv_heads, d, dtype=b.dtype if packed else b.keys.dtype, device="cuda")
+    first[:, :, 0] = size
+    if packed:
+        b.k[:, ::d] = 0.0
+        at = 0
+        for n in new:
+            b.k[at], b.v[at] = first.view(-1), 0.0
+            at += n
+    else:
+        (b.keys if b.layout == "position" else b.keys.transpose(1, 2))[..., 0] = 0.0
+        for s in range(len(new)):
+            b.put(b.keys, s, torch.tensor([0], device="cuda"), first)
+            b.put(b.values, s, torch.tensor([0], device="cuda"), torch.zeros_like(first))
+    return b
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("log2_weight", [12, 24, 60])
+def test_small_weights_of_prompts(qmv, heads, kv_heads, d, log2_weight):
+    b = sink_batch(qmv, "f32", heads, kv_heads, d, log2_weight, new=(700, 130), packed=True)
+    b.run_packed()
+    b.check(True)
+    assert rms_of(b, True, one_product=(0,)) <= 1.0
