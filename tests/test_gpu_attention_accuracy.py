@@ -11,6 +11,10 @@ Per output element, with A = sum_j w_j |v_j|, o the output and n the row's keys:
    score is off by sqrt(3 D / 16) 2^-23 c_j, and a normalised weight by twice
    that at most: sqrt(3 D / 16) 2^-22 (sum_j w_j c_j) A.  (A score that is one
    exact product has no such error.)
+ * a weight is 2^e_j, e_j <= 0 its score behind the row's largest one in log2,
+   rounded to f32: off by 2^-24 |e_j| at most, so the weight by ln 2 times that
+   of itself, and the output by ln 2 2^-24 sum_j w_j |e_j| |v_j|.  (Beside a sink
+   of 2^60 times their weight that is 2.5e-6 A, for exact scores too.)
  * the output is summed over 48 steps each 128 keys at most, each of which
    rounds the sum so far, of the size of o: sqrt(48 n / 128) 2^-23 |o|.
 """
@@ -47,8 +51,9 @@ def model(q, k, v, scale, one_product=()):
             c[:, j] = 0.0
         score = math.sqrt(3 * d / 16) * 2.0 ** -22 * (w * c).sum(-1, keepdim=True)
         steps = (48 * live.sum(-1, keepdim=True).double() / 128).sqrt() * 2.0 ** -23
+        behind = (w * torch.log2(w / w.amax(-1, keepdim=True)).clamp_min(-1e4).abs()) @ v[:, h].abs() / mass[:, a].clamp_min(1e-300)
         part = (out[:, a].abs() / mass[:, a].clamp_min(1e-300)) * steps
-        err[:, a] = (2 * 2.0 ** -44 + score ** 2 + part ** 2).sqrt()
+        err[:, a] = (2 * 2.0 ** -44 + score ** 2 + part ** 2 + (math.log(2.0) * 2.0 ** -24 * behind) ** 2).sqrt()
     return out, mass, err
 
 
