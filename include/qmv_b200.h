@@ -393,8 +393,10 @@ int qmv_qwen2_forward_profiled(QmvQwen2 *decoder, int token, float *logits, int 
  * softmax's weights meet the values in the 16-bit type of the values.  f32
  * activations: queries and keys meet as pairs of f16 that each row's largest
  * |x| scales (an element is held to 22 bits, or to 2^-39 of that largest one);
- * weights meet f16 pages in pairs of f16, and f32 values, which keep 24 bits
- * from 1e-30 on wherever they stand, with 24 bits.
+ * weights meet f16 pages in pairs of f16 (22 bits for weights down to 2^-18 of
+ * the row's largest, 2^-40 of that below), and f32 values, which keep 24 bits
+ * from 1e-30 on wherever they stand, with 24 bits.  A single f16 weight keeps
+ * its 11 bits down to 2^-27 of the row's largest.
  *
  * Row starts, lengths and page tables are read on the device, so a captured
  * graph can be replayed after they change; the counts passed by the host stay.

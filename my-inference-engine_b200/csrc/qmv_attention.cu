@@ -290,8 +290,12 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
     using C = Dc<D>;
     constexpr int NQ = sizeof(T) == 4 ? 2 : 1;  // f16 pairs for f32 activations
     constexpr int KS = D / 16, NT = D / 8;
-    // the weights' exponent offset: f16 weights down to 2^-22 stay normal
-    constexpr float kLift = std::is_same<KT, __half>::value ? 8.f : 0.f;
+    // the weights' exponent offset: the reference is the maximum itself, so f16
+    // weights may reach 2^15.875 (f16 ends at 2^16 - 32; a score so large that
+    // its rounding passes that gives an infinity, and its row is computed again)
+    // and stay normal down to 2^-29 of the largest (as pairs: 22 bits to 2^-18,
+    // 2^-40 below)
+    constexpr float kLift = std::is_same<KT, __half>::value ? 15.875f : 0.f;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ unsigned bad_rows;
     __shared__ Start<DcIter> begin;

@@ -23,8 +23,8 @@
 // softmax waited 950 to 1250 of 3250 cycles a block for its next scores; with
 // S in halves of 64 keys it did not wait, but the N = 64 MMAs ran at half rate.)
 // The reference m is the running maximum, but it is raised only when the
-// maximum passes it by 8 (a factor of 256; f32 sums and 16-bit floating
-// weights do not care), so O is rescaled a few times a row at most.
+// maximum passes it by kRaise (f32 sums do not care), so O is rescaled a few
+// times a row at most.
 //
 // Where no row of a tile sees the second half of its last block (half of all
 // tiles, and every short prompt), 16-bit activations leave it out of the
@@ -54,7 +54,6 @@ constexpr int kTcKeys = 128;     // keys of a block
 constexpr int kTcRows = 128;     // rows of a tile
 constexpr int kTcThreads = 384;  // warps 0-3 and 4-7: softmax of a tile each; then
 constexpr int kTcQkWarp = 8, kTcPvWarp = 9, kTcLoadVWarp = 11;  // 10: loads Q and K
-constexpr float kRaise = 8.f;  // how far the maximum may pass the reference, log2
 
 // T, KT: types of the activations and of the keys and values.
 //
@@ -98,6 +97,19 @@ template <typename T, typename KT, int D> struct Tc {
     static __host__ __device__ constexpr uint32_t s_col(int x) { return kScores == 2 ? 128u * x : 0u; }
     static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + kPCols * x; }
     static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + kPCols * kSubs + (uint32_t)D * x; }
+    // How far the maximum may pass the reference before it is raised, and how far
+    // the weights are lifted, both log2.  bf16 weights have exponents enough.
+    // f16 ones are lifted to 2^15.875 (f16 ends at 2^16 - 32): they keep their 11
+    // bits down to 2^-27 of the largest, and as pairs 22 bits down to 2^-18 and
+    // 2^-40 of the largest below; beside a sink that has most of the weight and
+    // little value, those make the output.  (With 8 and 4, a row whose sink had
+    // 2^20 times a middling key's weight kept 9 of 22 bits.  A score so large that
+    // its rounding passes the end gives an infinity, and that row is computed
+    // again.)  Raising at once takes 2 per cent of a step of 16 sequences with up
+    // to 256 tokens; a second output for the pairs' small halves, scaled to keep
+    // 22 bits down to 2^-27, took 12.
+    static constexpr float kRaise = !std::is_same<VT, __half>::value ? 8.f : kP == 2 ? 0.f : 2.f;
+    static constexpr float kLift = std::is_same<VT, __half>::value ? 15.875f - kRaise : 0.f;
     static_assert(128 * kScores + ((int)kPCols + D) * kSubs <= 512, "tensor memory");
     static constexpr int kPartial = kSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
 };
@@ -707,7 +719,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     using MT = typename C::MT;
     using VT = typename C::VT;
     constexpr int NS = C::kSlots, NV = C::kVSlots, kTcSubs = C::kSubs;
-    constexpr float kLift = std::is_same<VT, __half>::value ? 4.f : 0.f;  // small f16 weights stay normal
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * NS + 2 * NV + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
@@ -847,7 +858,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < N; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
-                const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : kRaise));
+                const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : C::kRaise));
                 // P and O as the block before this one left them
                 if (done > 0) {
                     if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
@@ -869,7 +880,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m - kLift;
+                const float base = m == -INFINITY ? 0.f : m - C::kLift;
                 const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 constexpr int W = C::kP > 1 ? 16 : 32;  // columns of P a store

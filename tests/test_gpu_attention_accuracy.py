@@ -136,9 +136,33 @@ def sink_batch(qmv, t, heads, kv_heads, d, log2_weight, new=(20, 1), kv=(1000, 9
 
 
 @pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("log2_weight", [12, 16, 20, 24])
+@pytest.mark.parametrize("hint", [1, 1000])
+def test_small_weights_beside_a_sink(qmv, heads, kv_heads, d, log2_weight, hint):
+    """f32 over f16 pages: the weights' pairs reach down to 2^-24 of the largest."""
+    b = sink_batch(qmv, "f32", heads, kv_heads, d, log2_weight)
+    b.run_paged(max_query=hint)
+    b.check(False)
+    assert rms_of(b, False, one_product=(0,)) <= 1.0
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
 @pytest.mark.parametrize("log2_weight", [12, 24, 60])
 def test_small_weights_of_prompts(qmv, heads, kv_heads, d, log2_weight):
     b = sink_batch(qmv, "f32", heads, kv_heads, d, log2_weight, new=(700, 130), packed=True)
     b.run_packed()
     b.check(True)
     assert rms_of(b, True, one_product=(0,)) <= 1.0
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("log2_weight", [12, 20, 26])
+@pytest.mark.parametrize("hint", [1, 1000])
+def test_small_weights_in_16_bits(qmv, t, heads, kv_heads, d, log2_weight, hint):
+    b = sink_batch(qmv, t, heads, kv_heads, d, log2_weight, new=(20, 1, 5), kv=(1000, 9000, 40))
+    b.run_paged(max_query=hint)
+    b.check(False)
+    b = sink_batch(qmv, t, heads, kv_heads, d, log2_weight, new=(300, 30), packed=True)
+    b.run_packed()
+    b.check(True)
