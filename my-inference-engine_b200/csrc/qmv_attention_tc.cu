@@ -39,6 +39,7 @@
 // So ragged lengths, causal triangles and single long chunks load every SM alike.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 #include <atomic>
@@ -703,7 +704,10 @@ __device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, cons
             attention_row<T, KT, D>(a, __shfl_sync(kFull, w.token_row, who), __shfl_sync(kFull, w.head, who), it.s, it.q, row_q, 0, D);
         }
     } else {
-        part[kTcRows * D + r] = w.any || sources > 0 ? w.m : -INFINITY;
+        // minus infinity: the row sees no key of the share.  Where it does, a
+        // maximum that met only NaN scores, or only minus infinities whose
+        // values may be NaN, must not say so.
+        part[kTcRows * D + r] = w.keys <= it.b0 * kTcKeys ? -INFINITY : isnan(w.l) ? w.l : fmaxf(w.m, -FLT_MAX);
         part[kTcRows * D + kTcRows + r] = w.l;
         __syncwarp();
         if (lane == 0) flag_set(flag + (size_t)share * (4 * C::kSubs), launch);
