@@ -546,7 +546,7 @@ struct TcMaps {
 // tc_join are not inlined: their registers would be taken from the softmax
 // loop (440 and not 400 us for a prompt of 8192 tokens).
 template <typename T, typename KT, int D>
-__device__ __noinline__ void tc_store(const AttnArgs &a, uint32_t o_t, float inv, int token_row, int head, int s, Seq q, float *row_q)
+__device__ __noinline__ void tc_store(const AttnArgs &a, uint32_t o_t, float inv, int token_row, int head, int *again)
 {
     const bool row = token_row >= 0, wide = (((uintptr_t)a.out | (uintptr_t)(a.out_ld * sizeof(T))) & 31u) == 0;
     T *out = (T *)a.out + (int64_t)(row ? token_row : 0) * a.out_ld + (int64_t)head * D;
@@ -571,12 +571,29 @@ __device__ __noinline__ void tc_store(const AttnArgs &a, uint32_t o_t, float inv
             store32<T>(out + c + 32, o + 32, wide);
         }
     }
-    const bool bad = !((check[0].x + check[0].y) + (check[1].x + check[1].y) == 0.f);
-    // a masked NaN or infinity met the sums: those rows again, without it
-    for (unsigned left = __ballot_sync(kFull, bad && row); left; left &= left - 1) {
-        const int who = __ffs(left) - 1;
-        __syncwarp();
-        attention_row<T, KT, D>(a, __shfl_sync(kFull, token_row, who), __shfl_sync(kFull, head, who), s, q, row_q, 0, D);
+    // a masked NaN or infinity may have met the sums
+    if (row && !((check[0].x + check[0].y) + (check[1].x + check[1].y) == 0.f)) *again = 1;
+}
+
+// The rows of this warp's share that came out not finite, computed again
+// without masked keys.  A row may take long (32 keys some microseconds), so
+// this comes when no other warp or CTA waits for anything of this warp's any
+// more: their limits stay those of a launch without such rows.
+template <typename T, typename KT, int D>
+__device__ __noinline__ void tc_again(const AttnArgs &a, const TcPlan &plan, TcIter it, long long u1, int x, float *row_q)
+{
+    const int lane = threadIdx.x & 31, r0 = 32 * ((threadIdx.x >> 5) & 3);
+    for (; it.s < plan.sequences && it.block_at(plan, u1) > it.b0; it.next(plan)) {
+        if (it.b0 > 0) continue;  // written by an earlier share
+        const TcSub me(plan, it, x);
+        for (int r = r0; r < min(r0 + 32, me.tokens * a.group); ++r) {
+            const int token = r / a.group, head = it.h * a.group + r - token * a.group, row = it.q.row0 + me.token0 + token;
+            const T *out = (const T *)a.out + (int64_t)row * a.out_ld + (int64_t)head * D;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < D; e += 32) bad |= !isfinite(Elem<T>::to_float(out[e + lane]));
+            if (__any_sync(kFull, bad)) attention_row<T, KT, D>(a, row, head, it.s, it.q, row_q, 0, D);
+        }
     }
 }
 
@@ -596,7 +613,7 @@ constexpr int kJoin = 8;
 
 template <typename T, typename KT, int D>
 __device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, const TcIter &it, const Deal &deal, int x, uint32_t o_t, TcRow w,
-                                     float *partials, unsigned long long *flags, unsigned long long launch, float *row_q)
+                                     float *partials, unsigned long long *flags, unsigned long long launch, int *again)
 {
     using C = Tc<T, KT, D>;
     const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, r = 32 * quarter + lane, share = my_share();
@@ -697,12 +714,7 @@ __device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, cons
         }
     }
     if (whole) {
-        // a masked NaN or infinity met the sums: those rows again, without it
-        for (unsigned left = __ballot_sync(kFull, w.row && !(check == 0.f)); left; left &= left - 1) {
-            const int who = __ffs(left) - 1;
-            __syncwarp();
-            attention_row<T, KT, D>(a, __shfl_sync(kFull, w.token_row, who), __shfl_sync(kFull, w.head, who), it.s, it.q, row_q, 0, D);
-        }
+        if (w.row && !(check == 0.f)) *again = 1;  // a masked NaN or infinity may have met the sums
     } else {
         // minus infinity: the row sees no key of the share.  Where it does, a
         // maximum that met only NaN scores, or only minus infinities whose
@@ -727,7 +739,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     __shared__ __align__(8) unsigned long long bars[2 * NS + 2 * NV + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ Start<TcIter> begin;
-    __shared__ float row_q[8][D];
+    __shared__ float row_q[4 * kTcSubs][D];
+    __shared__ int again[8];  // of each softmax warp: a row of its came out not finite
     // of f32 keys: each key's unit, a copy a warp, this block's and the next one's
     __shared__ __align__(16) float key_of[C::kK == 2 ? 4 * kTcSubs : 1][2][C::kK == 2 ? kTcKeys : 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -743,6 +756,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
     }
+    if (tid < 8) again[tid] = 0;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             bar_init(k_full + 8 * i, 1);
@@ -945,12 +959,14 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 fence_after();
             }
             if (it.b0 > 0 || b1 < it.blocks) {
-                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, launch, row_q[warp]);
+                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, launch, again + warp);
             } else {
-                tc_store<T, KT, D>(a, o_t, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, it.s, it.q, row_q[warp]);
+                tc_store<T, KT, D>(a, o_t, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, again + warp);
             }
             fence_before();
         }
+        __syncwarp();
+        if (ok && *(volatile int *)(again + warp)) tc_again<T, KT, D>(a, plan, begin.it, u1, x, row_q[warp]);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         uint32_t slot = 0, phase = 0;  // of this warp's next block of K or V
