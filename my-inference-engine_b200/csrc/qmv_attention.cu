@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                     if (!(bad >> r & 1u)) continue;
                     const int row = it.rt * kDcRows + r, token = row / a.group;
                     attention_row<T, KT, D>(a, it.q.row0 + token, it.h * a.group + row - token * a.group, it.s, it.q,
-                                            merge + warp * D, 0, D);
+                                            merge + warp * D);
                 }
                 __syncthreads();
                 if (tid == 0) bad_rows = 0u;

@@ -317,20 +317,20 @@ template <int NT, typename Plan, typename Iter> __device__ __forceinline__ void 
 // ------------------------------------------------------ attention by rows
 //
 // One warp computes one (token, query head) in f32 on the CUDA cores: a lane
-// a key for the scores, a lane D / 32 elements for the output, of which
-// columns [col0, col1) are written.  Masked keys are never read.  The faster
-// kernels come back to it for rows that are not finite: a masked key's weight
-// of 0 times a NaN or infinite value must not reach a sum, and theirs does.
+// a key for the scores, a lane D / 32 elements for the output.  Masked keys are
+// never read.  The faster kernels come back to it for rows that are not finite:
+// a masked key's weight of 0 times a NaN or infinite value must not reach a
+// sum, and theirs does.
 
 template <typename T, typename KT, int D>
-__device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head, int s, const Seq &sq, float *qs, int col0, int col1)
+__device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head, int s, const Seq &sq, float *qs)
 {
     constexpr int V = Elem<KT>::kVec, E = D / 32;
     const int lane = threadIdx.x & 31, h = head / a.group;
     const int n_keys = sq.keys - sq.n + (row - sq.row0) + 1;
     T *out = (T *)a.out + (int64_t)row * a.out_ld + head * D;
     if (n_keys <= 0) {
-        for (int e = col0 + lane; e < col1; e += 32) out[e] = Elem<T>::from_float(0.f);
+        for (int e = lane; e < D; e += 32) out[e] = Elem<T>::from_float(0.f);
         return;
     }
     const T *q = (const T *)a.q + (int64_t)row * a.q_ld + head * D;
@@ -410,8 +410,7 @@ __device__ __noinline__ void attention_row(const AttnArgs &a, int row, int head,
         lost = __all_sync(kFull, all_nan);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e * 32 + lane >= col0 && e * 32 + lane < col1) out[e * 32 + lane] = Elem<T>::from_float(o[e] / l);
+    for (int e = 0; e < E; ++e) out[e * 32 + lane] = Elem<T>::from_float(o[e] / l);
 }
 
 }  // namespace

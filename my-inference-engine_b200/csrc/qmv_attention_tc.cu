@@ -592,7 +592,7 @@ __device__ __noinline__ void tc_again(const AttnArgs &a, const TcPlan &plan, TcI
             bool bad = false;
 #pragma unroll
             for (int e = 0; e < D; e += 32) bad |= !isfinite(Elem<T>::to_float(out[e + lane]));
-            if (__any_sync(kFull, bad)) attention_row<T, KT, D>(a, row, head, it.s, it.q, row_q, 0, D);
+            if (__any_sync(kFull, bad)) attention_row<T, KT, D>(a, row, head, it.s, it.q, row_q);
         }
     }
 }
