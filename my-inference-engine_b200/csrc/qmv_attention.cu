@@ -23,6 +23,7 @@ namespace qmv {
 namespace {
 
 __device__ unsigned int g_attention_status;
+__device__ unsigned long long g_launch_count[kLaunchCounts];
 
 // ------------------------------------------------------ rope and append
 //
@@ -285,7 +286,7 @@ template <typename T> __device__ __forceinline__ bool store4(T *out, const float
 
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ DcPlan plan,
-                                                                                 float *partials, unsigned long long *flags, unsigned long long launch)
+                                                                                 float *partials, unsigned long long *flags, LaunchTag tag)
 {
     using C = Dc<D>;
     constexpr int NQ = sizeof(T) == 4 ? 2 : 1;  // f16 pairs for f32 activations
@@ -299,11 +300,13 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ unsigned bad_rows;
     __shared__ Start<DcIter> begin;
+    __shared__ unsigned long long number;
     float *merge = (float *)(smem + C::kRing);
     float2 *ml = (float2 *)(smem + C::kRing + C::kMerge);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane & 3, grp = lane >> 2;
     if (blockIdx.x == 0) check_metadata(a.status, a.start, a.length, a.sequences, a.tokens, plan.max_keys);
     if (tid == 0) bad_rows = 0u;
+    if (tid == kDcThreads - 1) number = number_of(tag);
     find_start<kDcThreads>(plan, &begin);
     const long long u1 = begin.u1;
     DcIter it = begin.it, pf = it;
@@ -501,7 +504,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
             const int share = my_share(), last = last_block ? share : begin.deal.holder(it.u + (it.blks - 1 - it.blk));
             if (!leaves && !last_block) {
                 bool good = true;
-                for (int p = share + 1 + tid; p <= last; p += kDcThreads) good &= flag_take(flags + p, launch);
+                for (int p = share + 1 + tid; p <= last; p += kDcThreads) good &= flag_wait(flags + p, number);
                 if (!good) report(a.status, kStatusAttentionWait);
             }
 #pragma unroll
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                 }
                 __syncthreads();
             }
-            if (leaves && tid == 0) flag_set(flags + share, launch);
+            if (leaves && tid == 0) flag_set(flags + share, number);
             const unsigned bad = bad_rows;
             if (bad) {  // a masked NaN or infinity met the sums: those rows again, without it
                 for (int r = warp; r < rows; r += kDcWarps) {
@@ -656,7 +659,7 @@ cudaError_t launch_paged_append(const AppendArgs &a, cudaStream_t s)
 
 // A number for a launch's flags that no other launch has and scratch does
 // not hold by chance (splitmix64 of a counter; not 0).
-unsigned long long launch_number()
+static unsigned long long launch_number()
 {
     static std::atomic<unsigned long long> count{0x243f6a8885a308d3ull};
     unsigned long long z = count.fetch_add(0x9e3779b97f4a7c15ull);
@@ -664,6 +667,22 @@ unsigned long long launch_number()
     z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
     z ^= z >> 31;
     return z ? z : 1;
+}
+
+cudaError_t launch_tag(LaunchTag *tag, void *flags, size_t flag_bytes, cudaStream_t s)
+{
+    *tag = LaunchTag{launch_number(), nullptr};
+    if (s == nullptr || s == cudaStreamLegacy) return cudaSuccess;  // never captured
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(s, &status);
+    if (e != cudaSuccess || status != cudaStreamCaptureStatusActive) return e;
+    static std::atomic<int> used{0};
+    const int i = used.load() < kLaunchCounts ? used.fetch_add(1) : kLaunchCounts;
+    if (i >= kLaunchCounts) return cudaMemsetAsync(flags, 0, flag_bytes, s);
+    void *counts = nullptr;
+    e = cudaGetSymbolAddress(&counts, g_launch_count);
+    tag->count = (unsigned long long *)counts + i;
+    return e;
 }
 
 cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
@@ -689,10 +708,13 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s)
         char *scratch = nullptr;  // a partial and a flag a share
         if (e == cudaSuccess && split) e = stream_alloc((void **)&scratch, bytes + (size_t)ctas * 8, s);
         if (e != cudaSuccess) return e;
+        LaunchTag tag{0, nullptr};
+        if (split) e = launch_tag(&tag, scratch + bytes, (size_t)ctas * 8, s);
         const DcPlan plan{a.start, a.length, a.sequences, a.tokens, a.kv.max_pages << a.kv.page_shift, a.kv_heads, a.group, divisor(ctas)};
-        decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, plan, (float *)scratch, (unsigned long long *)(scratch + bytes),
-                                                                                        launch_number());
-        e = cudaGetLastError();
+        if (e == cudaSuccess) {
+            decode_attention_kernel<T, KT, D><<<(unsigned)ctas, kDcThreads, C::kSmem, s>>>(a, plan, (float *)scratch, (unsigned long long *)(scratch + bytes), tag);
+            e = cudaGetLastError();
+        }
         const cudaError_t f = stream_free(scratch, s);
         return e != cudaSuccess ? e : f;
     });

@@ -175,10 +175,15 @@ __device__ __forceinline__ void check_metadata(unsigned int *status, const int *
 // as a rule it finds them there, adds them in order and writes the output.
 // CTA b has share gridDim.x - 1 - b: a share waits only for later shares,
 // whose CTAs were dispatched before its own, so every wait ends however
-// many CTAs are resident.  (A second kernel for the join took 4 to 10 us.)
+// many CTAs are resident.  (The hardware dispatches CTAs in the order of their
+// index; CUDA does not promise it, and where it did not hold a wait could run
+// into its limit, which the status reports.  A second kernel for the join took
+// 4 to 10 us.)
 //
-// Flags carry a number of the launch's own, so scratch needs no clearing; who
-// waited for a flag clears it, for the next replay of a captured launch.
+// Flags carry a number of the launch's own, so scratch needs no clearing.  A
+// captured launch has a count beside it (LaunchTag), so that each replay has its
+// own number too, and a flag that a share set after its wait had expired is
+// nothing to the next replay.
 
 // Division by a number the host knows: its floor(2^64 / d) + 1 (exact for
 // dividends below 2^31; within 1 above, and corrected).
@@ -236,18 +241,24 @@ __device__ __forceinline__ void flag_set(unsigned long long *flag, unsigned long
     asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(flag), "l"(launch) : "memory");
 }
 
-// Waits (bounded) for a flag and clears it; false when the wait expired.
-__device__ __forceinline__ bool flag_take(unsigned long long *flag, unsigned long long launch)
+// Waits (bounded) for a flag; false when the wait expired.
+__device__ __forceinline__ bool flag_wait(const unsigned long long *flag, unsigned long long launch, unsigned long long limit_ns = kWaitLimitNs)
 {
     unsigned long long v, t0 = 0;
     for (uint32_t n = 0;; ++n) {
         asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(flag) : "memory");
-        if (v == launch) break;
+        if (v == launch) return true;
         if (n == 0) t0 = now_ns();
-        if ((n & 63u) == 63u && now_ns() - t0 > kWaitLimitNs) return false;
+        if ((n & 63u) == 63u && now_ns() - t0 > limit_ns) return false;
     }
-    *flag = 0ull;
-    return true;
+}
+
+// The number of this launch, by one thread of every CTA, once.  All CTAs of a
+// replay count, and each before it knows the number, so the count is between
+// k gridDim.x and (k + 1) gridDim.x - 1 for all of replay k.
+__device__ __forceinline__ unsigned long long number_of(const LaunchTag &tag)
+{
+    return tag.number + (tag.count ? atomicAdd(tag.count, 1ull) / gridDim.x : 0ull);
 }
 
 // Sum over the CTA's NT threads of one value each, and the exclusive prefix.

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace qmv {
@@ -55,7 +56,16 @@ cudaError_t launch_decode_attention(const AttnArgs &a, cudaStream_t s);
 // Prompts and chunks, on tcgen05.
 cudaError_t launch_tc_attention(const AttnArgs &a, cudaStream_t s);
 
-unsigned long long launch_number();
+// What a launch's flags carry: a number that no other launch has, and where the
+// launch is captured, a count of CTAs on the device that is its own.  (A captured
+// launch is one executable graph's, since the scratch it allocates is.)
+struct LaunchTag {
+    unsigned long long number, *count;
+};
+// Captured launches beyond the counts clear their flags on the stream instead,
+// which costs a replay 2 us.
+constexpr int kLaunchCounts = 4096;
+cudaError_t launch_tag(LaunchTag *tag, void *flags, size_t flag_bytes, cudaStream_t s);
 
 // Status bits of the attention kernels on the current device.
 enum : unsigned int { kStatusBadMetadata = 32u, kStatusAttentionWait = 64u };

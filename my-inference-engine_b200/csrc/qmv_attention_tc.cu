@@ -631,7 +631,7 @@ __device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, cons
     float mine = 1.f;
     if (sources > 0) {
         bool good = true;
-        for (int k = lane; k < sources; k += 32) good &= flag_take(flag + (size_t)source(k) * (4 * C::kSubs), launch);
+        for (int k = lane; k < sources; k += 32) good &= flag_wait(flag + (size_t)source(k) * (4 * C::kSubs), launch);
         if (!good) report(a.status, kStatusAttentionWait);
         __syncwarp();
         float top = w.m, sum = 0.f;
@@ -729,7 +729,7 @@ __device__ __noinline__ void tc_join(const AttnArgs &a, const TcPlan &plan, cons
 template <typename T, typename KT, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
 tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ TcMaps maps, const __grid_constant__ TcPlan plan,
-                    float *partials, unsigned long long *flags, unsigned long long launch)
+                    float *partials, unsigned long long *flags, LaunchTag tag)
 {
     using C = Tc<T, KT, D>;
     using MT = typename C::MT;
@@ -739,6 +739,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     __shared__ __align__(8) unsigned long long bars[2 * NS + 2 * NV + 6 * kTcSubs + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ Start<TcIter> begin;
+    __shared__ unsigned long long number;
     __shared__ float row_q[4 * kTcSubs][D];
     __shared__ int again[8];  // of each softmax warp: a row of its came out not finite
     // of f32 keys: each key's unit, a copy a warp, this block's and the next one's
@@ -757,6 +758,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
     }
     if (tid < 8) again[tid] = 0;
+    if (tid == kTcThreads - 1) number = number_of(tag);
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             bar_init(k_full + 8 * i, 1);
@@ -959,7 +961,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 fence_after();
             }
             if (it.b0 > 0 || b1 < it.blocks) {
-                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, launch, again + warp);
+                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, number, again + warp);
             } else {
                 tc_store<T, KT, D>(a, o_t, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, again + warp);
             }
@@ -1294,6 +1296,8 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     if (e != cudaSuccess) return e;
     float *partials = split ? (float *)scratch : nullptr;
     unsigned long long *flags = (unsigned long long *)(scratch + part_bytes);
+    LaunchTag tag{0, nullptr};
+    if (split) e = launch_tag(&tag, flags, flag_bytes, s);
     TcMaps maps{};
     const void *k = a.kv.k, *v = a.kv.v;
     if constexpr (C::kK == 2) {
@@ -1301,8 +1305,10 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
         __nv_bfloat16 *vp = (__nv_bfloat16 *)(scratch + plane_at + key_bytes);
         float *units = (float *)(scratch + plane_at + key_bytes + value_bytes);
         const size_t want = (2 * rows + 7) / 8, cap = (size_t)sms * 8;
-        split_kv_kernel<D><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a, kp, vp, units);
-        e = cudaGetLastError();
+        if (e == cudaSuccess) {
+            split_kv_kernel<D><<<(unsigned)(want < cap ? want : cap), 256, 0, s>>>(a, kp, vp, units);
+            e = cudaGetLastError();
+        }
         k = kp;
         v = vp;
         maps.key_unit = units;
@@ -1332,7 +1338,7 @@ template <typename T, typename KT, int D> cudaError_t launch(const AttnArgs &a, 
     const TcPlan plan{a.start, a.length, a.sequences, a.tokens, paged ? a.kv.max_pages << a.kv.page_shift : 0x7fffffff, a.kv_heads, C::kOver,
                       sub, divisor(sub * C::kSubs), divisor(ctas)};
     if (e == cudaSuccess) {
-        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, flags, launch_number());
+        tc_attention_kernel<T, KT, D><<<(unsigned)ctas, kTcThreads, C::kSmem, s>>>(a, maps, plan, partials, flags, tag);
         e = cudaGetLastError();
     }
     const cudaError_t f = stream_free(scratch, s);
