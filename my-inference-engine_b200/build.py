@@ -8,9 +8,12 @@ library can be loaded next to torch's own runtime.
 from __future__ import annotations
 
 import concurrent.futures
+import contextlib
+import fcntl
 import os
 import subprocess
 import sys
+import time
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -54,44 +57,65 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(f) <= t for f in _inputs())
 
 
+def _run(cmd, out: str, began: int) -> str:
+    """nvcc into a file of this process, which takes its place once it is whole,
+    as old as ``began``, when its sources were last looked at (what changes
+    meanwhile is newer); an object's messages are in out + ".log" before it."""
+    part = f"{out}.tmp{os.getpid()}"
+    try:
+        proc = subprocess.run([*cmd, "-o", part], capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+        if out.endswith(".o"):
+            with open(out + ".log", "w") as fh:
+                fh.write(proc.stderr)
+        os.utime(part, ns=(began, began))
+        os.replace(part, out)
+    finally:
+        if os.path.exists(part):
+            os.remove(part)
+    return proc.stderr
+
+
+@contextlib.contextmanager
+def _alone():
+    """One build at a time in this tree."""
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(os.path.join(OBJ_DIR, "lock"), "w") as fh:
+        fcntl.flock(fh, fcntl.LOCK_EX)
+        yield
+
+
 def _compile(source: str, force: bool):
     """One source to its object (skipped when newer than the source and every
     header); (object, nvcc's messages)."""
     src, obj = os.path.join(CSRC, source), os.path.join(OBJ_DIR, source + ".o")
     log = obj + ".log"
+    began = time.time_ns()
     deps = [src] + [f for f in _inputs() if f.endswith((".h", ".cuh"))] + [os.path.abspath(__file__)]
     if not force and os.path.exists(obj) and os.path.exists(log) and \
             all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in deps):
         with open(log) as fh:
             return obj, fh.read()
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO_DIR, "include"), "-I", CSRC, "-c", src, "-o", obj]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
-    with open(log, "w") as fh:
-        fh.write(proc.stderr)
-    return obj, proc.stderr
+    cmd = [_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO_DIR, "include"), "-I", CSRC, "-c", src]
+    return obj, _run(cmd, obj, began)
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile libqmv_b200.so in place (skipped when up to date), the sources
     side by side."""
-    if not force and up_to_date():
-        return LIB_PATH
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
-        built = list(pool.map(lambda s: _compile(s, force), SOURCES))
-    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH + ".tmp", *[obj for obj, _ in built],
-           "-Xlinker", "--exclude-libs,ALL"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
-    messages = "".join(m for _, m in built)
+    with _alone():
+        if not force and up_to_date():
+            return LIB_PATH
+        began = time.time_ns()
+        with concurrent.futures.ThreadPoolExecutor(len(SOURCES)) as pool:
+            built = list(pool.map(lambda s: _compile(s, force), SOURCES))
+        messages = "".join(m for _, m in built)
+        _run([_nvcc(), *NVCC_FLAGS, "-shared", *[obj for obj, _ in built], "-Xlinker", "--exclude-libs,ALL"], LIB_PATH, began)
+        with open(os.path.join(PKG_DIR, "ptxas_report.txt"), "w") as fh:
+            fh.write(messages)
     if verbose:
         sys.stderr.write(messages)
-    os.replace(LIB_PATH + ".tmp", LIB_PATH)
-    with open(os.path.join(PKG_DIR, "ptxas_report.txt"), "w") as fh:
-        fh.write(messages)
     return LIB_PATH
 
 
