@@ -166,3 +166,19 @@ def test_small_weights_in_16_bits(qmv, t, heads, kv_heads, d, log2_weight, hint)
     b = sink_batch(qmv, t, heads, kv_heads, d, log2_weight, new=(300, 30), packed=True)
     b.run_packed()
     b.check(True)
+
+
+# ------------------------------------------------------------ wide groups
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 1), (27, 3), (16, 1), (33, 1), (126, 2), (64, 1)])
+def test_wide_groups_of_heads_at_128(qmv, t, heads, kv_heads):
+    for new, kv in (([1, 2, 1], [700, 65, 3]), ([40, 3, 129], [41, 600, 300])):
+        b = Batch(qmv, t, heads, kv_heads, 128, new, kv, page=32, layout="head", pad=2)
+        for hint in (1, 1000):
+            b.out.fill_(123.0)
+            b.run_paged(max_query=hint)
+            b.check(False)
+    b = Batch(qmv, t, heads, kv_heads, 128, [150, 1, 5, 64], pad=1)
+    b.run_packed()
+    b.check(True)

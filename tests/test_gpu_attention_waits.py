@@ -5,6 +5,7 @@ import os
 import shutil
 import subprocess
 import sys
+import threading
 
 import pytest
 
@@ -125,6 +126,7 @@ def test_captured_launches_beyond_the_counts(qmv):
     since counts are not given back."""
     code = """
 import sys
+import threading
 sys.path.insert(0, %r)
 import torch, conftest
 from cuda.bindings import runtime as rt
@@ -150,3 +152,81 @@ print("all right")
     pytest.importorskip("cuda.bindings.runtime")
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "all right" in done.stdout, done.stderr[-2000:]
+
+
+# ------------------------------------------------- calls that run side by side
+
+def _side_by_side(qmv):
+    return [Batch(qmv, "bf16", 14, 2, 64, [1, 1], [5000, 4000], page=64), Batch(qmv, "f16", 8, 2, 128, [200], [1500], page=32, seed=1),
+            Batch(qmv, "f32", 14, 2, 64, [90, 3], [900, 2000], seed=2)]
+
+
+def test_every_call_of_two_streams(qmv):
+    """Each of the calls in flight together against its result alone, bit for bit."""
+    work = [(b, run) for b in _side_by_side(qmv) for run in (b.run_paged, b.run_packed)]
+    alone = []
+    for b, run in work:
+        out = torch.full_like(b.out, SENTINEL)
+        run(out=out)
+        alone.append(out)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[torch.full_like(b.out, SENTINEL) for _ in range(10 * len(streams))] for b, _ in work]
+    torch.cuda.synchronize()
+    for i in range(10 * len(streams)):
+        for j, (b, run) in enumerate(work):
+            run(stream=streams[(i + j) % 3].cuda_stream, out=outs[j][i])
+    torch.cuda.synchronize()
+    for want, got in zip(alone, outs):
+        assert all(torch.equal(want, x) for x in got)
+
+
+def test_every_call_of_two_threads(qmv):
+    bs = _side_by_side(qmv)
+    alone = []
+    for b in bs:
+        out = torch.full_like(b.out, SENTINEL)
+        b.run_paged(out=out)
+        alone.append(out)
+    outs = [[torch.full_like(b.out, SENTINEL) for _ in range(50)] for b in bs]
+    streams = [torch.cuda.Stream() for _ in bs]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(b, stream, mine):
+        try:
+            for out in mine:
+                b.run_paged(stream=stream.cuda_stream, out=out)
+        except Exception as e:  # noqa: BLE001 - handed to the test's thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(bs, streams, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failures
+    for want, got in zip(alone, outs):
+        assert all(torch.equal(want, x) for x in got)
+
+
+def test_two_captured_graphs_at_once(qmv):
+    """Replays of two graphs on two streams, each with scratch of its own."""
+    bs = _side_by_side(qmv)
+    graphs = []
+    for b in bs:
+        b.run_paged()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+            b.run_paged(stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append((b, g, b.out.clone(), torch.zeros((), dtype=torch.int64, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for b, g, want, wrong, stream in graphs:
+            with torch.cuda.stream(stream):
+                b.out.fill_(SENTINEL)
+                g.replay()
+                wrong += (b.out != want).sum()
+    torch.cuda.synchronize()
+    assert [int(x[3]) for x in graphs] == [0, 0, 0]
