@@ -392,7 +392,8 @@ int qmv_qwen2_forward_profiled(QmvQwen2 *decoder, int token, float *logits, int 
  * Sums, the softmax and its statistics are f32 whatever the types; the
  * softmax's weights meet the values in the 16-bit type of the values.  f32
  * activations: queries and keys meet as pairs of f16 that each row's largest
- * |x| scales (an element is held to 22 bits, or to 2^-39 of that largest one);
+ * |x| scales (an element is held to 22 bits, or to 2^-39 of that largest one,
+ * in rows that reach 1e-30);
  * weights meet f16 pages in pairs of f16 (22 bits for weights down to 2^-18 of
  * the row's largest, 2^-40 of that below), and f32 values, which keep 24 bits
  * from 1e-30 on wherever they stand, with 24 bits.  A single f16 weight keeps

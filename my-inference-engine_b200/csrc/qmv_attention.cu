@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kDcThreads, kDcPerSm) decode_attention_kernel(
                     big = fmaxf(big, __shfl_xor_sync(kFull, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(kFull, big, 2));
                     int e = 14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127;
-                    e = min(max(e, -100), 100);
+                    e = min(max(e, kUnitMin), kUnitMax);
                     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                     factor[half] *= __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll

@@ -40,6 +40,10 @@ template <typename KT> __device__ __forceinline__ uint32_t pack2(float a, float 
     return w;
 }
 
+// The power of two that brings a row's largest |x| into [2^14, 2^15): any but
+// those of rows below 2^-100, whose product with the scale has to stay normal.
+constexpr int kUnitMin = -113, kUnitMax = 114;
+
 // What is left of (a, b) after their f16 rounding, as f16.
 __device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t hi)
 {

@@ -336,7 +336,7 @@ template <int D> __device__ __forceinline__ float split_rows(const AttnArgs &a, 
             float big = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
 #pragma unroll
             for (int d = L / 2; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, d));
-            const int e = min(max(14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127, -100), 100);
+            const int e = min(max(14 - (int)((__float_as_uint(big) >> 23) & 255u) + 127, kUnitMin), kUnitMax);
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
             const uint32_t h0 = pack2<__half>(v[i].x * up, v[i].y * up), h1 = pack2<__half>(v[i].z * up, v[i].w * up);
             const uint32_t l0 = pack2_rest(v[i].x * up, v[i].y * up, h0), l1 = pack2_rest(v[i].z * up, v[i].w * up, h1);
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(256) split_kv_kernel(AttnArgs a, __half *__res
 #pragma unroll
         for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, d));
         const int top = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
-        const int e = min(max(14 - top, -100), 100);
+        const int e = min(max(14 - top, kUnitMin), kUnitMax);
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         __half *to = kp + (size_t)at * D + E * lane;
 #pragma unroll

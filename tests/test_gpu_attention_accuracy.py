@@ -182,3 +182,16 @@ def test_wide_groups_of_heads_at_128(qmv, t, heads, kv_heads):
     b = Batch(qmv, t, heads, kv_heads, 128, [150, 1, 5, 64], pad=1)
     b.run_packed()
     b.check(True)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(14, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("exponent", [-111, -99, 60, 111])
+def test_queries_and_keys_of_any_size(qmv, heads, kv_heads, d, exponent):
+    """Queries that are tiny and keys that are large, or the other way: powers of
+    two that cancel in the scores change nothing."""
+    b = Batch(qmv, "f32", heads, kv_heads, d, [300, 65, 1], poison=False)
+    b.q.mul_(2.0 ** exponent)
+    b.k.mul_(2.0 ** -exponent)
+    b.run_packed()
+    b.check(True)
+    assert rms_of(b, True) <= 1.0
