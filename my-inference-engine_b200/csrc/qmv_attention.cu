@@ -31,8 +31,8 @@ __device__ unsigned long long g_launch_count[kLaunchCounts];
 // from the sequence over its length and page to the first store is paid once
 // for both.  Each token's angles are formed once, in fixed point: position *
 // base^(-2i / D) / 2 pi turns, the factor held as 64 bits of a turn, so the
-// product modulo one turn is exact to position * 2^-65 turns and no position
-// is too far for the f32 sine.  Threads then take 16-byte pieces of the
+// product modulo one turn is exact to position * 2^-63 turns (the factor is cut,
+// after powl and the product) and no position is too far for the f32 sine.  Threads then take 16-byte pieces of the
 // first half of a head together with the pieces of the second half that they
 // turn with, for all query and key heads, and the value pieces; a thread's
 // first piece is on its way while the sequence, the page and the angles are found.
