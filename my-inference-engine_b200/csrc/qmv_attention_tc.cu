@@ -30,8 +30,9 @@
 // tiles, and every short prompt), 16-bit activations leave it out of the
 // softmax and of PV: 61 prompts of 1..64 tokens (f16, 32/8/128) took 34.2 us and
 // take 29.6, 13 ragged prompts (bf16, 14/2/64) 126 and 120, and a prompt of 8192
-// tokens (bf16, 28/4/128) pays 387 to 393 for the larger code.  f32, for which
-// that code took 2 to 3 per cent everywhere, does not.
+// tokens (bf16, 28/4/128) pays 387 to 393 for the larger code (replayed).  f32 over
+// f16 pages, for which that code took 2 to 3 per cent everywhere, does not; f32
+// values come by halves anyway.
 //
 // Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
 // the launch in order are cut into one equal share per SM at multiples of 128
@@ -78,9 +79,12 @@ template <typename T, typename KT, int D> struct Tc {
     // 16 bits, head_dim 128: a prompt of 8192 tokens takes 400, 399, 393, 393 us
     // with 384, 448, 512, 640, 61 prompts of 1..64 tokens 25.4, 26.3, 26.4,
     // 29.6 us; head_dim 64: 13 ragged prompts 119, 120, 119, 127 us with 256, 288,
-    // 320, 384; f32: 640 over f16 keys, 320 over f32 keys, both a few per cent
-    // better than half and one and a half of it.
-    static constexpr int kOver = kK == 2 ? 320 : kQ == 2 ? 640 : D == 64 ? 320 : 512;
+    // 320, 384; f32 over f16 keys: 640, a few per cent better than half and one
+    // and a half of it; over f32 keys, head_dim 128: 3 prompts of 400..2000 tokens
+    // (28/4) 168, 151, 151, 155 us with 320, 560, 640, 768, one of 3000 429, 350,
+    // 348, 354; head_dim 64: 14 batches of 1 to 40 prompts (14/2 and 8/8) together
+    // 848, 826, 818, 819, 828 us with 224, 272, 320, 336, 352.
+    static constexpr int kOver = kK == 2 && D == 64 ? 336 : kK == 2 ? 560 : kQ == 2 ? 640 : D == 64 ? 320 : 512;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
@@ -525,6 +529,12 @@ struct TcSub {
     int keys;            // that any of its rows sees
     // no row sees the second half of block b
     __device__ __forceinline__ bool half(int b) const { return keys - b * kTcKeys <= kTcKeys / 2; }
+    // halves of blocks that its rows see of blocks 0 .. b1 - 1
+    __device__ __forceinline__ int halves(int b1) const
+    {
+        const int end = min(b1, blocks);
+        return 2 * end - (end > 0 && half(end - 1) ? 1 : 0);
+    }
     __device__ __forceinline__ TcSub(const TcPlan &p, const TcIter &it, int x)
     {
         token0 = it.i * p.wide.d + x * p.sub;
@@ -808,7 +818,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
         const uint32_t s_t = lanes + C::s_col(x), p_t = lanes + C::p_col(x), o_t = lanes + C::o_col(x);
-        uint32_t done = 0;  // blocks (or their halves) of this tile slot handed over so far
+        uint32_t done = 0, seen = 0;  // blocks (or their halves) of this tile slot handed over so far, and blocks
         // f32 keys: units of this lane's keys (4 lane ..) of block b
         auto units_of = [&](int b, float u[4]) {
             const int64_t at = (int64_t)it.h * a.tokens + it.q.row0;
@@ -844,7 +854,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             // block b, of its keys the first N
             auto block = [&](const int b, auto cols) {
                 constexpr int N = decltype(cols)::value;
-                if (!warp_wait(s_full + 8 * x, done / C::kHalves & 1)) return false;
+                if (!warp_wait(s_full + 8 * x, (C::kHalves == 1 ? done : seen++) & 1)) return false;
                 fence_after();
                 float s[N];
 #pragma unroll
@@ -906,7 +916,8 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 constexpr int W = C::kP > 1 ? 16 : 32;  // columns of P a store
 #pragma unroll
                 for (int g = 0; g < C::kHalves; ++g) {
-                    if (g > 0) {  // the half before has left tensor memory
+                    if (g > 0) {  // once the half before has left tensor memory
+                        if (me.half(b)) break;
                         if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
                         fence_after();
                     }
@@ -1046,7 +1057,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     half[x] = me.half(end[x] - 1);
                 }
                 if constexpr (C::kV == 3) {
-                    for (int g = 2 * it.b0; ok && g < 2 * b1; ++g) {
+                    int upto[2] = {0, 0};
+#pragma unroll
+                    for (int x = 0; x < kTcSubs; ++x) upto[x] = TcSub(plan, it, x).halves(b1);
+                    for (int g = 2 * it.b0; ok && g < max(upto[0], upto[1]); ++g) {
                         // 64 keys: their values' three parts, a slot each
                         uint64_t vb[3];
                         const int left = it.q.keys - 64 * g;
@@ -1071,7 +1085,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         }
 #pragma unroll
                         for (int x = 0; x < kTcSubs; ++x) {
-                            if (!ok || g >= 2 * end[x]) continue;
+                            if (!ok || g >= upto[x]) continue;
                             if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
                             p_phase[x] ^= 1;
                             fence_after();
@@ -1154,7 +1168,9 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 }
                 if constexpr (C::kV == 3) {
                     if (values) {  // 64 keys of one part after another
-                        for (int u = 6 * it.b0; ok && u < 6 * b1; ++u) {
+                        int upto = 0;
+                        for (int x = 0; x < kTcSubs; ++x) upto = max(upto, TcSub(plan, it, x).halves(b1));
+                        for (int u = 6 * it.b0; ok && u < 3 * upto; ++u) {
                             if (!(ok = warp_wait(empty + 8 * slot, phase))) break;
                             if (lane == 0) {
                                 bar_expect(full + 8 * slot, C::kVTile);
