@@ -394,8 +394,8 @@ int qmv_qwen2_forward_profiled(QmvQwen2 *decoder, int token, float *logits, int 
  * activations: queries and keys meet as pairs of f16 that each row's largest
  * |x| scales (an element is held to 22 bits, or to 2^-39 of that largest one,
  * in rows that reach 1e-30);
- * weights meet f16 pages in pairs of f16 (22 bits for weights down to 2^-18 of
- * the row's largest, 2^-40 of that below), and f32 values, which keep 24 bits
+ * weights meet f16 pages in pairs of f16 (22 bits for weights down to 2^-17 of
+ * the row's largest, 2^-39 of that below), and f32 values, which keep 24 bits
  * from 1e-30 on wherever they stand, with 24 bits.  A single f16 weight keeps
  * its 11 bits down to 2^-27 of the row's largest.
  *

@@ -30,9 +30,8 @@
 // tiles, and every short prompt), 16-bit activations leave it out of the
 // softmax and of PV: 61 prompts of 1..64 tokens (f16, 32/8/128) took 34.2 us and
 // take 29.6, 13 ragged prompts (bf16, 14/2/64) 126 and 120, and a prompt of 8192
-// tokens (bf16, 28/4/128) pays 387 to 393 for the larger code (replayed).  f32 over
-// f16 pages, for which that code took 2 to 3 per cent everywhere, does not; f32
-// values come by halves anyway.
+// tokens (bf16, 28/4/128) pays 387 to 393 for the larger code (replayed).  f32 goes
+// by halves of a block throughout.
 //
 // Work is dealt evenly: a tile costs its keys plus a constant, all tiles of
 // the launch in order are cut into one equal share per SM at multiples of 128
@@ -79,12 +78,13 @@ template <typename T, typename KT, int D> struct Tc {
     // 16 bits, head_dim 128: a prompt of 8192 tokens takes 400, 399, 393, 393 us
     // with 384, 448, 512, 640, 61 prompts of 1..64 tokens 25.4, 26.3, 26.4,
     // 29.6 us; head_dim 64: 13 ragged prompts 119, 120, 119, 127 us with 256, 288,
-    // 320, 384; f32 over f16 keys: 640, a few per cent better than half and one
-    // and a half of it; over f32 keys, head_dim 128: 3 prompts of 400..2000 tokens
-    // (28/4) 168, 151, 151, 155 us with 320, 560, 640, 768, one of 3000 429, 350,
-    // 348, 354; head_dim 64: 14 batches of 1 to 40 prompts (14/2 and 8/8) together
-    // 848, 826, 818, 819, 828 us with 224, 272, 320, 336, 352.
-    static constexpr int kOver = kK == 2 && D == 64 ? 336 : kK == 2 ? 560 : kQ == 2 ? 640 : D == 64 ? 320 : 512;
+    // 320, 384.  f32 over f16 keys: 16 chunks of 1..256 tokens (28/4/128) 108, 97,
+    // 92, 92, 93 us with 320, 448, 540, 640, 800, (14/2/64) 45, 45, 45, 47, 47;
+    // over f32 keys, head_dim 128: 3 prompts of 400..2000 tokens (28/4) 154, 156,
+    // 157, 161, 161 us and one of 3000 390, 382, 384, 387, 395 with 400, 480, 560,
+    // 640, 720; head_dim 64 (14/2) 62, 62, 60, 65 and 138, 133, 135, 141 with 224,
+    // 288, 336, 400.
+    static constexpr int kOver = kK == 2 && D == 64 ? 336 : kK == 2 ? 560 : kQ == 2 ? 540 : D == 64 ? 320 : 512;
     static constexpr uint32_t kTile = 128 * D * 2;  // 128 rows of 16-bit elements
     static constexpr uint32_t kHalf = 128 * 128;    // 128 rows of 64 elements
     static constexpr uint32_t kQTile = kQ * kTile, kKTile = kK * kTile;
@@ -93,29 +93,32 @@ template <typename T, typename KT, int D> struct Tc {
     static constexpr int kVSlots = kV == 1 ? kSlots : D == 64 ? 10 : 5;
     static constexpr uint32_t kVTile = kV == 1 ? kTile : kTile / 2;
     static constexpr uint32_t kSmem = kSubs * kQTile + kSlots * kKTile + kVSlots * kVTile + 1024;
-    // P of a block at once, or of its halves of 64 keys one after another (three
-    // parts of 128 keys are more than tensor memory holds)
-    static constexpr int kHalves = kP == 3 ? 2 : 1;
-    static constexpr uint32_t kPCols = kP == 3 ? 96u : 64u * kP;
+    // f32 goes by halves of a block: P of 64 keys in parts of 32 columns, and a
+    // product of its own for each half, added to the output's sum by the softmax
+    // warps.  (The tensor cores cut what an addition leaves behind the 24th bit,
+    // and always towards zero: each costs 2^-24 of the sum so far.  With all of a
+    // row's keys added there, 16000 keys with values about 1 were off by 2e-4;
+    // the plain form in f32 by 1e-7.)  For head_dim 64 the sum is in registers,
+    // for 128 in tensor memory behind the product.
+    static constexpr uint32_t kPCols = kQ == 2 ? 32u * kP : 64u;
+    static constexpr int kSum = kQ == 2 && D == 128 ? D : 0;  // columns of the sum
     // tensor memory columns
-    static constexpr int kScores = D == 64 && kQ == 1 ? 2 : 1;  // S buffers
+    static constexpr int kScores = D == 64 && kK == 1 ? 2 : 1;  // S buffers
     static __host__ __device__ constexpr uint32_t s_col(int x) { return kScores == 2 ? 128u * x : 0u; }
     static __host__ __device__ constexpr uint32_t p_col(int x) { return 128u * kScores + kPCols * x; }
-    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + kPCols * kSubs + (uint32_t)D * x; }
+    static __host__ __device__ constexpr uint32_t o_col(int x) { return 128u * kScores + kPCols * kSubs + (uint32_t)(D + kSum) * x; }
     // How far the maximum may pass the reference before it is raised, and how far
     // the weights are lifted, both log2.  bf16 weights have exponents enough.
     // f16 ones are lifted to 2^15.875 (f16 ends at 2^16 - 32): they keep their 11
-    // bits down to 2^-27 of the largest, and as pairs 22 bits down to 2^-18 and
-    // 2^-40 of the largest below; beside a sink that has most of the weight and
+    // bits down to 2^-27 of the largest, and as pairs 22 bits down to 2^-17 and
+    // 2^-39 of the largest below; beside a sink that has most of the weight and
     // little value, those make the output.  (With 8 and 4, a row whose sink had
     // 2^20 times a middling key's weight kept 9 of 22 bits.  A score so large that
     // its rounding passes the end gives an infinity, and that row is computed
-    // again.)  Raising at once takes 2 per cent of a step of 16 sequences with up
-    // to 256 tokens; a second output for the pairs' small halves, scaled to keep
-    // 22 bits down to 2^-27, took 12.
-    static constexpr float kRaise = !std::is_same<VT, __half>::value ? 8.f : kP == 2 ? 0.f : 2.f;
+    // again.)
+    static constexpr float kRaise = !std::is_same<VT, __half>::value ? 8.f : kP == 2 ? 1.f : 2.f;
     static constexpr float kLift = std::is_same<VT, __half>::value ? 15.875f - kRaise : 0.f;
-    static_assert(128 * kScores + ((int)kPCols + D) * kSubs <= 512, "tensor memory");
+    static_assert(128 * kScores + ((int)kPCols + D + kSum) * kSubs <= 512, "tensor memory");
     static constexpr int kPartial = kSubs * (kTcRows * D + 2 * kTcRows);  // floats: per tile O by column quads, m, l
 };
 
@@ -818,7 +821,7 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int x = warp >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
         const uint32_t s_t = lanes + C::s_col(x), p_t = lanes + C::p_col(x), o_t = lanes + C::o_col(x);
-        uint32_t done = 0, seen = 0;  // blocks (or their halves) of this tile slot handed over so far, and blocks
+        uint32_t done = 0, seen = 0;  // of this tile slot: blocks (f32: halves) handed over so far, and f32 blocks
         // f32 keys: units of this lane's keys (4 lane ..) of block b
         auto units_of = [&](int b, float u[4]) {
             const int64_t at = (int64_t)it.h * a.tokens + it.q.row0;
@@ -851,10 +854,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             float next_units[4];
             if constexpr (C::kK == 2)
                 if (end > it.b0) units_of(it.b0, next_units);
-            // block b, of its keys the first N
+            // 16 bits: block b, of its keys the first N
             auto block = [&](const int b, auto cols) {
                 constexpr int N = decltype(cols)::value;
-                if (!warp_wait(s_full + 8 * x, (C::kHalves == 1 ? done : seen++) & 1)) return false;
+                if (!warp_wait(s_full + 8 * x, done & 1)) return false;
                 fence_after();
                 float s[N];
 #pragma unroll
@@ -864,21 +867,6 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 __syncwarp();
                 if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
                 const int j0 = b * kTcKeys;
-                if constexpr (C::kK == 2) {
-                    float *unit = key_of[warp][b & 1];
-                    *(float4 *)(unit + 4 * lane) = make_float4(next_units[0], next_units[1], next_units[2], next_units[3]);
-                    __syncwarp();
-                    if (b + 1 < end) units_of(b + 1, next_units);
-#pragma unroll
-                    for (int i = 0; i < N; i += 4) {
-                        const float4 u = lds4(unit + i);
-                        const float2 lo = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(u.x, u.y)), hi = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(u.z, u.w));
-                        s[i] = lo.x;
-                        s[i + 1] = lo.y;
-                        s[i + 2] = hi.x;
-                        s[i + 3] = hi.y;
-                    }
-                }
                 if (__any_sync(kFull, j0 + N > lim)) {
 #pragma unroll
                     for (int i = 0; i < N; ++i)
@@ -913,68 +901,194 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                 const float base = m == -INFINITY ? 0.f : m - C::kLift;
                 const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                constexpr int W = C::kP > 1 ? 16 : 32;  // columns of P a store
 #pragma unroll
-                for (int g = 0; g < C::kHalves; ++g) {
-                    if (g > 0) {  // once the half before has left tensor memory
-                        if (me.half(b)) break;
-                        if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
-                        fence_after();
+                for (int h = 0; h < N / 64; ++h) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int j = 2 * (32 * h + i);
+                        const float2 e = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, n2), w = make_float2(ex2(e.x), ex2(e.y));
+                        sum[i & 1] = __fadd2_rn(sum[i & 1], w);
+                        p[i] = pack2<VT>(w.x, w.y);
                     }
+                    tmem_st32(p_t + 32 * h, p);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full + 8 * x);
+                ++done;
+                return true;
+            };
+            // f32: block b, by halves; the output's sum before them
+            constexpr bool kInRegisters = C::kQ == 2 && C::kSum == 0;
+            float o_sum[kInRegisters ? 64 : 1];
+            constexpr auto kAt = [](int column) { return kInRegisters ? column : 0; };
+            bool summed = false;  // there is one
+            uint32_t left = 0;    // products not in it yet
+            auto add_product = [&](float fix, bool raise) {
+                if (left == 0) return true;
+                if (!warp_wait(pv_done + 8 * x, (done - 1) & 1)) return false;
+                fence_after();
+                left = 0;
+                if constexpr (C::kSum == 0) {
 #pragma unroll
-                    for (int h = 0; h < N / 2 / W / C::kHalves; ++h) {
-                        uint32_t p[C::kP][W];
+                    for (int c = 0; c < 64; c += 32) {
+                        float o[32];
+                        tmem_ld32(o_t + c, o);
+                        wait_ld();
 #pragma unroll
-                        for (int i = 0; i < W; ++i) {
-                            const int j = N / C::kHalves * g + 2 * (W * h + i);
+                        for (int i = 0; i < 32; ++i) o_sum[kAt(c + i)] += o[i];  // (in pairs 2 us slower)
+                    }
+                    if (raise) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) o_sum[kAt(i)] *= fix;
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32], to[32];
+                        tmem_ld32(o_t + c, o);
+                        tmem_ld32(o_t + D + c, to);
+                        wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 y = make_float2(o[i], o[i + 1]), z = summed ? __fadd2_rn(make_float2(to[i], to[i + 1]), y) : y;
+                            to[i] = z.x;
+                            to[i + 1] = z.y;
+                        }
+                        if (raise) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) to[i] *= fix;
+                        }
+                        tmem_st32(o_t + D + c, (const uint32_t *)to);
+                    }
+                    summed = true;
+                }
+                return true;
+            };
+            auto block_by_halves = [&](const int b) {
+                if (!warp_wait(s_full + 8 * x, seen++ & 1)) return false;
+                fence_after();
+                float *unit = key_of[C::kK == 2 ? warp : 0][C::kK == 2 ? b & 1 : 0];
+                if constexpr (C::kK == 2) {
+                    *(float4 *)(unit + 4 * lane) = make_float4(next_units[0], next_units[1], next_units[2], next_units[3]);
+                    __syncwarp();
+                    if (b + 1 < end) units_of(b + 1, next_units);
+                }
+#pragma unroll 1
+                for (int g = 0; g < 2; ++g) {
+                    const bool last = g == 1 || me.half(b);
+                    float s[64];
+                    tmem_ld32(s_t + 64 * g, s);
+                    tmem_ld32(s_t + 64 * g + 32, s + 32);
+                    wait_ld();
+                    if (last) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(s_free + 8 * (C::kScores == 2 ? x : 0));
+                    }
+                    const int j0 = b * kTcKeys + 64 * g;
+                    if constexpr (C::kK == 2) {
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            const float4 u = lds4(unit + 64 * g + i);
+                            const float2 lo = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(u.x, u.y)), hi = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(u.z, u.w));
+                            s[i] = lo.x;
+                            s[i + 1] = lo.y;
+                            s[i + 2] = hi.x;
+                            s[i + 3] = hi.y;
+                        }
+                    }
+                    if (__any_sync(kFull, j0 + 64 > lim)) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i)
+                            if (j0 + i >= lim) s[i] = -INFINITY;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+                    const bool raise = __any_sync(kFull, mx > m + (m == -INFINITY ? 0.f : C::kRaise));
+                    float fix = 1.f;
+                    if (raise) {
+                        const float mn = fmaxf(m, mx);
+                        fix = m == -INFINITY ? 0.f : ex2(m - mn);
+                        m = mn;
+                        l *= fix;
+                    }
+                    if (C::kP == 3 && !add_product(fix, raise)) return false;
+                    const float base = m == -INFINITY ? 0.f : m - C::kLift;
+                    const float2 f2 = make_float2(f, f), n2 = make_float2(-base, -base);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t p[C::kP][16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int j = 2 * (16 * h + i);
                             const float2 e = __ffma2_rn(make_float2(s[j], s[j + 1]), f2, n2), w = make_float2(ex2(e.x), ex2(e.y));
                             sum[i & 1] = __fadd2_rn(sum[i & 1], w);
                             if constexpr (C::kP == 3) {
                                 uint32_t part[3];
                                 cut3(w.x, w.y, part);
 #pragma unroll
-                                for (int k = 0; k < 3; ++k) p[k][i] = part[k];
+                                for (int k = 0; k < 3; ++k) p[C::kP == 3 ? k : 0][i] = part[k];
                             } else {
                                 p[0][i] = pack2<VT>(w.x, w.y);
-                                if constexpr (C::kP == 2) p[1][i] = pack2_rest(w.x, w.y, p[0][i]);
+                                p[C::kP - 1][i] = pack2_rest(w.x, w.y, p[0][i]);
                             }
                         }
+                        if (C::kP == 2 && h == 0 && !add_product(fix, raise)) return false;
 #pragma unroll
-                        for (int k = 0; k < C::kP; ++k) {
-                            if constexpr (W == 16)
-                                tmem_st16(p_t + C::kPCols / C::kP * k + W * h, p[k]);
-                            else
-                                tmem_st32(p_t + W * h, p[k]);
-                        }
+                        for (int k = 0; k < C::kP; ++k) tmem_st16(p_t + 32 * k + 16 * h, p[k]);
                     }
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     wait_st();
                     fence_before();
                     __syncwarp();
                     if (lane == 0) bar_arrive(p_full + 8 * x);
                     ++done;
+                    left = 1;
+                    if (last) break;
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 return true;
             };
-            // the last block may go by halves; in a loop of its own, since a branch
-            // within the loop cost a long prompt another 1 to 4 per cent
-            const bool half = C::kQ == 1 && end > it.b0 && me.half(end - 1);
-            const int full = end - (half ? 1 : 0);
+            if constexpr (C::kQ == 2) {
+#pragma unroll
+                for (float &y : o_sum) y = 0.f;
 #pragma unroll 1
-            for (int b = it.b0; ok && b < full; ++b) ok = block(b, std::integral_constant<int, 128>{});
-            if constexpr (C::kQ == 1)
+                for (int b = it.b0; ok && b < end; ++b) ok = block_by_halves(b);
+            } else {
+                // the last block may go by halves; in a loop of its own, since a branch
+                // within the loop cost a long prompt another 1 to 4 per cent
+                const bool half = end > it.b0 && me.half(end - 1);
+                const int full = end - (half ? 1 : 0);
+#pragma unroll 1
+                for (int b = it.b0; ok && b < full; ++b) ok = block(b, std::integral_constant<int, 128>{});
                 if (ok && half) ok = block(end - 1, std::integral_constant<int, 64>{});
+            }
             if (!ok) break;
             if (me.tokens == 0) continue;
             const bool any = end > it.b0;  // this segment holds blocks of this tile
             if (any) {
-                if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
-                fence_after();
+                if constexpr (C::kQ == 2) {
+                    if (!(ok = add_product(1.f, false))) break;
+                    if constexpr (C::kSum == 0) {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 32) tmem_st32(o_t + c, (const uint32_t *)(o_sum + kAt(c)));
+                    }
+                    wait_st();
+                } else {
+                    if (!(ok = warp_wait(pv_done + 8 * x, (done - 1) & 1))) break;
+                    fence_after();
+                }
             }
             if (it.b0 > 0 || b1 < it.blocks) {
-                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, number, again + warp);
+                tc_join<T, KT, D>(a, plan, it, begin.deal, x, o_t + C::kSum, TcRow{m, l, keys, token_row, head, row, any}, partials, flags, number, again + warp);
             } else {
-                tc_store<T, KT, D>(a, o_t, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, again + warp);
+                tc_store<T, KT, D>(a, o_t + C::kSum, keys <= 0 ? 0.f : 1.f / l, row ? token_row : -1, head, again + warp);
             }
             fence_before();
         }
@@ -1056,17 +1170,23 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                     end[x] = min(b1, me.blocks);
                     half[x] = me.half(end[x] - 1);
                 }
-                if constexpr (C::kV == 3) {
+                constexpr uint32_t rows64 = 64 * 128 >> 4;
+                if constexpr (C::kQ == 2) {
+                    // f32: a product for each 64 keys
                     int upto[2] = {0, 0};
 #pragma unroll
                     for (int x = 0; x < kTcSubs; ++x) upto[x] = TcSub(plan, it, x).halves(b1);
-                    for (int g = 2 * it.b0; ok && g < max(upto[0], upto[1]); ++g) {
-                        // 64 keys: their values' three parts, a slot each
+                    for (int g = 2 * it.b0; ok && g < (C::kV == 3 ? max(upto[0], upto[1]) : 2 * b1); ++g) {
                         uint64_t vb[3];
                         const int left = it.q.keys - 64 * g;
                         uint32_t at[3];
+                        if constexpr (C::kV == 1) {
+                            if ((g & 1) == 0 && !(ok = warp_wait(v_full + 8 * slot, phase))) break;
+                            vb[0] = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kVTile, C::kHalf) + (g & 1) * rows64;
+                        }
+                        // the values' three parts, a slot each
 #pragma unroll
-                        for (int c = 0; c < 3; ++c) {
+                        for (int c = 0; c < (C::kV == 3 ? 3 : 0); ++c) {
                             if (!ok || !(ok = warp_wait(v_full + 8 * slot, phase))) continue;
                             at[c] = slot;
                             const uint32_t to = v_s + __shfl_sync(kFull, slot, 0) * C::kVTile;
@@ -1089,22 +1209,31 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                             if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
                             p_phase[x] ^= 1;
                             fence_after();
-                            // the products of part c of the values and k of the weights above 2^-24, small ones first
                             const uint32_t pt = tm + C::p_col(x), ot = tm + C::o_col(x);
-                            mma_ts64(ot, pt + 64u, vb[0], kId, g != 2 * it.b0);
-                            mma_ts64(ot, pt + 32u, vb[1], kId, 1u);
-                            mma_ts64(ot, pt, vb[2], kId, 1u);
-                            mma_ts64(ot, pt + 32u, vb[0], kId, 1u);
-                            mma_ts64(ot, pt, vb[1], kId, 1u);
+                            if constexpr (C::kV == 3) {
+                                // the products of the values' parts and the weights' above 2^-24, small ones first
+                                mma_ts64(ot, pt + 64u, vb[0], kId, 0u);
+                                mma_ts64(ot, pt + 32u, vb[1], kId, 1u);
+                                mma_ts64(ot, pt, vb[2], kId, 1u);
+                                mma_ts64(ot, pt + 32u, vb[0], kId, 1u);
+                                mma_ts64(ot, pt, vb[1], kId, 1u);
+                            } else {
+                                mma_ts64(ot, pt + 32u, vb[0], kId, 0u);
+                            }
                             mma_ts64(ot, pt, vb[0], kId, 1u);
                             commit(pv_done + 8 * x);
                         }
                         if (!ok) break;
+                        if constexpr (C::kV == 3) {
 #pragma unroll
-                        for (int c = 0; c < 3; ++c) commit(v_empty + 8 * at[c]);
+                            for (int c = 0; c < 3; ++c) commit(v_empty + 8 * at[c]);
+                        } else if (g & 1) {
+                            commit(v_empty + 8 * slot);
+                            step();
+                        }
                     }
                 }
-                for (int b = it.b0; C::kV == 1 && b < b1; ++b) {
+                for (int b = it.b0; C::kQ == 1 && b < b1; ++b) {
                     if (!(ok = warp_wait(v_full + 8 * slot, phase))) break;
                     const uint64_t vb = desc_mn(v_s + __shfl_sync(kFull, slot, 0) * C::kVTile, C::kHalf);
 #pragma unroll
@@ -1113,13 +1242,10 @@ tc_attention_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
                         if (!(ok = warp_wait(p_full + 8 * x, p_phase[x]))) continue;
                         p_phase[x] ^= 1;
                         fence_after();
-                        constexpr uint32_t rows64 = 64 * 128 >> 4;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            if (C::kQ == 1 && h == 1 && b + 1 == end[x] && half[x]) break;
-                            const uint32_t pt = tm + C::p_col(x) + 32u * h;
-                            mma_ts64(tm + C::o_col(x), pt, vb + h * rows64, kId, h != 0 || b != it.b0);
-                            if constexpr (C::kQ == 2) mma_ts64(tm + C::o_col(x), pt + 64u, vb + h * rows64, kId, 1u);
+                            if (h == 1 && b + 1 == end[x] && half[x]) break;
+                            mma_ts64(tm + C::o_col(x), tm + C::p_col(x) + 32u * h, vb + h * rows64, kId, h != 0 || b != it.b0);
                         }
                         commit(pv_done + 8 * x);
                     }

@@ -195,3 +195,57 @@ def test_queries_and_keys_of_any_size(qmv, heads, kv_heads, d, exponent):
     b.run_packed()
     b.check(True)
     assert rms_of(b, True) <= 1.0
+
+
+# ------------------------------------------------- sums over many keys in f32
+
+def _rows_near(b, packed, s, rows):
+    """Some rows of sequence s: the norm of their error against that of the row.
+
+    With values about 1 the sums all have one sign, so that additions that cut
+    towards zero show: they cost 2^-24 of the sum each, 2^-13 over 16000 keys in
+    steps of 16.  What is allowed: 2^-21 for weights and values in parts; a
+    product of 64 keys by itself, 4 additions of its large parts and 20 of parts
+    that are 2^-7 of them, each cut by 2^-23 of the sum so far, (4 + 20 2^-7) 2^-23;
+    the sum of the products, rounded by half of 2^-23 each, independently:
+    sqrt(n / 16) 2^-24 (decode adds one for each 16 keys); the scores as in
+    model()."""
+    torch.cuda.synchronize()
+    k, v = b.kv_of(s, packed)
+    a, n = sum(b.new[:s]), b.new[s]
+    worst = 0.0
+    for r in rows:
+        keys = k.shape[0] - n + r + 1
+        q = b.q[a + r:a + r + 1].double().view(1, b.heads, b.d)
+        out, _, _ = model(q, k[:keys], v[:keys], 1.0 / math.sqrt(b.d))
+        c = ((q ** 2).mean() * (k[:keys] ** 2).mean()).sqrt()  # a middling c_j of model()
+        bound = 2.0 ** -21 + (4 + 20 * 2.0 ** -7) * 2.0 ** -23 + math.sqrt(keys / 16) * 2.0 ** -24 + math.sqrt(3 * b.d / 16) * 2.0 ** -22 * float(c)
+        got = b.out[a + r:a + r + 1].double().view_as(out)
+        worst = max(worst, float((got - out).norm() / out.norm()) / bound)
+    return worst
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 2, 64), (16, 2, 128)])
+def test_sums_of_long_prompts(qmv, heads, kv_heads, d):
+    b = Batch(qmv, "f32", heads, kv_heads, d, [16384])
+    b.v.mul_(0.25).add_(1.0)
+    b.run_packed()
+    assert _rows_near(b, True, 0, [0, 100, 999, 4000, 8100, 12345, 16383]) <= 1.0
+
+
+@pytest.mark.parametrize("heads,kv_heads,d", [(16, 2, 64), (16, 2, 128)])
+def test_sums_of_chunks_over_long_contexts(qmv, heads, kv_heads, d):
+    b = Batch(qmv, "f32", heads, kv_heads, d, [2048], [32768], page=64, poison=False)
+    b.values.mul_(0.25).add_(1.0)
+    b.run_paged()
+    assert _rows_near(b, False, 0, [0, 5, 1000, 2047]) <= 1.0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_sums_of_decode_over_long_contexts(qmv, d):
+    """Enough sequences that no CTA's part of one is short."""
+    b = Batch(qmv, "f32", 16, 8, d, [1] * 64, [16000] * 62 + [1000, 100], page=64, poison=False)
+    b.values.mul_(0.25).add_(1.0)
+    b.run_paged()
+    for s in (0, 30, 62, 63):
+        assert _rows_near(b, False, s, [0]) <= 1.0
