@@ -397,7 +397,9 @@ int qmv_qwen2_forward_profiled(QmvQwen2 *decoder, int token, float *logits, int 
  * weights meet f16 pages in pairs of f16 (22 bits for weights down to 2^-17 of
  * the row's largest, 2^-39 of that below), and f32 values, which keep 24 bits
  * from 1e-30 on wherever they stand, with 24 bits.  A single f16 weight keeps
- * its 11 bits down to 2^-27 of the row's largest.
+ * its 11 bits down to 2^-27 of the row's largest.  f32 outputs are summed in f32;
+ * 16-bit ones in the tensor cores, which cut each addition of 16 keys' products
+ * at the 24th bit of the sum (about 2^-25 n / 16 of the output for n keys).
  *
  * Row starts, lengths and page tables are read on the device, so a captured
  * graph can be replayed after they change; the counts passed by the host stay.
